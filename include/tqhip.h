@@ -55,7 +55,9 @@ extern "C" {
 #define TQHIP_ELAUNCH (-4)      /* the kernel launch failed */
 #define TQHIP_EFILE (-5)        /* a .tqwen file was unreadable, invalid or of an unsupported kind */
 #define TQHIP_EHIP (-6)         /* a HIP allocation or copy failed */
-#define TQHIP_ENOSCRATCH (-7)   /* tqhip_matmul_i4_noalloc_dev: the call needs more than the static scratch */
+#define TQHIP_ENOSCRATCH (-7)   /* tqhip_matmul_i4_noalloc_dev: the call needs more than the static scratch; the calls
+                                   of section 2b: the workspace given is too small, or none was given under the
+                                   caller's own stream capture */
 
 /* ---- 1. host-pointer entry points (the "hip" variants) ------------------ */
 
@@ -169,6 +171,129 @@ int tqhip_biip_rotate_dev(const float *x, float *y, int dim, const float *scale,
 int tqhip_matvec_i4_generic_dev(const uint8_t *w, const float *x, float *y, int out_dim, int in_dim,
                                 int group_size, void *stream);
 
+/* ---- 2b. a batch of requests between the projections ---------------------
+ * The reference serves one sequence, a token at a time, out of one contiguous cache
+ * (runtime/qwen_forward_token.cpp:401-458, kernels/attention/attention_decode_ref.cpp); these
+ * calls serve many requests at once, each with its own number of new tokens, on device
+ * buffers like the _dev calls above: asynchronous on `stream`, status codes, no aborts. The
+ * stream has to be one of the current device. The structs are read during the call.
+ *
+ * Types: activations f32 (what the projections above read and write), or f16 / bf16; the
+ * cache f32 / f16 / bf16. Arithmetic, norms and softmax statistics are in fp32, angles in
+ * fp64; results are rounded once, to nearest even. */
+#define TQHIP_F32 0
+#define TQHIP_F16 1
+#define TQHIP_BF16 2
+
+/* The query, key and value heads of a batch of tokens as the projections leave them. Head h
+ * of token t is at pointer + t * stride + h * head_dim elements; a stride of 0 stands for
+ * heads * head_dim. Each element becomes, in this order, x + bias (where given), for q and k
+ * x * w / sqrt(mean over the head of x^2 + eps) (where a norm is given), and the rotation of
+ * the pairs (i, i + rotary_dim / 2), i < rotary_dim / 2 (rope_ref, kernels/rope/rope_ref.cpp)
+ * by position * theta^(-2i / rotary_dim), or position * inv_freq[i]; elements past rotary_dim
+ * are not rotated, and v is neither normed nor rotated. */
+typedef struct tqhip_head_proj {
+    int dtype;                       /* of q, k, v, q_out and k_out: TQHIP_F32 / F16 / BF16 */
+    int n_tokens, n_heads, n_kv_heads;
+    int head_dim;                    /* even, 2 to 512 */
+    int rotary_dim;                  /* even, 0 (no rotation) to head_dim */
+    const void *q, *k, *v;
+    void *q_out, *k_out;             /* may be q and k themselves, with their strides */
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    const float *q_bias, *k_bias, *v_bias;   /* [heads * head_dim] or NULL */
+    const float *q_norm, *k_norm;            /* [head_dim] or NULL */
+    float eps;
+    double theta;                    /* > 0 where there is a rotation without inv_freq */
+    const float *inv_freq;           /* [rotary_dim / 2] or NULL */
+    const int *positions;            /* [n_tokens], >= 0 */
+} tqhip_head_proj;
+
+/* A paged cache. Row r of page p holds, for key/value head h, head_dim elements at
+ * p * page_stride + r * token_stride + h * head_stride; all three strides 0 stand for
+ * [n_pages][page_size][n_kv_heads][head_dim]. */
+typedef struct tqhip_kv_cache {
+    void *k, *v;
+    int dtype;
+    int n_pages, page_size, n_kv_heads, head_dim;
+    int64_t page_stride, token_stride, head_stride;
+} tqhip_kv_cache;
+
+/* A ragged batch of sequences. Tokens q_start[b] .. q_start[b + 1] - 1 of the call belong to
+ * sequence b (any number, none included); they are its last ones: with n of them, token i is
+ * at position kv_len[b] - n + i, and kv_len counts them. Position p of sequence b is in row
+ * p % page_size of page block_table[b * table_stride + p / page_size]. Tokens of no sequence
+ * (before q_start[0], from q_start[n_seqs] on) keep their outputs as they were; so do tokens
+ * at negative positions in kv_append. A position whose page number is outside
+ * [0, n_pages), or past the table's table_stride entries, does not exist: it is neither
+ * written nor attended to. */
+typedef struct tqhip_seqs {
+    int n_seqs, n_tokens;
+    const int *q_start;              /* device, [n_seqs + 1], not decreasing */
+    const int *kv_len;               /* device, [n_seqs] */
+    const int *block_table;          /* device, [n_seqs][table_stride] */
+    int table_stride;
+    int max_kv;                      /* the largest kv_len, or 0 where the host does not know it: decides how
+                                        the work is split, never what is computed */
+} tqhip_seqs;
+
+/* q -> q_out and k -> k_out (either pair may be NULL) at proj->positions; v is not read. */
+int tqhip_qk_norm_rope_dev(const tqhip_head_proj *proj, void *stream);
+
+/* k and v into the cache rows of their tokens' positions, k finished as above; q -> q_out in the
+ * same launch where both are given. The rotation takes proj->positions, or the cache positions
+ * where that is NULL. k_out is not used. Two tokens of a call must not fall on one row. */
+int tqhip_kv_append_dev(const tqhip_head_proj *proj, const tqhip_kv_cache *cache, const tqhip_seqs *seqs,
+                        void *stream);
+
+/* Attention of the batch's tokens over their sequences' cached rows (their own among them):
+ * query head h reads key/value head h / (n_heads / n_kv_heads). causal: position p attends to
+ * positions <= p, with window > 0 to the last `window` of those; otherwise to all kv_len. A
+ * token that may attend to nothing gets zeros. head_dim 64, 128 or 256; f16 / bf16 activations
+ * take a cache of their own type, f32 activations any; q, out and the cache 16-byte aligned,
+ * their strides multiples of 16 bytes. The keys and values of positions that are masked are
+ * never used, whatever they hold (NaN and infinities too).
+ *
+ * workspace: NULL takes the stream's scratch (grown on demand like that of the other calls); a
+ * caller that captures the call itself gives device memory of tqhip_paged_attention_workspace()
+ * bytes, 256-byte aligned, which no other launch may use at the same time. */
+typedef struct tqhip_attn {
+    int dtype;                       /* of q and out */
+    int n_heads;
+    const void *q;                   /* token t's head h at t * q_stride + h * head_dim (0: n_heads * head_dim) */
+    void *out;
+    int64_t q_stride, out_stride;
+    float scale;                     /* of q . k, usually 1 / sqrt(head_dim) */
+    int causal, window;
+    void *workspace;
+    size_t workspace_bytes;
+} tqhip_attn;
+int tqhip_paged_attention_dev(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs,
+                              void *stream);
+/* Bytes of workspace that call needs (0: none), from the host's numbers alone. */
+size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs);
+
+/* The low-rank adapters of many requests, beside the projection that they share:
+ * y_t = base_t + scale[a] * B_a (A_a x_t), a = adapter[b] of the sequence b that token t is in.
+ * Tokens of no sequence, and those whose adapter is outside [0, n_adapters) (-1: none), get
+ * base_t. x is [n_tokens][in_dim] and base / y [n_tokens][out_dim], as matmul_i4 reads and
+ * writes them; base may be y, or NULL for zeros. An adapter of a lower rank has zero rows.
+ * rank 1 to 256. workspace: as for the attention, tqhip_lora_workspace() bytes. */
+typedef struct tqhip_lora {
+    int dtype;                       /* of a and b: TQHIP_F32 / F16 / BF16 */
+    int n_tokens, in_dim, out_dim, rank, n_adapters, n_seqs;
+    const float *x, *base;
+    float *y;
+    const void *a;                   /* [n_adapters][rank][in_dim] */
+    const void *b;                   /* [n_adapters][out_dim][rank] */
+    const float *scale;              /* device, [n_adapters] */
+    const int *q_start;              /* device, [n_seqs + 1], not decreasing */
+    const int *adapter;              /* device, [n_seqs] */
+    void *workspace;
+    size_t workspace_bytes;
+} tqhip_lora;
+int tqhip_lora_add_dev(const tqhip_lora *lora, void *stream);
+size_t tqhip_lora_workspace(const tqhip_lora *lora);
+
 /* ---- 3. registry (kernels/dispatch.h:155-159, 191-195; set_matmul_i4_impl_by_name is new) */
 
 int tqhip_set_matvec_i4_impl_by_name(const char *name);   /* 1 = selected, 0 = unknown name */
@@ -238,6 +363,11 @@ typedef struct tqhip_op {
 #define TQHIP_OP_BIIP_ROTATE 6   /* x -> y, in_dim = dim, group_size = block_size, w2 = scale (or NULL), w3 = sign */
 #define TQHIP_OP_I4_SET 7        /* w = const tqhip_i4_mat * (n matrices, read when the op runs or is captured), group_size */
 #define TQHIP_OP_VQ2_SET 8       /* w = const tqhip_i4_mat * (n VQ2 matrices, read when the op runs or is captured) */
+/* The calls of section 2b; their structs are read when the op runs or is captured. */
+#define TQHIP_OP_QK_NORM_ROPE 9  /* w = const tqhip_head_proj * */
+#define TQHIP_OP_KV_APPEND 10    /* w = const tqhip_head_proj *, w2 = const tqhip_kv_cache *, w3 = const tqhip_seqs * */
+#define TQHIP_OP_PAGED_ATTENTION 11  /* w = const tqhip_attn *, w2 = const tqhip_kv_cache *, w3 = const tqhip_seqs * */
+#define TQHIP_OP_LORA_ADD 12     /* w = const tqhip_lora * */
 int tqhip_run_ops(const tqhip_op *ops, int n_ops, int repeats, void *stream);
 /* As tqhip_run_ops, with a HIP event pair around every call; op_ms[i] gets the
  * mean event-to-event time of call i over the repeats (kernel duration as the

@@ -1,0 +1,306 @@
+"""The batch calls on the GPU against plain 64-bit forms (batch_ref.py): heads normed and rotated, appended to a paged
+cache, attended to, and low-rank adapters, at the sizes, masks and layouts where each can go wrong.
+
+Tolerances. One rounding to a type is off by at most half a step (HALF). In fp32 u = 2^-24:
+heads: a result is made of two normed values, each a sum (1 u), a root of a mean of up to 512 squares summed in a tree of
+depth <= 14 (at most 8 u after the root), two products (2 u), times a sine or cosine (within 4 u of its argument's: a rounded
+half-turn, pi u, and the function's own step), and added (2 u): 20 u of the size of its terms.
+attention: a score is D products and sums, at most (D + 4) u of the sum of their sizes, S; e^x multiplies its error, and the
+weights enter numerator and denominator: 2 (D + 4) u S; N weights and products summed: at most (N + 16) u each. So within
+(2 (D + 4) S + 2 N + 32) u of sum p |v|. f16 / bf16 activations: one rounding of the weights (a bf16 or f16 half step of
+sum p |v|) and one of the result. That bound is loose for fp32, where errors are random, so those results are held to a
+relative L2 distance of 2^-17 too: a lost 16-bit term of a score or weight is 2^-8 or 2^-11 of it.
+lora: K products and sums, then r, of the size of the terms: (K + r + 8) u at most, and 2^-18 of them in L2.
+"""
+import numpy as np
+import pytest
+
+import batch_ref as ref
+from batch_ref import HALF, TINY, Batch, Dev, ints
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = 0, 1, 2
+U = 2.0 ** -24
+
+
+def f32_buffer(gpu, x):
+    return None if x is None else gpu.DeviceBuffer.from_array(np.asarray(x, np.float32))
+
+
+def ptr(b):
+    return None if b is None else b.ptr
+
+
+def head_inputs(gpu, rng, T, Hq, Hk, D, act, bias, norm, packed=False):
+    """q, k, v as the projections leave them (one matrix when packed), and their biases and norms."""
+    s = {}
+    if packed:
+        x = Dev(gpu, rng.standard_normal((T, (Hq + 2 * Hk) * D)), act)
+        w = {0: 4, 1: 2, 2: 2}[act]
+        cut = {"q": (0, Hq), "k": (Hq, Hk), "v": (Hq + Hk, Hk)}
+        s["keep"] = x
+        for n, (at, h) in cut.items():
+            s[n] = (x.ptr + at * D * w, (Hq + 2 * Hk) * D, x.values[:, at * D:(at + h) * D].reshape(T, h, D))
+    else:
+        for n, h in (("q", Hq), ("k", Hk), ("v", Hk)):
+            x = Dev(gpu, rng.standard_normal((T, h, D)), act)
+            s["keep_" + n] = x
+            s[n] = (x.ptr, 0, x.values)
+    for n, h in (("q", Hq), ("k", Hk), ("v", Hk)):
+        b = rng.standard_normal(h * D).astype(np.float32) if bias else None
+        s[n + "_bias"] = (b, f32_buffer(gpu, b))
+        w = (1 + 0.2 * rng.standard_normal(D)).astype(np.float32) if norm and n != "v" else None
+        s[n + "_norm"] = (w, f32_buffer(gpu, w))
+    return s
+
+
+def proj_of(gpu, s, T, Hq, Hk, D, act, rotary, q_out, k_out=None, positions=None, eps=1e-6, theta=1e6, inv_freq=None):
+    return gpu.HeadProj(dtype=act, n_tokens=T, n_heads=Hq, n_kv_heads=Hk, head_dim=D, rotary_dim=rotary, q=s["q"][0], k=s["k"][0], v=s["v"][0],
+                        q_out=ptr(q_out), k_out=ptr(k_out), q_stride=s["q"][1], k_stride=s["k"][1], v_stride=s["v"][1],
+                        q_bias=ptr(s["q_bias"][1]), k_bias=ptr(s["k_bias"][1]), v_bias=ptr(s["v_bias"][1]), q_norm=ptr(s["q_norm"][1]),
+                        k_norm=ptr(s["k_norm"][1]), eps=eps, theta=theta, positions=ptr(positions), inv_freq=ptr(inv_freq))
+
+
+def check_heads(got, want, size, dtype, what):
+    bound = 20 * U * size + HALF[dtype] * np.abs(want) * (dtype != F32) + TINY[dtype]
+    bad = ~(np.abs(got - want) <= bound)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(got - want) / np.maximum(bound, 1e-300)):.2f} bounds"
+
+
+# Head widths on the vector path (4 to 32 lanes a head) and off it (odd pairs, 24, 80, 512), partial rotation, no rotation;
+# one token and more tokens than waves; one matrix of q, k and v; positions far out.
+HEADS = [
+    (1, 32, 8, 128, F32, False, True, 128, False), (3, 14, 2, 64, F32, True, False, 64, True), (5, 2, 1, 256, F32, False, True, 256, False),
+    (77, 4, 4, 32, F32, True, True, 16, False), (9, 3, 1, 24, F32, False, True, 24, False), (6, 2, 2, 80, F32, True, True, 80, False),
+    (2, 1, 1, 512, F32, False, True, 512, False), (4, 5, 1, 6, F32, True, True, 2, False), (31, 14, 2, 64, F16, False, True, 64, True),
+    (13, 32, 8, 128, BF16, True, True, 32, False), (2500, 7, 1, 128, F32, False, True, 128, True), (9, 2, 1, 256, BF16, False, False, 0, False),
+    (4, 3, 1, 2, F16, True, True, 2, False),
+]
+
+
+@pytest.mark.parametrize("T,Hq,Hk,D,act,bias,norm,rotary,packed", HEADS)
+def test_qk_norm_rope(gpu, T, Hq, Hk, D, act, bias, norm, rotary, packed):
+    rng = np.random.default_rng(T * 7 + D)
+    s = head_inputs(gpu, rng, T, Hq, Hk, D, act, bias, norm, packed)
+    pos = rng.integers(0, 150000, T)
+    pos[0] = 0
+    q_out, k_out = Dev(gpu, np.full((T, Hq, D), 7.0), act), Dev(gpu, np.full((T, Hk, D), 7.0), act)
+    d_pos = ints(gpu, pos)
+    gpu.qk_norm_rope_dev(proj_of(gpu, s, T, Hq, Hk, D, act, rotary, q_out, k_out, d_pos))
+    gpu.synchronize()
+    for n, out in (("q", q_out), ("k", k_out)):
+        want, size = ref.finish_heads(s[n][2], s[n + "_bias"][0], s[n + "_norm"][0], pos, rotary, 1e-6, 1e6)
+        check_heads(out.read(), want, size, act, n)
+
+
+def test_qk_norm_rope_in_place_one_side_and_strided_outputs(gpu):
+    T, Hq, Hk, D = 10, 6, 2, 64
+    rng = np.random.default_rng(5)
+    s = head_inputs(gpu, rng, T, Hq, Hk, D, F32, False, True)
+    pos = np.arange(T) * 1000
+    d_pos = ints(gpu, pos)
+    want_q, size_q = ref.finish_heads(s["q"][2], None, s["q_norm"][0], pos, D, 1e-6, 1e6)
+    want_k, size_k = ref.finish_heads(s["k"][2], None, s["k_norm"][0], pos, D, 1e-6, 1e6)
+    # q alone, into rows twice as far apart (the gap untouched)
+    wide = Dev(gpu, np.full((T, 2 * Hq, D), 3.0), F32)
+    p = proj_of(gpu, s, T, Hq, Hk, D, F32, D, wide, None, d_pos)
+    p.k, p.q_out_stride = None, 2 * Hq * D
+    gpu.qk_norm_rope_dev(p)
+    # k alone, in place
+    p = proj_of(gpu, s, T, Hq, Hk, D, F32, D, None, None, d_pos)
+    p.q, p.k_out = None, p.k
+    gpu.qk_norm_rope_dev(p)
+    gpu.synchronize()
+    got = wide.read()
+    check_heads(got[:, :Hq], want_q, size_q, F32, "strided q")
+    assert np.all(got[:, Hq:] == 3.0)
+    check_heads(s["keep_k"].read(), want_k, size_k, F32, "in-place k")
+
+
+def test_qk_norm_rope_frequencies_and_unaligned_rows(gpu):
+    T, Hq, Hk, D = 7, 2, 1, 64
+    rng = np.random.default_rng(6)
+    inv = (1e4 ** (-np.arange(D // 2) / (D // 2)) / 8).astype(np.float32)
+    pos = rng.integers(0, 1000000, T)
+    d_pos, d_inv = ints(gpu, pos), f32_buffer(gpu, inv)
+    x = Dev(gpu, rng.standard_normal((T, Hq * D + 1)), F32)  # rows of an odd number of elements, from the second one on
+    out = Dev(gpu, np.full((T, Hq, D), 7.0), F32)
+    gpu.qk_norm_rope_dev(gpu.HeadProj(dtype=F32, n_tokens=T, n_heads=Hq, n_kv_heads=Hk, head_dim=D, rotary_dim=D, q=x.ptr + 4, q_out=out.ptr,
+                                      q_stride=Hq * D + 1, inv_freq=d_inv.ptr, positions=d_pos.ptr))
+    gpu.synchronize()
+    flat = np.concatenate([x.values.reshape(-1)[1:], [0.0]])
+    q = np.stack([flat[t * (Hq * D + 1):t * (Hq * D + 1) + Hq * D] for t in range(T - 1)] + [flat[(T - 1) * (Hq * D + 1):][:Hq * D]]).reshape(T, Hq, D)
+    want, size = ref.finish_heads(q, None, None, pos, D, 0, 0, inv)
+    check_heads(out.read()[:T - 1], want[:T - 1], size[:T - 1], F32, "inv_freq")
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)])
+@pytest.mark.parametrize("Hq,Hk,D,page,layout", [(14, 2, 64, 48, "token"), (8, 2, 128, 16, "head"), (3, 1, 24, 7, "token")])
+def test_kv_append(gpu, act, cache, Hq, Hk, D, page, layout):
+    """Sequences with many, one and no new tokens, one with more tokens than positions, missing pages, tokens outside."""
+    new, kv = [5, 1, 0, 40, 3, 1], [5, 100, 33, 90, 2, 2 * page + 1]
+    b = Batch(gpu, new, kv, page, Hk, D, cache, seed=3, tail=2, lead=1, bad=[(3, 80 // page)], layout=layout)
+    T = b.tokens
+    s = head_inputs(gpu, b.rng, T, Hq, Hk, D, act, True, True)
+    before = b.k.read_bits(), b.v.read_bits()
+    q_out = Dev(gpu, np.full((T, Hq, D), 7.0), act)
+    gpu.kv_append_dev(proj_of(gpu, s, T, Hq, Hk, D, act, D, q_out), b.c, b.s)
+    gpu.synchronize()
+    at = b.token_positions()
+    pos = np.array([at.get(t, (0, 0))[1] for t in range(T)])
+    want_q, size_q = ref.finish_heads(s["q"][2], s["q_bias"][0], s["q_norm"][0], pos, D, 1e-6, 1e6)
+    want_k, size_k = ref.finish_heads(s["k"][2], s["k_bias"][0], s["k_norm"][0], pos, D, 1e-6, 1e6)
+    want_v, size_v = ref.finish_heads(s["v"][2], s["v_bias"][0], None, pos, 0, 0, 1)
+    got_q = q_out.read()
+    live = [t for t in at if at[t][1] >= 0]
+    dead = [t for t in range(T) if t not in live]
+    check_heads(got_q[live], want_q[live], size_q[live], act, "q")
+    assert dead and np.all(got_q[dead] == 7.0)
+    for dev, old, want, size, what in ((b.k, before[0], want_k, size_k, "k"), (b.v, before[1], want_v, size_v, "v")):
+        got, bits = b.rows(dev.read()), b.rows(dev.read_bits())
+        old = b.rows(old).copy()
+        written = 0
+        for t in live:
+            pl = b.place(*at[t])
+            if pl:
+                check_heads(got[pl], want[t], size[t], cache, f"{what} row {at[t]}")
+                old[pl] = bits[pl]
+                written += 1
+        assert 0 < written < len(live)  # (one page is missing)
+        assert np.array_equal(old, bits), f"{what}: rows outside the call's positions changed"
+
+
+def check_attention(gpu, b, act, Hq, causal, window, scale=None, q_std=1.5, stream=None, q_pad=0):
+    T, D = b.tokens, b.D
+    scale = D ** -0.5 if scale is None else scale
+    q = Dev(gpu, q_std * b.rng.standard_normal((T, Hq + q_pad, D)), act)
+    out = Dev(gpu, np.full((T, Hq + q_pad, D), 7.0), act)
+    gpu.paged_attention_dev(gpu.Attn(dtype=act, n_heads=Hq, q=q.ptr, out=out.ptr, scale=scale, causal=causal, window=window,
+                                     q_stride=(Hq + q_pad) * D, out_stride=(Hq + q_pad) * D), b.c, b.s, stream)
+    gpu.synchronize()
+    want, spread, score, live = ref.attention(b, q.values[:, :Hq], float(np.float32(scale)), causal, window)
+    got = out.read()
+    dead = np.setdiff1d(np.arange(T), live)
+    assert np.all(got[dead] == 7.0) and np.all(got[:, Hq:] == 7.0), "rows outside the call changed"
+    got = got[:, :Hq]
+    N = max(b.kv)
+    bound = (2 * (D + 4) * score + 2 * N + 32) * U * spread
+    if act != F32:
+        bound = bound + HALF[act] * (spread + np.abs(want)) + TINY[act]
+    bad = ~(np.abs(got - want) <= bound)[live]
+    assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.nanmax((np.abs(got - want) / np.maximum(bound, 1e-300))[live]):.2f} bounds"
+    if act == F32:
+        den = np.linalg.norm(want[live])
+        assert np.linalg.norm((got - want)[live]) <= 2.0 ** -17 * den
+
+
+TYPES = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
+SHAPES = [(14, 2, 64), (8, 2, 128), (2, 1, 256)]
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("Hq,Hk,D", SHAPES)
+def test_attention_single_tokens(gpu, act, cache, Hq, Hk, D):
+    """Lengths of zero (more tokens than positions), one, about a tile, and long ones; tokens outside every sequence."""
+    kv = [1, 0, 2, 31, 32, 33, 63, 64, 65, 700, 129, 1500]
+    b = Batch(gpu, [1] * len(kv), kv, 16, Hk, D, cache, seed=D, tail=2, lead=1)
+    check_attention(gpu, b, act, Hq, 1, 0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("Hq,Hk,D", SHAPES)
+def test_attention_chunks(gpu, act, cache, Hq, Hk, D):
+    """Chunks of 0, 1, a few and many tokens over caches that end inside a page, positions before the cache's first."""
+    b = Batch(gpu, [70, 1, 0, 5, 129, 4], [70, 90, 12, 300, 400, 2], 48, Hk, D, cache, seed=D + 1, tail=3, layout="head")
+    check_attention(gpu, b, act, Hq, 1, 0)
+
+
+@pytest.mark.parametrize("page", [1, 7, 40, 64, 1000])
+def test_attention_page_sizes(gpu, page):
+    b = Batch(gpu, [33, 1, 3], [200, 333, 70], page, 2, 64, F16, seed=page)
+    check_attention(gpu, b, F32, 6, 1, 0)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [90, 3, 1, 64]])
+@pytest.mark.parametrize("causal,window", [(0, 0), (1, 1), (1, 37), (1, 5000)])
+def test_attention_masks(gpu, new, causal, window):
+    b = Batch(gpu, new, [600, 77, 1, 64], 16, 1, 128, BF16, seed=window)
+    check_attention(gpu, b, F32, 4, causal, window)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [50, 64, 3]])
+def test_attention_missing_pages(gpu, new):
+    """Pages outside the cache hold no positions; a sequence of them alone gives zeros."""
+    b = Batch(gpu, new, [200, 64, 500], 32, 2, 64, F16, seed=4, bad=[(0, 0), (0, 3), (1, 0), (1, 1), (2, 5), (2, 15)])
+    check_attention(gpu, b, F32, 4, 1, 0)
+
+
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (5, 5), (20, 1), (33, 1), (64, 8)])
+def test_attention_head_groups(gpu, Hq, Hk):
+    b = Batch(gpu, [1, 9, 40], [130, 70, 41], 16, Hk, 64, F16, seed=Hq)
+    check_attention(gpu, b, F32, Hq, 1, 0)
+
+
+@pytest.mark.parametrize("new", [[1] * 3, [200] * 2])
+@pytest.mark.parametrize("cache", [F16, BF16, F32])
+def test_attention_large_scores(gpu, new, cache):
+    """Scores of hundreds, of either sign: one weight is near 1, the rest are tiny, and maxima move late."""
+    b = Batch(gpu, new, [400 + 17 * i for i in range(len(new))], 16, 1, 64, cache, seed=9)
+    check_attention(gpu, b, F32, 4, 1, 0, scale=1.0, q_std=12.0)
+
+
+@pytest.mark.parametrize("q_std", [1e-20, 1e5, 1e20])
+def test_attention_wide_range_queries(gpu, q_std):
+    """fp32 queries beyond fp16's range, brought back by the scale."""
+    b = Batch(gpu, [1, 70], [100, 200], 16, 2, 64, F16, seed=10)
+    check_attention(gpu, b, F32, 4, 1, 0, scale=float(np.float32(0.2 / q_std)), q_std=q_std)
+
+
+def test_attention_strided_queries_and_a_stream(gpu):
+    b = Batch(gpu, [1, 30, 1], [50, 60, 900], 16, 2, 128, BF16, seed=11)
+    check_attention(gpu, b, F32, 6, 1, 0, q_pad=3, stream=gpu.Stream())
+
+
+def test_attention_long_sequence_without_a_length_hint(gpu):
+    b = Batch(gpu, [1, 1, 20], [9000, 40, 3000], 16, 1, 64, F16, seed=12)
+    b.s.max_kv = 0
+    check_attention(gpu, b, F32, 7, 1, 0)
+
+
+LORA = [  # tokens of each request, adapters of each, K, M, rank
+    ([1], [0], 64, 5, 1), ([1] * 9, [0, 3, -1, 2, 2, 7, 1, 0, 3], 896, 130, 16), ([5, 0, 17, 40, 1, 3], [1, 0, 3, -1, 2, 1], 260, 33, 8),
+    ([70, 130], [2, 0], 516, 900, 64), ([33], [1], 100, 64, 3), ([3, 200], [0, 1], 1001, 257, 100), ([2, 2], [3, 1], 40, 30, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,adapter,K,M,r", LORA)
+def test_lora_add(gpu, dtype, new, adapter, K, M, r):
+    """Adapter 7 is outside the four: as none. Tokens before the first and after the last request get the base."""
+    rng = np.random.default_rng(K + M + r)
+    n, starts = 4, 1 + np.concatenate(([0], np.cumsum(new)))
+    T = int(starts[-1]) + 2
+    x, base = rng.standard_normal((T, K)).astype(np.float32), rng.standard_normal((T, M)).astype(np.float32)
+    a, b = Dev(gpu, rng.standard_normal((n, r, K)) / np.sqrt(K), dtype), Dev(gpu, 0.3 * rng.standard_normal((n, M, r)), dtype)
+    scale = rng.uniform(0.5, 2, n).astype(np.float32)
+    dx, db, ds, dst, dad = f32_buffer(gpu, x), f32_buffer(gpu, base), f32_buffer(gpu, scale), ints(gpu, starts), ints(gpu, adapter)
+    want, size = ref.lora(x.astype(np.float64), base.astype(np.float64), a.values, b.values, scale.astype(np.float64), starts, adapter, T)
+
+    def call(dbase, dy):
+        gpu.lora_add_dev(gpu.Lora(dtype=dtype, n_tokens=T, in_dim=K, out_dim=M, rank=r, n_adapters=n, n_seqs=len(new), x=dx.ptr, base=dbase, y=dy,
+                                  a=a.ptr, b=b.ptr, scale=ds.ptr, q_start=dst.ptr, adapter=dad.ptr))
+        gpu.synchronize()
+
+    def check(got, want, what):
+        got = got.reshape(T, M).astype(np.float64)
+        assert np.all(np.abs(got - want) <= (K + r + 8) * U * size), what
+        assert np.linalg.norm(got - want) <= 2.0 ** -18 * np.linalg.norm(size), what
+
+    dy = gpu.DeviceBuffer(4 * T * M)
+    call(db.ptr, dy.ptr)
+    check(dy.download(np.float32, T * M), want, "y = base + delta")
+    call(None, dy.ptr)
+    check(dy.download(np.float32, T * M), want - base, "y = delta")
+    call(db.ptr, db.ptr)
+    check(db.download(np.float32, T * M), want, "in place")

@@ -37,6 +37,8 @@ tqwen_synth = _load_sibling("tqwen_synth")
 OK, EBADSHAPE, EBADGROUP, ETOOLARGE, ELAUNCH, EFILE, EHIP, ENOSCRATCH = 0, -1, -2, -3, -4, -5, -6, -7
 NOALLOC_SCRATCH_BYTES = 16 << 20  # TQHIP_NOALLOC_SCRATCH_BYTES
 OP_I4_MATVEC, OP_VQ2_MATVEC, OP_I4_MATMUL, OP_I4_PAIR, OP_I4_QKV, OP_BIIP_ROTATE, OP_I4_SET, OP_VQ2_SET = 1, 2, 3, 4, 5, 6, 7, 8
+OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD = 9, 10, 11, 12
+F32, F16, BF16 = 0, 1, 2  # TQHIP_F32 / F16 / BF16
 
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _f32p = ctypes.POINTER(ctypes.c_float)
@@ -70,6 +72,52 @@ def set_op(mats: "ctypes.Array", group_size: int) -> Op:
 def vq2_set_op(mats: "ctypes.Array") -> Op:
     """A TQHIP_OP_VQ2_SET op over a tqhip_i4_mat array of VQ2 matrices; keep the array alive."""
     return Op(OP_VQ2_SET, ctypes.addressof(mats), None, None, 0, 0, len(mats), 0)
+
+
+_i64 = ctypes.c_int64
+
+
+class HeadProj(ctypes.Structure):
+    """tqhip_head_proj: the q / k / v heads of a batch of tokens, their biases, norms and rotation. Pointers are
+    device addresses (``DeviceBuffer.ptr``, a tensor's ``data_ptr()``); fields left out are NULL or 0."""
+    _fields_ = [(n, _i) for n in ("dtype", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "rotary_dim")] + \
+               [(n, _vp) for n in ("q", "k", "v", "q_out", "k_out")] + \
+               [(n, _i64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + \
+               [(n, _vp) for n in ("q_bias", "k_bias", "v_bias", "q_norm", "k_norm")] + \
+               [("eps", ctypes.c_float), ("theta", ctypes.c_double), ("inv_freq", _vp), ("positions", _vp)]
+
+
+class KvCache(ctypes.Structure):
+    """tqhip_kv_cache: a paged cache of keys and values."""
+    _fields_ = [("k", _vp), ("v", _vp)] + \
+               [(n, _i) for n in ("dtype", "n_pages", "page_size", "n_kv_heads", "head_dim")] + \
+               [(n, _i64) for n in ("page_stride", "token_stride", "head_stride")]
+
+
+class Seqs(ctypes.Structure):
+    """tqhip_seqs: a ragged batch of sequences and their pages."""
+    _fields_ = [("n_seqs", _i), ("n_tokens", _i), ("q_start", _vp), ("kv_len", _vp), ("block_table", _vp),
+                ("table_stride", _i), ("max_kv", _i)]
+
+
+class Attn(ctypes.Structure):
+    """tqhip_attn: the queries and outputs of an attention call, its mask and its workspace."""
+    _fields_ = [("dtype", _i), ("n_heads", _i), ("q", _vp), ("out", _vp), ("q_stride", _i64), ("out_stride", _i64),
+                ("scale", ctypes.c_float), ("causal", _i), ("window", _i), ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class Lora(ctypes.Structure):
+    """tqhip_lora: the low-rank adapters of the requests of a batch."""
+    _fields_ = [(n, _i) for n in ("dtype", "n_tokens", "in_dim", "out_dim", "rank", "n_adapters", "n_seqs")] + \
+               [(n, _vp) for n in ("x", "base", "y", "a", "b", "scale", "q_start", "adapter", "workspace")] + \
+               [("workspace_bytes", _sz)]
+
+
+def batch_op(kind: int, *structs) -> Op:
+    """An Op of one of the batch calls (OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD) over its
+    structs, in the order in which the call takes them; keep the structs alive while the op is used."""
+    at = [ctypes.addressof(s) for s in structs] + [None, None]
+    return Op(kind, at[0], None, None, 0, 0, 0, 0, at[1], at[2])
 
 
 class TensorInfo(ctypes.Structure):
@@ -110,6 +158,13 @@ _SIGS = {
     "tqhip_matvec_vq2_set_dev": (_i, [_vp, _i, _vp]),
     "tqhip_biip_rotate_dev": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp]),
     "tqhip_dequant_i4_rows_dev": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp]),
+    # a batch of requests between the projections
+    "tqhip_qk_norm_rope_dev": (_i, [ctypes.POINTER(HeadProj), _vp]),
+    "tqhip_kv_append_dev": (_i, [ctypes.POINTER(HeadProj), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _vp]),
+    "tqhip_paged_attention_dev": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _vp]),
+    "tqhip_paged_attention_workspace": (_sz, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs)]),
+    "tqhip_lora_add_dev": (_i, [ctypes.POINTER(Lora), _vp]),
+    "tqhip_lora_workspace": (_sz, [ctypes.POINTER(Lora)]),
     # registry
     "tqhip_set_ops_impl_by_name": (_i, [ctypes.c_char_p]),
     "tqhip_ops_impl_name": (ctypes.c_char_p, []),
@@ -462,6 +517,36 @@ def matmul_i4_noalloc_dev(w, x, y, M: int, K: int, N: int, group_size: int, stre
     device array (no allocation). Returns the status (ENOSCRATCH when the call needs more than
     NOALLOC_SCRATCH_BYTES)."""
     return int(lib().tqhip_matmul_i4_noalloc_dev(_ptr(w), _ptr(x), _ptr(y), M, K, N, group_size, _stream(stream)))
+
+
+# ---- a batch of requests between the projections ---------------------------------------------
+
+def qk_norm_rope_dev(proj: HeadProj, stream=None) -> None:
+    """q -> q_out and k -> k_out: biases, per-head RMSNorm and rotation at proj.positions."""
+    _check(lib().tqhip_qk_norm_rope_dev(proj, _stream(stream)), "tqhip_qk_norm_rope_dev")
+
+
+def kv_append_dev(proj: HeadProj, cache: KvCache, seqs: Seqs, stream=None) -> None:
+    """k (normed and rotated) and v into the sequences' pages; q -> q_out in the same launch where both are given."""
+    _check(lib().tqhip_kv_append_dev(proj, cache, seqs, _stream(stream)), "tqhip_kv_append_dev")
+
+
+def paged_attention_dev(attn: Attn, cache: KvCache, seqs: Seqs, stream=None) -> None:
+    """Attention of the batch's tokens over their sequences' pages."""
+    _check(lib().tqhip_paged_attention_dev(attn, cache, seqs, _stream(stream)), "tqhip_paged_attention_dev")
+
+
+def paged_attention_workspace(attn: Attn, cache: KvCache, seqs: Seqs) -> int:
+    return int(lib().tqhip_paged_attention_workspace(attn, cache, seqs))
+
+
+def lora_add_dev(lora: Lora, stream=None) -> None:
+    """y = base + scale[a] * B_a (A_a x) for the tokens of every request with an adapter a."""
+    _check(lib().tqhip_lora_add_dev(lora, _stream(stream)), "tqhip_lora_add_dev")
+
+
+def lora_workspace(lora: Lora) -> int:
+    return int(lib().tqhip_lora_workspace(lora))
 
 
 class Stream:

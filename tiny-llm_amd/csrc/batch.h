@@ -1,0 +1,123 @@
+// batch.h -- what the kernels of a batch of requests share (heads.hip, paged_attn.hip, lora.hip):
+// element types, the search of a token's sequence, positions to pages.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/tqhip.h"
+
+namespace tqhip {
+namespace {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+template <typename T, int N>
+using vec = T __attribute__((ext_vector_type(N)));
+
+inline int type_bytes(int dtype) { return dtype == TQHIP_F32 ? 4 : 2; }
+inline bool type_known(int dtype) { return dtype >= TQHIP_F32 && dtype <= TQHIP_BF16; }
+
+// N elements at p (aligned to their size) as floats, and floats rounded to nearest even at p.
+template <typename T, int N>
+__device__ inline void load_as_float(const T *p, float *out) {
+    const vec<T, N> v = *reinterpret_cast<const vec<T, N> *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = static_cast<float>(v[i]);
+}
+template <typename T, int N>
+__device__ inline void store_rounded(T *p, const float *in) {
+    vec<T, N> v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = static_cast<T>(in[i]);
+    *reinterpret_cast<vec<T, N> *>(p) = v;
+}
+
+// The last b < n with start[b] <= t, or -1, found by the 64 lanes of a wave together (all of them call
+// it with the same arguments): one load for up to 64 sequences, two for up to 4096, where a bisection
+// by one lane waits for 6 and 12 loads one after the other. Whatever the array holds, the result is
+// in range.
+__device__ inline int last_start_at_or_before(const int *start, int n, int t) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    for (;;) {
+        const int step = (n + 63) / 64;
+        const int i = lane * step;
+        const bool in = i < n && start[lo + i] <= t;
+        const int c = __popcll(__ballot(in));
+        if (c == 0) return lo - 1;  // (only in the first round for an increasing array: lo = 0)
+        lo += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+        if (step == 1) return lo;
+    }
+}
+
+// Division of 0 <= n < 2^31 by a fixed d >= 1 as a multiplication (Granlund and Montgomery, Division by
+// Invariant Integers using Multiplication, 1994): with s = ceil(log2 d) and
+// m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(m, n) + n) >> s; the sum stays below 2^32.
+struct FastDiv {
+    uint32_t m, s, d;
+    explicit FastDiv(uint32_t div) : m(0), s(0), d(div) {
+        while ((uint64_t{1} << s) < d) ++s;
+        m = static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << s) - d)) / d + 1);
+    }
+    __device__ inline int quot(int n) const {
+        return static_cast<int>((__umulhi(m, static_cast<uint32_t>(n)) + static_cast<uint32_t>(n)) >> s);
+    }
+};
+
+// A paged cache and a batch's pages as the kernels take them (strides in elements).
+struct Pages {
+    const int *table;
+    int table_stride, n_pages;
+    FastDiv page_size;
+    int64_t page_stride, token_stride, head_stride;
+};
+
+// Element offset of position p of sequence b (head 0), or -1 where it does not exist.
+__device__ inline int64_t row_offset(const Pages &g, int b, int p) {
+    if (p < 0) return -1;
+    const int i = g.page_size.quot(p);
+    if (i >= g.table_stride) return -1;
+    const int page = g.table[static_cast<int64_t>(b) * g.table_stride + i];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(g.n_pages)) return -1;
+    return page * g.page_stride + (p - i * static_cast<int>(g.page_size.d)) * g.token_stride;
+}
+
+// The cache's strides with the contiguous layout for zeros; false: not a layout in which every row is apart.
+inline bool cache_strides(const tqhip_kv_cache &c, int64_t *page, int64_t *token, int64_t *head) {
+    if (c.page_stride == 0 && c.token_stride == 0 && c.head_stride == 0) {
+        *head = c.head_dim;
+        *token = static_cast<int64_t>(c.n_kv_heads) * c.head_dim;
+        *page = *token * c.page_size;
+        return true;
+    }
+    *page = c.page_stride;
+    *token = c.token_stride;
+    *head = c.head_stride;
+    return *page > 0 && *token >= c.head_dim && *head >= c.head_dim;
+}
+
+// Checks of the cache and the batch that kv_append and paged_attention share.
+inline int check_cache(const tqhip_kv_cache &c, const tqhip_seqs &s) {
+    if (!c.k || !c.v || !type_known(c.dtype) || c.n_pages < 1 || c.page_size < 1 || c.n_kv_heads < 1 || c.head_dim < 1)
+        return TQHIP_EBADSHAPE;
+    if (s.n_seqs < 1 || s.n_tokens < 1 || !s.q_start || !s.kv_len || !s.block_table || s.table_stride < 1 || s.max_kv < 0)
+        return TQHIP_EBADSHAPE;
+    int64_t page, token, head;
+    if (!cache_strides(c, &page, &token, &head)) return TQHIP_EBADSHAPE;
+    // offsets are 64-bit; what has to fit 32 bits are the positions
+    if (static_cast<int64_t>(s.table_stride) * c.page_size > INT32_MAX) return TQHIP_ETOOLARGE;
+    return TQHIP_OK;
+}
+
+inline Pages make_pages(const tqhip_kv_cache &c, const tqhip_seqs &s) {
+    Pages g{s.block_table, s.table_stride, c.n_pages, FastDiv(static_cast<uint32_t>(c.page_size)), 0, 0, 0};
+    (void)cache_strides(c, &g.page_stride, &g.token_stride, &g.head_stride);
+    return g;
+}
+
+}  // namespace
+}  // namespace tqhip

@@ -526,6 +526,16 @@ static int launch_op(const tqhip_op &op, hipStream_t s) {
         case TQHIP_OP_BIIP_ROTATE:
             return launch_biip_rotate(op.x, op.y, op.in_dim, static_cast<const float *>(op.w2),
                                       static_cast<const float *>(op.w3), op.group_size, s);
+        case TQHIP_OP_QK_NORM_ROPE: return tqhip_qk_norm_rope_dev(static_cast<const tqhip_head_proj *>(op.w), s);
+        case TQHIP_OP_KV_APPEND:
+            return tqhip_kv_append_dev(static_cast<const tqhip_head_proj *>(op.w),
+                                       static_cast<const tqhip_kv_cache *>(op.w2),
+                                       static_cast<const tqhip_seqs *>(op.w3), s);
+        case TQHIP_OP_PAGED_ATTENTION:
+            return tqhip_paged_attention_dev(static_cast<const tqhip_attn *>(op.w),
+                                             static_cast<const tqhip_kv_cache *>(op.w2),
+                                             static_cast<const tqhip_seqs *>(op.w3), s);
+        case TQHIP_OP_LORA_ADD: return tqhip_lora_add_dev(static_cast<const tqhip_lora *>(op.w), s);
         default: return kBadShape;
     }
 }

@@ -128,6 +128,13 @@ int scratch_prefill(hipStream_t s, size_t bytes, void **ws) {
     return grow(*set, set->xws, bytes, size_t{1} << 20, false, s, ws);
 }
 
+// The prefill workspace for a call that takes the caller's own workspace too: under a capture that
+// no scope owns it is refused, because two graphs captured on one stream would share the buffer.
+int scratch_batch(hipStream_t s, size_t bytes, void **ws) {
+    if (!t_scope && capturing(s)) return kNoScratch;
+    return scratch_prefill(s, bytes, ws);
+}
+
 ScratchSet *scratch_set_new() { return new ScratchSet; }
 
 ScratchSet *scratch_set_fixed(void *xws, size_t xws_bytes) {

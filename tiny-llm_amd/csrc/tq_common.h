@@ -51,7 +51,7 @@ enum Status : int {
     kLaunchFailed = -4,  // hipGetLastError after the launch was not hipSuccess
     kBadFile = -5,       // a .tqwen file was unreadable, invalid or of an unsupported kind
     kHipFailed = -6,     // a HIP allocation or copy failed
-    kNoScratch = -7,     // the allocation-free entry point's static scratch is too small for the call
+    kNoScratch = -7,     // the allocation-free entry point's static scratch, or the caller's workspace, is too small
     kNotFused = 1,       // a fused path does not apply to these operands; nothing was launched
 };
 
@@ -167,6 +167,7 @@ int device_cu_count();
 struct ScratchSet;
 int scratch_split_slots(hipStream_t s, size_t nslots, unsigned long long **slots);
 int scratch_prefill(hipStream_t s, size_t bytes, void **ws);
+int scratch_batch(hipStream_t s, size_t bytes, void **ws);  // kNoScratch under the caller's own capture
 ScratchSet *scratch_set_new();
 ScratchSet *scratch_set_fixed(void *xws, size_t xws_bytes);
 void scratch_set_free(ScratchSet *set);  // the caller has synchronised every launch that used it
