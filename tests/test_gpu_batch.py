@@ -304,3 +304,35 @@ def test_lora_add(gpu, dtype, new, adapter, K, M, r):
     check(dy.download(np.float32, T * M), want - base, "y = delta")
     call(db.ptr, db.ptr)
     check(db.download(np.float32, T * M), want, "in place")
+
+
+@pytest.mark.parametrize("cache", [F16, BF16, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_masked_infinities_and_nan(gpu, cache, D):
+    """Rows of a chunk's later tokens hold infinities and NaN: the tokens before them must not notice, the ones that see
+    them must not be finite in the value's dimension."""
+    n, kv = 40, 150
+    b = Batch(gpu, [n, 1], [kv, 90], 16, 1, D, cache, seed=13)
+    rows = {}
+    for p, (where, x) in {120: ("v", np.inf), 133: ("k", np.nan), 140: ("v", np.nan), 149: ("v", -np.inf)}.items():
+        pg, r = b.place(0, p)
+        dev = b.v if where == "v" else b.k
+        full = dev.values
+        full[pg, r, 0, 5] = x
+        dev.buf.upload(ref.raw(full, cache)[0])
+        rows[p] = (where, x)
+    q = Dev(gpu, 1.5 * b.rng.standard_normal((b.tokens, 4, D)), F32)
+    out = Dev(gpu, np.full((b.tokens, 4, D), 7.0), F32)
+    gpu.paged_attention_dev(gpu.Attn(dtype=F32, n_heads=4, q=q.ptr, out=out.ptr, scale=D ** -0.5, causal=1), b.c, b.s)
+    gpu.synchronize()
+    got = out.read()
+    with np.errstate(invalid="ignore"):
+        want = ref.attention(b, q.values, float(np.float32(D ** -0.5)), 1, 0)[0]
+    first = kv - n  # position of token 0
+    clean = [t for t in range(n + 1) if t == n or first + t < 120]
+    assert np.linalg.norm(got[clean] - want[clean]) <= 2.0 ** -17 * np.linalg.norm(want[clean])
+    one = [t for t in range(n) if 120 <= first + t < 133]  # see the infinity in dimension 5 alone
+    keep = np.arange(D) != 5
+    assert np.linalg.norm((got - want)[one][..., keep]) <= 2.0 ** -17 * np.linalg.norm(want[one][..., keep])
+    assert not np.isfinite(got[one][..., 5]).any()
+    assert np.isnan(got[[t for t in range(n) if first + t >= 133]]).all()

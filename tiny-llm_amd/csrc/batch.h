@@ -108,8 +108,8 @@ inline int check_cache(const tqhip_kv_cache &c, const tqhip_seqs &s) {
         return TQHIP_EBADSHAPE;
     int64_t page, token, head;
     if (!cache_strides(c, &page, &token, &head)) return TQHIP_EBADSHAPE;
-    // offsets are 64-bit; what has to fit 32 bits are the positions
-    if (static_cast<int64_t>(s.table_stride) * c.page_size > INT32_MAX) return TQHIP_ETOOLARGE;
+    // offsets are 64-bit; what has to fit 32 bits, a tile's length to spare, are the positions
+    if (static_cast<int64_t>(s.table_stride) * c.page_size > INT32_MAX / 2) return TQHIP_ETOOLARGE;
     return TQHIP_OK;
 }
 

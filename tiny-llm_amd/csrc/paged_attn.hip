@@ -1,8 +1,10 @@
 // paged_attn.hip -- attention of the new tokens of a batch of sequences over their paged cache.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "batch.h"
+#include "lane_sum.h"
 #include "tq_common.h"
 
 namespace tqhip {
@@ -14,66 +16,499 @@ struct AttnArgs {
     int64_t q_stride, out_stride;
     const int *q_start, *kv_len;
     int n_seqs, n_tokens, n_heads, group;  // group: query heads per key/value head
-    float scale;
+    float scale;                           // |scale| * log2 e; the sign goes into q
+    float sign;
     int causal, window;
+    int parts, span;                       // parts of `span` keys, the last one to the end
+    float *part_o;                         // [n_tokens * n_heads][parts][head_dim], unnormalised
+    float2 *part_ml;                       // [n_tokens * n_heads][parts]: exponent bias, sum of weights
     Pages pages;
 };
 
-// One wave per token and query head, 64 keys at a time.
-template <typename T, typename C, int D>
-__global__ __launch_bounds__(64) void attn_simple(AttnArgs a) {
-    __shared__ float qs[D];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int b = last_start_at_or_before(a.q_start, a.n_seqs, t);
-    if (b < 0) return;
-    const int end = a.q_start[b + 1];
-    if (t >= end) return;
-    const int pos = a.kv_len[b] - (end - t), len = min(a.kv_len[b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
-    for (int d = lane; d < D; d += 64)
-        qs[d] = static_cast<float>((static_cast<const T *>(a.q) + t * a.q_stride + h * D)[d]) * a.scale;
-    __syncthreads();
-    const int hi = a.causal ? min(pos + 1, len) : len;
-    const int lo = a.causal && a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-    const C *kc = static_cast<const C *>(a.k) + h / a.group * a.pages.head_stride;
-    const C *vc = static_cast<const C *>(a.v) + h / a.group * a.pages.head_stride;
-    float m = -INFINITY, l = 0.0f, acc[D / 64] = {};
-    for (int j0 = lo; j0 < hi; j0 += 64) {
-        const int64_t row = j0 + lane < hi ? row_offset(a.pages, b, j0 + lane) : -1;
-        float s = -INFINITY;
-        if (row >= 0) {
-            s = 0.0f;
-            for (int d = 0; d < D; ++d) s += qs[d] * static_cast<float>(kc[row + d]);
-        }
-        float mx = s;
-        for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
-        const float mn = fmaxf(m, mx);
-        if (mn == -INFINITY) continue;
-        const float p = row >= 0 ? expf(s - mn) : 0.0f, f = expf(m - mn);
-        m = mn;
-        float sum = p;
-        for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-        l = l * f + sum;
-        for (int i = 0; i < D / 64; ++i) acc[i] *= f;
-        for (int j = 0; j < min(64, hi - j0); ++j) {
-            const int64_t r = __shfl(row, j);
-            const float pj = __shfl(p, j);
-            if (r < 0) continue;
-            for (int i = 0; i < D / 64; ++i) acc[i] += pj * static_cast<float>(vc[r + lane + 64 * i]);
+// ---- numbers as terms of 16 bits ----------------------------------------------------------------
+
+// How a product's operands are held: E the type of the matrix instruction, QT terms of a query element
+// or a weight, KT of a cache element. 16-bit activations meet a cache of their own type as they are.
+// fp32 activations keep their precision: against an fp16 cache two fp16 terms (22 bits), against
+// a bf16 one three bf16 terms (24 bits), and an fp32 cache is three bf16 terms itself.
+template <typename T, typename C>
+struct Terms {
+    using E = std::conditional_t<std::is_same_v<C, f16>, f16, bf16>;
+    static constexpr int KT = std::is_same_v<C, float> ? 3 : 1;
+    static constexpr int QT = std::is_same_v<T, C> && !std::is_same_v<C, float> ? 1 : std::is_same_v<C, f16> ? 2 : 3;
+    // products of term i and term j are kept while i + j < max(QT, KT): the next ones are below 2^-24
+    static constexpr int kMost = QT > KT ? QT : KT;
+};
+
+// x as N terms of 16 bits, the largest first: the last one rounded to nearest even, those before it so
+// that the rest is exact. bf16 terms before the last are cut off, which cannot overflow.
+template <typename E, int N>
+__device__ inline void split(const float *x, vec<E, 8> *out) {
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if (n == N - 1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) out[n][i] = static_cast<E>(r[i]);
+        } else if constexpr (std::is_same_v<E, bf16>) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned u = __float_as_uint(r[i]);
+                out[n][i] = __builtin_bit_cast(bf16, static_cast<unsigned short>(u >> 16));
+                const float cut = __uint_as_float(u & 0xffff0000u);
+                r[i] = r[i] == cut ? 0.0f : r[i] - cut;  // (an infinity is its first term)
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                out[n][i] = static_cast<E>(r[i]);
+                r[i] -= static_cast<float>(out[n][i]);
+            }
         }
     }
-    T *o = static_cast<T *>(a.out) + t * a.out_stride + h * D;
-    for (int i = 0; i < D / 64; ++i) o[lane + 64 * i] = static_cast<T>(l > 0.0f ? acc[i] / l : 0.0f);
+}
+
+using f32x16 = vec<float, 16>;
+__device__ inline f32x16 mfma32(vec<f16, 8> a, vec<f16, 8> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mfma32(vec<bf16, 8> a, vec<bf16, 8> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Four rows of 16 elements each, held 4 elements a lane by 16 lanes, as columns: lane i gets column i's four.
+template <typename E>
+__device__ inline vec<E, 4> lds_columns(const E *p) {
+    using raw = vec<short, 4>;
+    return __builtin_bit_cast(vec<E, 4>, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) raw *)p));
+}
+
+template <typename C>
+__device__ inline bool is_finite(C x) {
+    if constexpr (std::is_same_v<C, float>)
+        return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+    constexpr unsigned short kExp = std::is_same_v<C, f16> ? 0x7c00 : 0x7f80;
+    return (__builtin_bit_cast(vec<unsigned short, sizeof(C) / 2>, x)[0] & kExp) != kExp;
+}
+
+// Weights are 2^(s c + bias): with fp16 terms they are held 2^8 times larger, above fp16's subnormals.
+template <typename E>
+constexpr float kWeightShift = std::is_same_v<E, f16> ? 8.0f : 0.0f;
+
+// ---- the sequence and the rows of a tile -----------------------------------------------------------
+
+// Rows of a sequence with n new tokens: (token, head of the group), n * group of them. Tiles of BM rows
+// are numbered over the batch without a scan of the lengths: sequence b's start at
+// floor(start[b] group / BM) + b, which leaves room for ceil(n group / BM) of them.
+struct TileRows {
+    int b, first, n, r0, pos0, len;  // sequence, its first token, its tokens, the tile's first row, position of token 0, cached length
+};
+template <int BM>
+__device__ inline bool find_tile(const AttnArgs &a, int tile, TileRows &t) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.n_seqs;
+    const auto base = [&](int b) {
+        const int64_t s = min(max(a.q_start[b], 0), a.n_tokens);
+        return static_cast<int>(s * a.group / BM) + b;
+    };
+    for (;;) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const int c = __popcll(__ballot(i < n && base(lo + i) <= tile));
+        if (c == 0) return false;
+        lo += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+        if (step == 1) break;
+    }
+    const int end = min(max(a.q_start[lo + 1], 0), a.n_tokens);
+    t.b = lo;
+    t.first = min(max(a.q_start[lo], 0), a.n_tokens);
+    t.n = end - t.first;
+    t.r0 = (tile - base(lo)) * BM;
+    t.pos0 = a.kv_len[lo] - t.n;
+    t.len = min(a.kv_len[lo], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
+    return t.n > 0 && t.r0 < t.n * a.group;
+}
+
+// Keys [lo, hi) of the row's token at position p.
+__device__ inline int key_lo(const AttnArgs &a, int p) { return a.causal && a.window > 0 ? max(0, p + 1 - a.window) : 0; }
+__device__ inline int key_hi(const AttnArgs &a, int p, int len) { return a.causal ? min(p + 1, len) : len; }
+
+// ---- many rows: tiles of 128 rows ---------------------------------------------------------------
+// Bits below n (none for n <= 0, all from 32 on).
+__device__ inline unsigned below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// A chunk of 8 cache elements into the LDS planes of its terms.
+template <typename C, typename E, int KT, int BN, int STRIDE>
+__device__ inline void put_terms(const vec<C, 8> &x, E (*planes)[BN][STRIDE], int row, int at) {
+    if constexpr (KT == 1) {
+        *reinterpret_cast<vec<C, 8> *>(&planes[0][row][at]) = x;
+    } else {
+        float f[8];
+        vec<E, 8> terms[KT];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = x[e];
+        split<E, KT>(f, terms);
+#pragma unroll
+        for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&planes[n][row][at]) = terms[n];
+    }
+}
+
+template <typename T, typename C, int D>
+struct TileShape {
+    using Tm = Terms<T, C>;
+    static constexpr int BN = (D == 256 && Tm::QT > 1) || (D == 128 && Tm::QT == 3 && Tm::KT == 1) ? 32 : 64;
+    static constexpr int kWavesPerSimd = D == 256 || (D == 128 && Tm::KT == 3) ? 1 : 2;
+};
+
+constexpr int kTileRows = 128;
+
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn_tiles(AttnArgs a) {
+    using Tm = Terms<T, C>;
+    using E = typename Tm::E;
+    constexpr int QT = Tm::QT, KT = Tm::KT, BN = TileShape<T, C, D>::BN;
+    constexpr int NCH = BN * (D / 8) / 256;  // chunks of 8 elements per thread
+    constexpr int KS = D + 8, VS = D + 16;   // row strides: reads of 16 rows touch every bank once
+    constexpr int NK = BN / 32, ND = D / 32;
+    __shared__ __attribute__((aligned(16))) E ks[KT][BN][KS];
+    __shared__ __attribute__((aligned(16))) E vs[KT][BN][VS];
+    __shared__ int64_t offs[2][BN];
+    __shared__ unsigned long long here[2];  // which of the tile's keys exist
+    __shared__ unsigned long long wild[2];  // keys of a partly masked tile whose values are not all finite
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, col = lane & 31;
+    const int kv_heads = a.n_heads / a.group;
+    const int kvh = blockIdx.x % kv_heads;
+    const int tile = gridDim.x / kv_heads - 1 - static_cast<int>(blockIdx.x) / kv_heads;  // the longest first
+    TileRows t;
+    if (!find_tile<kTileRows>(a, tile, t)) return;
+    const int rows = t.n * a.group;
+    const int last = min(t.r0 + kTileRows, rows) - 1;
+    const int p_first = t.pos0 + t.r0 / a.group, p_last = t.pos0 + last / a.group;
+    int kb = key_lo(a, p_first), ke = key_hi(a, p_last, t.len);
+    if (a.parts > 1) {
+        kb = max(kb, static_cast<int>(blockIdx.y) * a.span);
+        if (static_cast<int>(blockIdx.y) < a.parts - 1) ke = min(ke, (static_cast<int>(blockIdx.y) + 1) * a.span);
+        // (a row without keys gets its zeros from the join; the first part writes nothing for it)
+        if (kb >= ke) return;
+    }
+    // keys that every row may attend to
+    const int full_lo = key_lo(a, p_last), full_hi = key_hi(a, p_first, t.len);
+
+    // this lane's row
+    const int wr0 = t.r0 + wave * 32;
+    const int r = min(wr0 + col, rows - 1);
+    const int token = t.first + r / a.group, head = kvh * a.group + r % a.group;
+    const int pos = t.pos0 + r / a.group;
+    const int lo = key_lo(a, pos), hi = key_hi(a, pos, t.len);
+    const bool wave_live = wr0 < rows;
+    const int wp_first = t.pos0 + min(wr0, rows - 1) / a.group, wp_last = t.pos0 + min(wr0 + 31, rows - 1) / a.group;
+    const int w_lo = key_lo(a, wp_first), w_hi = key_hi(a, wp_last, t.len);
+    const int wf_lo = key_lo(a, wp_last), wf_hi = key_hi(a, wp_first, t.len);
+
+    vec<E, 8> q[QT][D / 16];
+    float c = a.scale;
+    {
+        const T *qp = static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * h;
+        if constexpr (QT == 1) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                q[0][i] = *reinterpret_cast<const vec<E, 8> *>(qp + 16 * i);
+                if (a.sign < 0.0f) q[0][i] = -q[0][i];
+            }
+        } else {
+            float mx = 0.0f;
+            if constexpr (std::is_same_v<E, f16>) {  // the row scaled to fp16's range by a power of two
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    float x[8];
+                    load_as_float<T, 8>(qp + 16 * i, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+                }
+                mx = fmaxf(mx, lane_xor<32>(mx, lane));
+            }
+            int ex = 0;
+            if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
+            c = ldexpf(c, ex);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                float x[8];
+                load_as_float<T, 8>(qp + 16 * i, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], -ex) * a.sign;
+                vec<E, 8> terms[QT];
+                split<E, QT>(x, terms);
+#pragma unroll
+                for (int n = 0; n < QT; ++n) q[n][i] = terms[n];
+            }
+        }
+    }
+
+    const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride;
+    const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride;
+    vec<C, 8> kr[NCH], vr[NCH];
+    const auto load_tile = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int ch = tid + 256 * i;
+            const int64_t o = offs[buf][ch / (D / 8)];
+            kr[i] = vec<C, 8>{};
+            vr[i] = vec<C, 8>{};
+            if (o >= 0) {
+                kr[i] = *reinterpret_cast<const vec<C, 8> *>(kc + o + ch % (D / 8) * 8);
+                vr[i] = *reinterpret_cast<const vec<C, 8> *>(vc + o + ch % (D / 8) * 8);
+            }
+        }
+    };
+    const auto key_offset = [&](int key) { return tid < BN && key < ke ? row_offset(a.pages, t.b, key) : -1; };
+    const auto put_offset = [&](int buf, int64_t o) {
+        if (wave == 0) {
+            const unsigned long long m = __ballot(o >= 0);
+            if (tid < BN) offs[buf][tid] = o;
+            if (tid == 0) {
+                here[buf] = m;
+                wild[buf] = 0;
+            }
+        }
+    };
+
+    f32x16 acc[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[i] = f32x16{};
+    float m = -INFINITY, bias = 0.0f, l = 0.0f;
+
+    put_offset(0, key_offset(kb + tid));
+    __syncthreads();
+    if (kb < ke) load_tile(0);
+    int64_t next_off = key_offset(kb + BN + tid);
+    int buf = 0;
+    for (int k0 = kb; k0 < ke; k0 += BN, buf ^= 1) {
+        if (k0 != kb) __syncthreads();  // the last tile has been read
+        const bool partial = k0 < full_lo || k0 + BN > full_hi;  // some row of the block masks some key
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int ch = tid + 256 * i, row = ch / (D / 8), at = ch % (D / 8) * 8;
+            if (partial) {
+                // An infinite or NaN value would reach rows that mask its key through a product with their weight of zero.
+                // It goes into the products as zero and is added below where its key is seen.
+                bool finite = true;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!is_finite<C>(vr[i][e])) {
+                        finite = false;
+                        vr[i][e] = static_cast<C>(0.0f);
+                    }
+                if (!finite) atomicOr(&wild[buf], 1ull << row);
+            }
+            put_terms<C, E, KT, BN, KS>(kr[i], ks, row, at);
+            put_terms<C, E, KT, BN, VS>(vr[i], vs, row, at);
+        }
+        put_offset(buf ^ 1, next_off);
+        __syncthreads();
+        if (k0 + BN < ke) {
+            load_tile(buf ^ 1);
+            next_off = key_offset(k0 + 2 * BN + tid);
+        }
+        if (!wave_live || k0 >= w_hi || k0 + BN <= w_lo) continue;
+
+        // S^T: keys down, queries across; the lane holds its query's keys 32 kt + (i % 4) + 8 (i / 4) + 4 h
+        f32x16 s[NK];
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt) {
+            s[kt] = f32x16{};
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+                for (int kj = 0; kj < KT; ++kj) {
+                    const vec<E, 8> kf = *reinterpret_cast<const vec<E, 8> *>(&ks[kj][32 * kt + col][16 * i + 8 * h]);
+#pragma unroll
+                    for (int qi = 0; qi < QT; ++qi)
+                        if (qi + kj < Tm::kMost) s[kt] = mfma32(kf, q[qi][i], s[kt]);
+                }
+            }
+        }
+        const unsigned long long exist = here[buf];
+        const bool all_here = BN == 64 ? exist == ~0ull : (exist & 0xffffffffull) == 0xffffffffull;
+        if (k0 < wf_lo || k0 + BN > wf_hi || !all_here) {
+            // which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt) {
+                const int k1 = k0 + 32 * kt + 4 * h;
+                const unsigned may = static_cast<unsigned>(exist >> (32 * kt + 4 * h)) & below(hi - k1) & ~below(lo - k1);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[kt][i] = -INFINITY;
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+        mx = fmaxf(mx, lane_xor<32>(mx, lane));
+        if (__ballot(mx != m)) {  // a row's maximum moved: what is summed is brought down to the new one
+            const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
+            const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
+            m = mx;
+            bias = nb;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] *= f;
+        }
+#pragma unroll
+        for (int kt = 0; kt < NK; ++kt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kt][i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, bias));
+                l += s[kt][i];
+            }
+        }
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float x[8];
+                    vec<E, 8> p[QT];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = s[kt][8 * half + e];
+                    split<E, QT>(x, p);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+#pragma unroll
+                        for (int kj = 0; kj < KT; ++kj) {
+                            const E *v0 = &vs[kj][32 * kt + 16 * half + 4 * h + (lane & 15) / 4]
+                                             [32 * d + (lane & 16) + 4 * (lane & 3)];
+                            const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * VS);
+                            const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                            for (int qi = 0; qi < QT; ++qi)
+                                if (qi + kj < Tm::kMost) acc[d] = mfma32(vf, p[qi], acc[d]);
+                        }
+                    }
+                }
+        for (unsigned long long w = partial ? wild[buf] : 0; w; w &= w - 1) {
+            const int j = __builtin_ctzll(w), key = k0 + j;
+            if (key < lo || key >= hi) continue;
+            const C *v0 = vc + offs[buf][j] + 4 * h;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const C x = v0[32 * d + (e & 3) + 8 * (e >> 2)];
+                    if (!is_finite<C>(x)) acc[d][e] += static_cast<float>(x);
+                }
+        }
+    }
+    if (wr0 + col >= rows) return;
+    l += lane_xor<32>(l, lane);
+    if (a.parts > 1) {
+        const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts + blockIdx.y;
+        if (h == 0) a.part_ml[at] = make_float2(bias, l);
+        float *o = a.part_o + at * D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4 *>(o + 32 * d + 8 * g + 4 * h) =
+                    make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *o = static_cast<T *>(a.out) + token * a.out_stride + head * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[d][4 * g + e] * inv;
+            store_rounded<T, 4>(o + 32 * d + 8 * g + 4 * h, x);
+        }
+}
+
+// ---- the join of the parts ----------------------------------------------------------------------
+
+// One workgroup of 64 lanes per token and head: out = sum of parts 2^(least bias - bias) o / the same of l.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void attn_join(AttnArgs a) {
+    const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    const int b = last_start_at_or_before(a.q_start, a.n_seqs, token);
+    if (b < 0) return;
+    const int end = a.q_start[b + 1];
+    if (token >= end) return;
+    const int pos = a.kv_len[b] - (end - token);
+    const int len = min(a.kv_len[b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
+    const int lo = key_lo(a, pos), hi = key_hi(a, pos, len);
+    const int z0 = min(lo / a.span, a.parts - 1), z1 = hi > lo ? min((hi - 1) / a.span + 1, a.parts) : z0;
+    const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts;
+    float least = INFINITY;
+    for (int z = z0; z < z1; ++z) {
+        const float2 ml = a.part_ml[at + z];
+        if (ml.y != 0.0f) least = fminf(least, ml.x);
+    }
+    float acc[D / 64] = {}, l = 0.0f;
+    for (int z = z0; z < z1; ++z) {
+        const float2 ml = a.part_ml[at + z];
+        if (ml.y == 0.0f) continue;
+        const float f = exp2f(least - ml.x);
+        l += ml.y * f;
+        const float *o = a.part_o + (at + z) * D;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) acc[i] += o[lane + 64 * i] * f;
+    }
+    T *o = static_cast<T *>(a.out) + token * a.out_stride + head * D;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[lane + 64 * i] = static_cast<T>(l == 0.0f ? 0.0f : acc[i] / l);
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+// How the work is cut, from the host's numbers alone.
+struct Plan {
+    int tiles, parts, span;
+};
+
+Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
+    const int group = p.n_heads / c.n_kv_heads;
+    Plan n{};
+    n.tiles = static_cast<int>(static_cast<int64_t>(s.n_tokens) * group / kTileRows) + s.n_seqs;
+    const int64_t most = static_cast<int64_t>(s.table_stride) * c.page_size;
+    const int64_t kv = s.max_kv > 0 ? std::min<int64_t>(s.max_kv, most) : most;
+    const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads;
+    int64_t parts = std::max<int64_t>(1, 2 * device_cu_count() / blocks);
+    parts = std::min<int64_t>(parts, std::max<int64_t>(1, kv / 256));
+    if (parts > 1) {
+        n.span = static_cast<int>(((kv + parts - 1) / parts + 63) / 64 * 64);
+        parts = (kv + n.span - 1) / n.span;
+    }
+    n.parts = static_cast<int>(parts);
+    return n;
+}
+
+size_t plan_bytes(const Plan &n, const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
+    if (n.parts == 1) return 0;
+    const size_t rows = static_cast<size_t>(s.n_tokens) * p.n_heads * n.parts;
+    return rows * (c.head_dim * sizeof(float) + sizeof(float2));
+}
+
+template <typename T, typename C, int D>
+void launch_dim(const AttnArgs &a, const Plan &n, hipStream_t s) {
+    const int kv_heads = a.n_heads / a.group;
+    attn_tiles<T, C, D><<<dim3(n.tiles * kv_heads, n.parts), 256, 0, s>>>(a);
+    if (n.parts > 1) attn_join<T, D><<<dim3(a.n_tokens, a.n_heads), 64, 0, s>>>(a);
 }
 
 template <typename T, typename C>
-void launch_attn(const AttnArgs &a, int D, hipStream_t s) {
-    const dim3 grid(a.n_tokens, a.n_heads);
+void launch_attn(const AttnArgs &a, const Plan &n, int D, hipStream_t s) {
     if (D == 64)
-        attn_simple<T, C, 64><<<grid, 64, 0, s>>>(a);
+        launch_dim<T, C, 64>(a, n, s);
     else if (D == 128)
-        attn_simple<T, C, 128><<<grid, 64, 0, s>>>(a);
+        launch_dim<T, C, 128>(a, n, s);
     else
-        attn_simple<T, C, 256><<<grid, 64, 0, s>>>(a);
+        launch_dim<T, C, 256>(a, n, s);
 }
 
 int check_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
@@ -92,27 +527,38 @@ int check_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s
         return kBadShape;
     const int64_t row = static_cast<int64_t>(p.n_heads) * c.head_dim;
     if (s.n_tokens > 1 && ((p.q_stride && p.q_stride < row) || (p.out_stride && p.out_stride < row))) return kBadShape;
-    if (p.n_heads > 65535 || static_cast<int64_t>(s.n_tokens) * p.n_heads > INT32_MAX) return kTooLarge;
+    if (p.n_heads > 65535 || static_cast<int64_t>(s.n_tokens) * p.n_heads > INT32_MAX / 4 ||
+        static_cast<int64_t>(s.n_seqs) * p.n_heads > INT32_MAX / 4)
+        return kTooLarge;
     return kOk;
 }
 
 int run_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &b, hipStream_t s) {
-    const int st = check_attn(p, c, b);
+    int st = check_attn(p, c, b);
     if (st != kOk) return st;
+    const Plan n = plan(p, c, b);
+    const size_t bytes = plan_bytes(n, p, c, b);
+    void *ws = p.workspace;
+    if (ws && p.workspace_bytes < bytes) return kNoScratch;
+    if (bytes && !ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
     const int64_t row = static_cast<int64_t>(p.n_heads) * c.head_dim;
+    const float c2 = std::max(std::fabs(p.scale) * 1.4426950408889634f, 1e-37f);  // (> 0: 0 times an infinite score is no number)
+    const int64_t parts = static_cast<int64_t>(b.n_tokens) * p.n_heads * n.parts;
+    float *po = static_cast<float *>(ws);
     const AttnArgs a{p.q, c.k, c.v, p.out, p.q_stride ? p.q_stride : row, p.out_stride ? p.out_stride : row, b.q_start,
-                     b.kv_len, b.n_seqs, b.n_tokens, p.n_heads, p.n_heads / c.n_kv_heads, p.scale, p.causal,
-                     p.window, make_pages(c, b)};
+                     b.kv_len, b.n_seqs, b.n_tokens, p.n_heads, p.n_heads / c.n_kv_heads, c2, p.scale < 0 ? -1.0f : 1.0f,
+                     p.causal, p.window, n.parts, n.span, po, bytes ? reinterpret_cast<float2 *>(po + parts * c.head_dim) : nullptr,
+                     make_pages(c, b)};
     if (p.dtype == TQHIP_F16)
-        launch_attn<f16, f16>(a, c.head_dim, s);
+        launch_attn<f16, f16>(a, n, c.head_dim, s);
     else if (p.dtype == TQHIP_BF16)
-        launch_attn<bf16, bf16>(a, c.head_dim, s);
+        launch_attn<bf16, bf16>(a, n, c.head_dim, s);
     else if (c.dtype == TQHIP_F32)
-        launch_attn<float, float>(a, c.head_dim, s);
+        launch_attn<float, float>(a, n, c.head_dim, s);
     else if (c.dtype == TQHIP_F16)
-        launch_attn<float, f16>(a, c.head_dim, s);
+        launch_attn<float, f16>(a, n, c.head_dim, s);
     else
-        launch_attn<float, bf16>(a, c.head_dim, s);
+        launch_attn<float, bf16>(a, n, c.head_dim, s);
     return hipGetLastError() == hipSuccess ? kOk : kLaunchFailed;
 }
 
@@ -124,12 +570,16 @@ extern "C" {
 int tqhip_paged_attention_dev(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs,
                               void *stream) {
     if (!attn || !cache || !seqs) return tqhip::kBadShape;
-    return tqhip::run_attn(*attn, *cache, *seqs, static_cast<hipStream_t>(stream));
+    try {
+        return tqhip::run_attn(*attn, *cache, *seqs, static_cast<hipStream_t>(stream));
+    } catch (...) {  // (host memory ran out)
+        return tqhip::kHipFailed;
+    }
 }
 
 size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs) {
-    (void)attn, (void)cache, (void)seqs;
-    return 0;
+    if (!attn || !cache || !seqs || tqhip::check_attn(*attn, *cache, *seqs) != tqhip::kOk) return 0;
+    return tqhip::plan_bytes(tqhip::plan(*attn, *cache, *seqs), *attn, *cache, *seqs);
 }
 
 }  // extern "C"
