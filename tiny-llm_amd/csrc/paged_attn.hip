@@ -70,7 +70,14 @@ __device__ inline void split(const float *x, vec<E, 8> *out) {
     }
 }
 
+using f32x4 = vec<float, 4>;
 using f32x16 = vec<float, 16>;
+__device__ inline f32x4 mfma16(vec<f16, 8> a, vec<f16, 8> b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x4 mfma16(vec<bf16, 8> a, vec<bf16, 8> b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
 __device__ inline f32x16 mfma32(vec<f16, 8> a, vec<f16, 8> b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
@@ -91,6 +98,42 @@ __device__ inline bool is_finite(C x) {
         return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
     constexpr unsigned short kExp = std::is_same_v<C, f16> ? 0x7c00 : 0x7f80;
     return (__builtin_bit_cast(vec<unsigned short, sizeof(C) / 2>, x)[0] & kExp) != kExp;
+}
+
+// Bits below n (none for n <= 0, all from 32 on).
+__device__ inline unsigned below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// A chunk of 8 cache elements as its terms.
+template <typename C, typename E, int KT>
+__device__ inline void as_terms(const vec<C, 8> &x, vec<E, 8> *out) {
+    if constexpr (KT == 1) {
+        out[0] = x;
+    } else {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = x[e];
+        split<E, KT>(f, out);
+    }
+}
+
+// Infinities and NaN replaced by zeros; false if there were any.
+template <typename C>
+__device__ inline bool make_finite(vec<C, 8> &x) {
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (!is_finite<C>(x[e])) {
+            finite = false;
+            x[e] = static_cast<C>(0.0f);
+        }
+    return finite;
+}
+
+// LDS that only one wave uses: what its lanes wrote is there for all of them (a wave's LDS accesses complete in order; this
+// keeps the compiler from reordering them).
+__device__ inline void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // Weights are 2^(s c + bias): with fp16 terms they are held 2^8 times larger, above fp16's subnormals.
@@ -135,26 +178,281 @@ __device__ inline bool find_tile(const AttnArgs &a, int tile, TileRows &t) {
 __device__ inline int key_lo(const AttnArgs &a, int p) { return a.causal && a.window > 0 ? max(0, p + 1 - a.window) : 0; }
 __device__ inline int key_hi(const AttnArgs &a, int p, int len) { return a.causal ? min(p + 1, len) : len; }
 
-// ---- many rows: tiles of 128 rows ---------------------------------------------------------------
-// Bits below n (none for n <= 0, all from 32 on).
-__device__ inline unsigned below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
-
-// A chunk of 8 cache elements into the LDS planes of its terms.
-template <typename C, typename E, int KT, int BN, int STRIDE>
-__device__ inline void put_terms(const vec<C, 8> &x, E (*planes)[BN][STRIDE], int row, int at) {
-    if constexpr (KT == 1) {
-        *reinterpret_cast<vec<C, 8> *>(&planes[0][row][at]) = x;
+// A row's query as the operand of the score products: N chunks of 8 elements, STEP apart, in each of the lanes that hold the
+// row (wide(x): the largest x over them). Returns the factor that takes a product to a power of two's exponent. fp32 rows
+// against fp16 keys are scaled into fp16's range by a power of two, which that factor takes back.
+template <typename T, typename E, int QT, int N, int STEP, typename Wide>
+__device__ inline float load_query(const AttnArgs &a, const T *qp, vec<E, 8> (*q)[N], Wide wide) {
+    float c = a.scale;
+    if constexpr (QT == 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            q[0][i] = *reinterpret_cast<const vec<E, 8> *>(qp + STEP * i);
+            if (a.sign < 0.0f) q[0][i] = -q[0][i];
+        }
     } else {
-        float f[8];
-        vec<E, 8> terms[KT];
+        int ex = 0;
+        if constexpr (std::is_same_v<E, f16>) {
+            float mx = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = x[e];
-        split<E, KT>(f, terms);
+            for (int i = 0; i < N; ++i) {
+                float x[8];
+                load_as_float<T, 8>(qp + STEP * i, x);
 #pragma unroll
-        for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&planes[n][row][at]) = terms[n];
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+            }
+            mx = wide(mx);
+            if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
+            c = ldexpf(c, ex);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float x[8];
+            load_as_float<T, 8>(qp + STEP * i, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], -ex) * a.sign;
+            vec<E, 8> terms[QT];
+            split<E, QT>(x, terms);
+#pragma unroll
+            for (int n = 0; n < QT; ++n) q[n][i] = terms[n];
+        }
+    }
+    return c;
+}
+
+// ---- few rows: tiles of 16 rows ------------------------------------------------------------------
+
+// A tile's keys are dealt to the four waves 32 at a time; each wave keeps a softmax of its own, and the four meet at the end.
+// K goes from the cache straight into operand registers; V passes through LDS of the wave's own, which turns rows into columns.
+// Both registers are filled again as soon as they have been used, so K's loads are under way during the softmax and the
+// value product and V's during the next scores, with no wave waiting for another.
+constexpr int kFewRows = 16;
+constexpr int kFewKeys = 32;   // per wave and step
+constexpr int kFewStep = 4 * kFewKeys;
+
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 : 2)) void attn_few(AttnArgs a) {
+    using Tm = Terms<T, C>;
+    using E = typename Tm::E;
+    constexpr int QT = Tm::QT, KT = Tm::KT;
+    constexpr int VS = D + 16, ND = D / 16, NS = D / 32;
+    static_assert(4 * kFewKeys * VS * sizeof(E) >= 4 * kFewRows * D * sizeof(float), "the waves' outputs fit where V was");
+    __shared__ __attribute__((aligned(16))) E vs[4][kFewKeys][VS];
+    __shared__ float meet[2][4][kFewRows];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
+    const int kv_heads = a.n_heads / a.group;
+    const int kvh = blockIdx.x % kv_heads;
+    TileRows t;
+    if (!find_tile<kFewRows>(a, blockIdx.x / kv_heads, t)) return;
+    const int rows = t.n * a.group;
+    const int last = min(t.r0 + kFewRows, rows) - 1;
+    const int p_first = t.pos0 + t.r0 / a.group, p_last = t.pos0 + last / a.group;
+    int kb = key_lo(a, p_first), ke = key_hi(a, p_last, t.len);
+    if (a.parts > 1) {
+        kb = max(kb, static_cast<int>(blockIdx.y) * a.span);
+        if (static_cast<int>(blockIdx.y) < a.parts - 1) ke = min(ke, (static_cast<int>(blockIdx.y) + 1) * a.span);
+        if (kb >= ke) return;
+    }
+    const int full_lo = key_lo(a, p_last), full_hi = key_hi(a, p_first, t.len);
+    const int r = min(t.r0 + col, rows - 1);
+    const int token = t.first + r / a.group, head = kvh * a.group + r % a.group;
+    const int pos = t.pos0 + r / a.group;
+    const int lo = key_lo(a, pos), hi = key_hi(a, pos, t.len);
+
+    const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride + 8 * g;
+    const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride + 8 * g;
+    vec<C, 8> kr[2][NS], vr[2][NS];
+    // the lane's keys of a step: k0 + col and k0 + 16 + col
+    const auto offsets = [&](int k0, int64_t *o) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const int key = k0 + 16 * kt + col;
+            o[kt] = key < ke ? row_offset(a.pages, t.b, key) : -1;
+        }
+    };
+    const auto load_rows = [&](const C *base, const int64_t *o, vec<C, 8> (*x)[NS]) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) x[kt][i] = vec<C, 8>{};
+            if (o[kt] >= 0) {
+#pragma unroll
+                for (int i = 0; i < NS; ++i) x[kt][i] = *reinterpret_cast<const vec<C, 8> *>(base + o[kt] + 32 * i);
+            }
+        }
+    };
+
+    int64_t off[2], next[2];
+    int k0 = kb + wave * kFewKeys;
+    offsets(k0, off);
+    load_rows(kc, off, kr);
+    load_rows(vc, off, vr);
+    offsets(k0 + kFewStep, next);
+    vec<E, 8> q[QT][NS];
+    const float c = load_query<T, E, QT, NS, 32>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * g, q,
+                                                 [&](float x) {
+                                                     x = fmaxf(x, lane_xor<16>(x, lane));
+                                                     return fmaxf(x, lane_xor<32>(x, lane));
+                                                 });
+    f32x4 acc[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[i] = f32x4{};
+    float m = -INFINITY, bias = 0.0f, l = 0.0f;
+
+    for (; k0 < ke; k0 += kFewStep) {
+        // S^T: the lane holds its row's scores of keys 16 kt + 4 g + i
+        f32x4 s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            s[kt] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                vec<E, 8> kf[KT];
+                as_terms<C, E, KT>(kr[kt][i], kf);
+#pragma unroll
+                for (int kj = 0; kj < KT; ++kj)
+#pragma unroll
+                    for (int qi = 0; qi < QT; ++qi)
+                        if (qi + kj < Tm::kMost) s[kt] = mfma16(kf[kj], q[qi][i], s[kt]);
+            }
+        }
+        const unsigned exist = static_cast<unsigned>(__ballot(off[0] >= 0) & 0xffff) |
+                               static_cast<unsigned>(__ballot(off[1] >= 0) & 0xffff) << 16;
+        const bool partial = k0 < full_lo || k0 + kFewKeys > full_hi;
+        const int64_t was[2] = {off[0], off[1]};
+        off[0] = next[0];
+        off[1] = next[1];
+        load_rows(kc, off, kr);
+        offsets(k0 + 2 * kFewStep, next);
+        if (partial || exist != ~0u) {
+            const int k1 = k0 + 4 * g;
+            const unsigned may = (exist >> (4 * g)) & below(hi - k1) & ~below(lo - k1);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(may & (1u << (16 * kt + i)))) s[kt][i] = -INFINITY;
+        }
+        float mx = m;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kt][i]);
+        mx = fmaxf(mx, lane_xor<16>(mx, lane));
+        mx = fmaxf(mx, lane_xor<32>(mx, lane));
+        if (__ballot(mx != m)) {
+            const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
+            const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
+            m = mx;
+            bias = nb;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) acc[i] *= f;
+        }
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            w[e] = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], c, bias));
+            l += w[e];
+        }
+        vec<E, 8> p[QT];
+        split<E, QT>(w, p);
+        unsigned wild = 0;
+        if (partial) {  // infinite and NaN values as in attn_tiles
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                bool finite = true;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) finite = make_finite<C>(vr[kt][i]) && finite;
+                const unsigned long long bad = __ballot(!finite);
+                wild |= static_cast<unsigned>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff) << (16 * kt);
+            }
+        }
+#pragma unroll
+        for (int kj = 0; kj < KT; ++kj) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    vec<E, 8> vf[KT];
+                    as_terms<C, E, KT>(vr[kt][i], vf);
+                    *reinterpret_cast<vec<E, 8> *>(&vs[wave][16 * kt + col][32 * i + 8 * g]) = vf[kj];
+                }
+            wave_lds_order();
+            if (kj == KT - 1) load_rows(vc, off, vr);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const E *v0 = &vs[wave][4 * g + (lane & 15) / 4][16 * d + 4 * (lane & 3)];
+                const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 16 * VS);
+                const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int qi = 0; qi < QT; ++qi)
+                    if (qi + kj < Tm::kMost) acc[d] = mfma16(vf, p[qi], acc[d]);
+            }
+            wave_lds_order();
+        }
+        for (; wild; wild &= wild - 1) {
+            const int j = __builtin_ctz(wild), key = k0 + j;
+            const int64_t o = __shfl(static_cast<long long>(j < 16 ? was[0] : was[1]), j & 15);
+            if (key < lo || key >= hi) continue;
+            const C *v0 = vc + o - 8 * g + 4 * g;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!is_finite<C>(v0[16 * d + e])) acc[d][e] += static_cast<float>(v0[16 * d + e]);
+        }
+    }
+    l += lane_xor<16>(l, lane);
+    l += lane_xor<32>(l, lane);
+    // the four waves' sums, brought to the least exponent bias among those that have any
+    if (g == 0) {
+        meet[0][wave][col] = bias;
+        meet[1][wave][col] = l;
+    }
+    __syncthreads();  // (and every wave is done with V)
+    float least = INFINITY, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        if (meet[1][w][col] != 0.0f) least = fminf(least, meet[0][w][col]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        if (meet[1][w][col] != 0.0f) total += meet[1][w][col] * exp2f(least - meet[0][w][col]);
+    const float f = l != 0.0f ? exp2f(least - bias) : 0.0f;
+    float(*os)[kFewRows][D] = reinterpret_cast<float(*)[kFewRows][D]>(&vs[0][0][0]);
+    if (l != 0.0f) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= f;
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&os[wave][col][16 * d + 4 * g]) = acc[d];
+    __syncthreads();
+    // thread: row tid / 16, every 16th group of four dimensions
+    const int row = tid >> 4;
+    if (t.r0 + row >= rows) return;
+    const int r2 = t.r0 + row, token2 = t.first + r2 / a.group, head2 = kvh * a.group + r2 % a.group;
+    const float total2 = __shfl(total, row), least2 = __shfl(least, row);
+    const int64_t at = (static_cast<int64_t>(token2) * a.n_heads + head2) * a.parts + blockIdx.y;
+    if (a.parts > 1 && (tid & 15) == 0) a.part_ml[at] = make_float2(least2, total2);
+    const float inv = total2 == 0.0f ? 0.0f : 1.0f / total2;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const int d = 4 * (tid & 15) + 64 * i;
+        f32x4 o = *reinterpret_cast<f32x4 *>(&os[0][row][d]);
+#pragma unroll
+        for (int w = 1; w < 4; ++w) o += *reinterpret_cast<f32x4 *>(&os[w][row][d]);
+        if (a.parts > 1) {
+            *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) = o;
+        } else {
+            o *= inv;
+            float x[4] = {o[0], o[1], o[2], o[3]};
+            store_rounded<T, 4>(static_cast<T *>(a.out) + token2 * a.out_stride + head2 * D + d, x);
+        }
     }
 }
 
+// ---- many rows: tiles of 128 rows ---------------------------------------------------------------
 template <typename T, typename C, int D>
 struct TileShape {
     using Tm = Terms<T, C>;
@@ -209,44 +507,8 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     const int wf_lo = key_lo(a, wp_last), wf_hi = key_hi(a, wp_first, t.len);
 
     vec<E, 8> q[QT][D / 16];
-    float c = a.scale;
-    {
-        const T *qp = static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * h;
-        if constexpr (QT == 1) {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                q[0][i] = *reinterpret_cast<const vec<E, 8> *>(qp + 16 * i);
-                if (a.sign < 0.0f) q[0][i] = -q[0][i];
-            }
-        } else {
-            float mx = 0.0f;
-            if constexpr (std::is_same_v<E, f16>) {  // the row scaled to fp16's range by a power of two
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    float x[8];
-                    load_as_float<T, 8>(qp + 16 * i, x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
-                }
-                mx = fmaxf(mx, lane_xor<32>(mx, lane));
-            }
-            int ex = 0;
-            if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
-            c = ldexpf(c, ex);
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                float x[8];
-                load_as_float<T, 8>(qp + 16 * i, x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], -ex) * a.sign;
-                vec<E, 8> terms[QT];
-                split<E, QT>(x, terms);
-#pragma unroll
-                for (int n = 0; n < QT; ++n) q[n][i] = terms[n];
-            }
-        }
-    }
-
+    const float c = load_query<T, E, QT, D / 16, 16>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * h, q,
+                                                     [&](float x) { return fmaxf(x, lane_xor<32>(x, lane)); });
     const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride;
     const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride;
     vec<C, 8> kr[NCH], vr[NCH];
@@ -294,17 +556,15 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
             if (partial) {
                 // An infinite or NaN value would reach rows that mask its key through a product with their weight of zero.
                 // It goes into the products as zero and is added below where its key is seen.
-                bool finite = true;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!is_finite<C>(vr[i][e])) {
-                        finite = false;
-                        vr[i][e] = static_cast<C>(0.0f);
-                    }
-                if (!finite) atomicOr(&wild[buf], 1ull << row);
+                if (!make_finite<C>(vr[i])) atomicOr(&wild[buf], 1ull << row);
             }
-            put_terms<C, E, KT, BN, KS>(kr[i], ks, row, at);
-            put_terms<C, E, KT, BN, VS>(vr[i], vs, row, at);
+            vec<E, 8> terms[KT];
+            as_terms<C, E, KT>(kr[i], terms);
+#pragma unroll
+            for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&ks[n][row][at]) = terms[n];
+            as_terms<C, E, KT>(vr[i], terms);
+#pragma unroll
+            for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&vs[n][row][at]) = terms[n];
         }
         put_offset(buf ^ 1, next_off);
         __syncthreads();
@@ -468,23 +728,27 @@ __global__ __launch_bounds__(64) void attn_join(AttnArgs a) {
 
 // How the work is cut, from the host's numbers alone.
 struct Plan {
+    bool few;
     int tiles, parts, span;
 };
 
 Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
     const int group = p.n_heads / c.n_kv_heads;
+    const int64_t rows = static_cast<int64_t>(s.n_tokens) * group;
     Plan n{};
-    n.tiles = static_cast<int>(static_cast<int64_t>(s.n_tokens) * group / kTileRows) + s.n_seqs;
+    n.few = rows <= int64_t{2} * kFewRows * s.n_seqs;
+    n.tiles = static_cast<int>(rows / (n.few ? kFewRows : kTileRows)) + s.n_seqs;
     const int64_t most = static_cast<int64_t>(s.table_stride) * c.page_size;
     const int64_t kv = s.max_kv > 0 ? std::min<int64_t>(s.max_kv, most) : most;
     const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads;
-    int64_t parts = std::max<int64_t>(1, 2 * device_cu_count() / blocks);
-    parts = std::min<int64_t>(parts, std::max<int64_t>(1, kv / 256));
-    if (parts > 1) {
+    if (n.few) {
+        const int64_t want = kv * blocks / (8 * device_cu_count());
+        n.span = static_cast<int>(std::clamp<int64_t>((want + kFewStep - 1) / kFewStep * kFewStep, kFewStep, 1024));
+    } else {
+        const int64_t parts = std::min<int64_t>(std::max<int64_t>(1, 2 * device_cu_count() / blocks), std::max<int64_t>(1, kv / 256));
         n.span = static_cast<int>(((kv + parts - 1) / parts + 63) / 64 * 64);
-        parts = (kv + n.span - 1) / n.span;
     }
-    n.parts = static_cast<int>(parts);
+    n.parts = static_cast<int>((kv + n.span - 1) / n.span);
     return n;
 }
 
@@ -497,7 +761,11 @@ size_t plan_bytes(const Plan &n, const tqhip_attn &p, const tqhip_kv_cache &c, c
 template <typename T, typename C, int D>
 void launch_dim(const AttnArgs &a, const Plan &n, hipStream_t s) {
     const int kv_heads = a.n_heads / a.group;
-    attn_tiles<T, C, D><<<dim3(n.tiles * kv_heads, n.parts), 256, 0, s>>>(a);
+    const dim3 grid(n.tiles * kv_heads, n.parts);
+    if (n.few)
+        attn_few<T, C, D><<<grid, 256, 0, s>>>(a);
+    else
+        attn_tiles<T, C, D><<<grid, 256, 0, s>>>(a);
     if (n.parts > 1) attn_join<T, D><<<dim3(a.n_tokens, a.n_heads), 64, 0, s>>>(a);
 }
 
