@@ -274,8 +274,8 @@ size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_ca
 
 /* The low-rank adapters of many requests, beside the projection that they share:
  * y_t = base_t + scale[a] * B_a (A_a x_t), a = adapter[b] of the sequence b that token t is in.
- * Tokens of no sequence, and those whose adapter is outside [0, n_adapters) (-1: none), get
- * base_t. x is [n_tokens][in_dim] and base / y [n_tokens][out_dim], as matmul_i4 reads and
+ * Tokens whose adapter is outside [0, n_adapters) (-1: none) get base_t; tokens of no sequence
+ * keep their y. x is [n_tokens][in_dim] and base / y [n_tokens][out_dim], as matmul_i4 reads and
  * writes them; base may be y, or NULL for zeros. An adapter of a lower rank has zero rows.
  * rank 1 to 256. workspace: as for the attention, tqhip_lora_workspace() bytes. */
 typedef struct tqhip_lora {

@@ -157,7 +157,7 @@ def attention(batch, q, scale, causal, window):
 
 
 def lora(x, base, a, b, scale, starts, adapter, tokens):
-    """-> (y, size): size bounds the terms of each result."""
+    """-> (y, size): size bounds the terms of each result. Rows of tokens in no sequence are the base's."""
     y = np.zeros((tokens, b.shape[1])) if base is None else base.copy()
     size = np.abs(y)
     for i, ad in enumerate(adapter):

@@ -277,7 +277,7 @@ LORA = [  # tokens of each request, adapters of each, K, M, rank
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("new,adapter,K,M,r", LORA)
 def test_lora_add(gpu, dtype, new, adapter, K, M, r):
-    """Adapter 7 is outside the four: as none. Tokens before the first and after the last request get the base."""
+    """Adapter 7 is outside the four: as none. Tokens before the first and after the last request keep their y."""
     rng = np.random.default_rng(K + M + r)
     n, starts = 4, 1 + np.concatenate(([0], np.cumsum(new)))
     T = int(starts[-1]) + 2
@@ -286,24 +286,28 @@ def test_lora_add(gpu, dtype, new, adapter, K, M, r):
     scale = rng.uniform(0.5, 2, n).astype(np.float32)
     dx, db, ds, dst, dad = f32_buffer(gpu, x), f32_buffer(gpu, base), f32_buffer(gpu, scale), ints(gpu, starts), ints(gpu, adapter)
     want, size = ref.lora(x.astype(np.float64), base.astype(np.float64), a.values, b.values, scale.astype(np.float64), starts, adapter, T)
+    inside = slice(1, int(starts[-1]))
 
     def call(dbase, dy):
         gpu.lora_add_dev(gpu.Lora(dtype=dtype, n_tokens=T, in_dim=K, out_dim=M, rank=r, n_adapters=n, n_seqs=len(new), x=dx.ptr, base=dbase, y=dy,
                                   a=a.ptr, b=b.ptr, scale=ds.ptr, q_start=dst.ptr, adapter=dad.ptr))
         gpu.synchronize()
 
-    def check(got, want, what):
-        got = got.reshape(T, M).astype(np.float64)
-        assert np.all(np.abs(got - want) <= (K + r + 8) * U * size), what
-        assert np.linalg.norm(got - want) <= 2.0 ** -18 * np.linalg.norm(size), what
+    def check(got, want, outside, what):
+        got = got.reshape(T, M)
+        assert np.array_equal(got[0], outside[0]) and np.array_equal(got[-2:], outside[-2:]), f"{what}: rows outside the call changed"
+        off = np.abs(got.astype(np.float64) - want)[inside]
+        assert np.all(off <= (K + r + 8) * U * size[inside]), what
+        assert np.linalg.norm(off) <= 2.0 ** -18 * np.linalg.norm(size[inside]), what
 
-    dy = gpu.DeviceBuffer(4 * T * M)
+    seven = np.full((T, M), 7.0, np.float32)
+    dy = f32_buffer(gpu, seven)
     call(db.ptr, dy.ptr)
-    check(dy.download(np.float32, T * M), want, "y = base + delta")
+    check(dy.download(np.float32, T * M), want, seven, "y = base + delta")
     call(None, dy.ptr)
-    check(dy.download(np.float32, T * M), want - base, "y = delta")
+    check(dy.download(np.float32, T * M), want - base, seven, "y = delta")
     call(db.ptr, db.ptr)
-    check(db.download(np.float32, T * M), want, "in place")
+    check(db.download(np.float32, T * M), want, base, "in place")
 
 
 @pytest.mark.parametrize("cache", [F16, BF16, F32])

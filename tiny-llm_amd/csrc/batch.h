@@ -54,6 +54,35 @@ __device__ inline int last_start_at_or_before(const int *start, int n, int t) {
     }
 }
 
+// The rows of a ragged batch in tiles of BM: a sequence with n tokens has n * per rows (per: rows of a token). Tiles are numbered
+// over the batch without a scan of the lengths: sequence b's start at floor(start[b] per / BM) + b, which leaves room for
+// ceil(n per / BM) of them, so there are floor(n_tokens per / BM) + n_seqs numbers and some name no tile.
+struct Run {
+    int b, first, n, r0;  // sequence, its first token, its number of tokens, the tile's first row
+};
+template <int BM>
+__device__ inline bool find_run(const int *q_start, int n_seqs, int n_tokens, int per, int tile, Run &t) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = n_seqs;
+    const auto base = [&](int b) {
+        const int64_t s = min(max(q_start[b], 0), n_tokens);
+        return static_cast<int>(s * per / BM) + b;
+    };
+    for (;;) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const int c = __popcll(__ballot(i < n && base(lo + i) <= tile));
+        if (c == 0) return false;
+        lo += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+        if (step == 1) break;
+    }
+    t.b = lo;
+    t.first = min(max(q_start[lo], 0), n_tokens);
+    t.n = min(max(q_start[lo + 1], 0), n_tokens) - t.first;
+    t.r0 = (tile - base(lo)) * BM;
+    return t.n > 0 && t.r0 < t.n * per;
+}
+
 // Division of 0 <= n < 2^31 by a fixed d >= 1 as a multiplication (Granlund and Montgomery, Division by
 // Invariant Integers using Multiplication, 1994): with s = ceil(log2 d) and
 // m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(m, n) + n) >> s; the sum stays below 2^32.

@@ -142,36 +142,16 @@ constexpr float kWeightShift = std::is_same_v<E, f16> ? 8.0f : 0.0f;
 
 // ---- the sequence and the rows of a tile -----------------------------------------------------------
 
-// Rows of a sequence with n new tokens: (token, head of the group), n * group of them. Tiles of BM rows
-// are numbered over the batch without a scan of the lengths: sequence b's start at
-// floor(start[b] group / BM) + b, which leaves room for ceil(n group / BM) of them.
-struct TileRows {
-    int b, first, n, r0, pos0, len;  // sequence, its first token, its tokens, the tile's first row, position of token 0, cached length
+// A tile of (token, head of the group) rows.
+struct TileRows : Run {
+    int pos0, len;  // position of the sequence's first new token, its cached length
 };
 template <int BM>
 __device__ inline bool find_tile(const AttnArgs &a, int tile, TileRows &t) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, n = a.n_seqs;
-    const auto base = [&](int b) {
-        const int64_t s = min(max(a.q_start[b], 0), a.n_tokens);
-        return static_cast<int>(s * a.group / BM) + b;
-    };
-    for (;;) {
-        const int step = (n + 63) / 64, i = lane * step;
-        const int c = __popcll(__ballot(i < n && base(lo + i) <= tile));
-        if (c == 0) return false;
-        lo += (c - 1) * step;
-        n = min(step, n - (c - 1) * step);
-        if (step == 1) break;
-    }
-    const int end = min(max(a.q_start[lo + 1], 0), a.n_tokens);
-    t.b = lo;
-    t.first = min(max(a.q_start[lo], 0), a.n_tokens);
-    t.n = end - t.first;
-    t.r0 = (tile - base(lo)) * BM;
-    t.pos0 = a.kv_len[lo] - t.n;
-    t.len = min(a.kv_len[lo], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
-    return t.n > 0 && t.r0 < t.n * a.group;
+    if (!find_run<BM>(a.q_start, a.n_seqs, a.n_tokens, a.group, tile, t)) return false;
+    t.pos0 = a.kv_len[t.b] - t.n;
+    t.len = min(a.kv_len[t.b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
+    return true;
 }
 
 // Keys [lo, hi) of the row's token at position p.
