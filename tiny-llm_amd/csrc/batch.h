@@ -35,23 +35,34 @@ __device__ inline void store_rounded(T *p, const float *in) {
     *reinterpret_cast<vec<T, N> *>(p) = v;
 }
 
-// The last b < n with start[b] <= t, or -1, found by the 64 lanes of a wave together (all of them call
-// it with the same arguments): one load for up to 64 sequences, two for up to 4096, where a bisection
-// by one lane waits for 6 and 12 loads one after the other. Whatever the array holds, the result is
-// in range.
-__device__ inline int last_start_at_or_before(const int *start, int n, int t) {
+// LDS that only one wave uses: what its lanes wrote is there for all of them (a wave's LDS accesses complete in order; this
+// keeps the compiler from reordering them).
+__device__ inline void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The sequence b of token t and the token's position in it; false where it is in none. The 64 lanes of a wave search
+// together (all call with the same arguments): up to 64 sequences' starts and lengths are one round of loads, and 4096 are
+// two and a third, where a bisection waits for 6 and 12 loads one after the other. Whatever the arrays hold, b is in range.
+__device__ inline bool find_token(const int *start, const int *len, int n, int t, int &b, int &pos) {
     const int lane = threadIdx.x & 63;
     int lo = 0;
-    for (;;) {
-        const int step = (n + 63) / 64;
-        const int i = lane * step;
-        const bool in = i < n && start[lo + i] <= t;
-        const int c = __popcll(__ballot(in));
-        if (c == 0) return lo - 1;  // (only in the first round for an increasing array: lo = 0)
+    while (n > 64) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const int c = __popcll(__ballot(i < n && start[lo + i] <= t));
+        if (c == 0) return false;
         lo += (c - 1) * step;
         n = min(step, n - (c - 1) * step);
-        if (step == 1) return lo;
     }
+    const int at = lo + min(lane, n - 1);
+    const int first = start[at], end = start[at + 1], kv = len[at];
+    const int c = __popcll(__ballot(lane < n && first <= t));
+    if (c == 0) return false;
+    b = lo + c - 1;
+    const int e = __builtin_amdgcn_readlane(end, c - 1);
+    pos = __builtin_amdgcn_readlane(kv, c - 1) - (e - t);
+    return t < e;
 }
 
 // The rows of a ragged batch in tiles of BM: a sequence with n tokens has n * per rows (per: rows of a token). Tiles are numbered

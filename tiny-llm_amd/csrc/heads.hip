@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kHeadThreads = 256;
 constexpr int kHeadWaves = kHeadThreads / 64;
+constexpr int kHeadRounds = 4;
 
 struct HeadArgs {
     const void *in[3];       // q, k, v
@@ -54,125 +55,144 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a) {
     constexpr int HPI = 64 / LPH;
     const int lane = threadIdx.x & 63;
     const int wave = blockIdx.x * kHeadWaves + (threadIdx.x >> 6);
-    const int waves = gridDim.x * kHeadWaves;
+    const int t = wave / a.split, part = wave - t * a.split;
+    if (t >= a.n_tokens) return;
     const int n_heads = a.heads[0] + a.heads[1] + a.heads[2];
     const int iters = (n_heads + HPI - 1) / HPI;
-    const int per = (iters + a.split - 1) / a.split;
-    const int part = wave % a.split;
-    const int it0 = part * per, it1 = min(it0 + per, iters);
+    const int it0 = iters * part / a.split, it1 = iters * (part + 1) / a.split;  // at most kHeadRounds
     const int half = a.rot / 2;
     const int sub = lane / LPH;
 
     int at0[NU], at1[NU];
     bool has[NU], turned[NU];
-    double turns[NU][V];  // per position
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
         const int u = V == 1 ? lane + 64 * j : lane % LPH;
         const int rot_units = half / V;
         has[j] = V > 1 || u < a.D / 2;
         turned[j] = has[j] && u < rot_units;
-        at0[j] = turned[j] ? u * V : a.rot + 2 * V * (u - rot_units);
-        at1[j] = turned[j] ? half + u * V : at0[j] + V;
+        at0[j] = !has[j] ? 0 : turned[j] ? u * V : a.rot + 2 * V * (u - rot_units);
+        at1[j] = !has[j] ? 0 : turned[j] ? half + u * V : at0[j] + V;
+    }
+    const auto kind_of = [&](int &h) {
+        const int kind = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
+        if (kind > 0) h -= a.heads[0];
+        if (kind > 1) h -= a.heads[1];
+        return kind;
+    };
+    // All of the wave's elements are requested at once, before anything waits, and without branches (heads past the last are the
+    // last again): a load after a store would wait for the store too, since both count on one in-order counter.
+    vec<T, V> raw0[kHeadRounds][NU], raw1[kHeadRounds][NU];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            constexpr double kInvTwoPi = 0.15915494309189535;
-            const int i = u * V + e;
-            turns[j][e] = !turned[j] ? 0.0
-                          : a.inv_freq ? static_cast<double>(a.inv_freq[i]) * kInvTwoPi
-                                       : exp2(-a.log2_theta * i / half) * kInvTwoPi;
+    for (int i = 0; i < kHeadRounds; ++i) {
+        int h = min(min(it0 + i, it1 - 1) * HPI + sub, n_heads - 1);
+        const int kind = kind_of(h);
+        const T *src = static_cast<const T *>(a.in[kind]) + t * a.in_stride[kind] + h * a.D;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            raw0[i][j] = *reinterpret_cast<const vec<T, V> *>(src + at0[j]);
+            raw1[i][j] = *reinterpret_cast<const vec<T, V> *>(src + at1[j]);
         }
     }
 
-    for (int t = wave / a.split; t < a.n_tokens; t += waves / a.split) {
-        int pos = 0;
-        int64_t row = -1;
-        if constexpr (APPEND) {
-            const int b = last_start_at_or_before(a.q_start, a.n_seqs, t);
-            if (b < 0) continue;
-            const int end = a.q_start[b + 1];
-            if (t >= end) continue;
-            pos = a.kv_len[b] - (end - t);
-            if (pos < 0) continue;
-            row = row_offset(a.pages, b, pos);
-        }
-        if (!APPEND || a.positions) pos = a.positions ? a.positions[t] : 0;
-        float c[NU][V], s[NU][V];
+    int pos = 0;
+    int64_t row = -1;
+    if constexpr (APPEND) {
+        int b;
+        if (!find_token(a.q_start, a.kv_len, a.n_seqs, t, b, pos) || pos < 0) return;
+        row = row_offset(a.pages, b, pos);
+    }
+    if (!APPEND || a.positions) pos = a.positions ? a.positions[t] : 0;
+
+    // The token's cosines and sines are formed one pair per lane and go to the lanes of all heads through LDS of the wave's own
+    // (formed where they are used, each is formed 64 V / half times over).
+    __shared__ __attribute__((aligned(16))) float turn[kHeadWaves][2][256];
+    float *cosines = turn[threadIdx.x >> 6][0], *sines = turn[threadIdx.x >> 6][1];
+    float c[NU][V], s[NU][V];
+    for (int i = lane; i < half; i += 64) {
+        constexpr double kInvTwoPi = 0.15915494309189535;
+        const double freq = a.inv_freq ? static_cast<double>(a.inv_freq[i]) : exp2(-a.log2_theta * i / half);
+        const double w = pos * (freq * kInvTwoPi);
+        sincospif(static_cast<float>(2.0 * (w - rint(w))), &sines[i], &cosines[i]);
+    }
+    wave_lds_order();
 #pragma unroll
-        for (int j = 0; j < NU; ++j)
+    for (int j = 0; j < NU; ++j)
+        if (turned[j]) {
+            load_as_float<float, V>(cosines + at0[j], c[j]);
+            load_as_float<float, V>(sines + at0[j], s[j]);
+        }
+
+#pragma unroll
+    for (int i = 0; i < kHeadRounds; ++i) {
+        if (it0 + i >= it1) break;
+        int h = (it0 + i) * HPI + sub;
+        const bool live = h < n_heads;
+        const int kind = kind_of(h);
+        const float *bias = a.bias[kind];
+        float x0[NU][V], x1[NU][V];
+        float sq = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const double w = pos * turns[j][e];
-                sincospif(static_cast<float>(2.0 * (w - rint(w))), &s[j][e], &c[j][e]);
+                x0[j][e] = has[j] ? static_cast<float>(raw0[i][j][e]) : 0.0f;
+                x1[j][e] = has[j] ? static_cast<float>(raw1[i][j][e]) : 0.0f;
             }
-        for (int it = it0; it < it1; ++it) {
-            int h = it * HPI + sub;
-            const bool live = h < n_heads;
-            const int kind = h < a.heads[0] ? 0 : h < a.heads[0] + a.heads[1] ? 1 : 2;
-            if (kind > 0) h -= a.heads[0];
-            if (kind > 1) h -= a.heads[1];
-            const T *src = static_cast<const T *>(a.in[kind]) + t * a.in_stride[kind] + h * a.D;
-            const float *bias = a.bias[kind];
-            float x0[NU][V], x1[NU][V];
-            float sq = 0.0f;
+            if (bias && live && has[j]) {
+                float b0[V], b1[V];
+                load_as_float<float, V>(bias + h * a.D + at0[j], b0);
+                load_as_float<float, V>(bias + h * a.D + at1[j], b1);
 #pragma unroll
-            for (int j = 0; j < NU; ++j) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) x0[j][e] = x1[j][e] = 0.0f;
-                if (live && has[j]) {
-                    load_as_float<T, V>(src + at0[j], x0[j]);
-                    load_as_float<T, V>(src + at1[j], x1[j]);
-                    if (bias) {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            x0[j][e] += bias[h * a.D + at0[j] + e];
-                            x1[j][e] += bias[h * a.D + at1[j] + e];
-                        }
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < V; ++e) sq += x0[j][e] * x0[j][e] + x1[j][e] * x1[j][e];
-            }
-            if (a.norm[0] || a.norm[1]) {
-#pragma unroll
-                for (int d = 1; d < LPH; d *= 2) sq += __shfl_xor(sq, d);
-                const float *w = kind == 0 ? a.norm[0] : kind == 1 ? a.norm[1] : nullptr;
-                if (w) {
-                    const float r = 1.0f / sqrtf(sq / static_cast<float>(a.D) + a.eps);
-#pragma unroll
-                    for (int j = 0; j < NU; ++j)
-                        if (has[j]) {
-#pragma unroll
-                            for (int e = 0; e < V; ++e) {
-                                x0[j][e] = x0[j][e] * r * w[at0[j] + e];
-                                x1[j][e] = x1[j][e] * r * w[at1[j] + e];
-                            }
-                        }
+                for (int e = 0; e < V; ++e) {
+                    x0[j][e] += b0[e];
+                    x1[j][e] += b1[e];
                 }
             }
-            if (!live) continue;
 #pragma unroll
-            for (int j = 0; j < NU; ++j) {
-                if (!has[j]) continue;
-                if (turned[j] && kind < 2) {
+            for (int e = 0; e < V; ++e) sq += x0[j][e] * x0[j][e] + x1[j][e] * x1[j][e];
+        }
+        if (a.norm[0] || a.norm[1]) {
+#pragma unroll
+            for (int d = 1; d < LPH; d *= 2) sq += __shfl_xor(sq, d);
+            const float *w = kind < 2 ? a.norm[kind] : nullptr;
+            if (w) {
+                const float r = 1.0f / sqrtf(sq / static_cast<float>(a.D) + a.eps);
+#pragma unroll
+                for (int j = 0; j < NU; ++j) {
+                    float w0[V], w1[V];
+                    load_as_float<float, V>(w + at0[j], w0);
+                    load_as_float<float, V>(w + at1[j], w1);
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        const float y0 = x0[j][e], y1 = x1[j][e];
-                        x0[j][e] = y0 * c[j][e] - y1 * s[j][e];
-                        x1[j][e] = y1 * c[j][e] + y0 * s[j][e];
+                        x0[j][e] = x0[j][e] * r * w0[e];
+                        x1[j][e] = x1[j][e] * r * w1[e];
                     }
                 }
-                if (APPEND && kind > 0) {
-                    if (row >= 0) {
-                        C *dst = static_cast<C *>(a.cache[kind - 1]) + row + h * a.pages.head_stride;
-                        store_rounded<C, V>(dst + at0[j], x0[j]);
-                        store_rounded<C, V>(dst + at1[j], x1[j]);
-                    }
-                } else {
-                    T *dst = static_cast<T *>(a.out[kind]) + t * a.out_stride[kind] + h * a.D;
-                    store_rounded<T, V>(dst + at0[j], x0[j]);
-                    store_rounded<T, V>(dst + at1[j], x1[j]);
+            }
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            if (!has[j]) continue;
+            if (turned[j] && kind < 2) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float y0 = x0[j][e], y1 = x1[j][e];
+                    x0[j][e] = y0 * c[j][e] - y1 * s[j][e];
+                    x1[j][e] = y1 * c[j][e] + y0 * s[j][e];
                 }
+            }
+            if (APPEND && kind > 0) {
+                if (row >= 0) {
+                    C *dst = static_cast<C *>(a.cache[kind - 1]) + row + h * a.pages.head_stride;
+                    store_rounded<C, V>(dst + at0[j], x0[j]);
+                    store_rounded<C, V>(dst + at1[j], x1[j]);
+                }
+            } else {
+                T *dst = static_cast<T *>(a.out[kind]) + t * a.out_stride[kind] + h * a.D;
+                store_rounded<T, V>(dst + at0[j], x0[j]);
+                store_rounded<T, V>(dst + at1[j], x1[j]);
             }
         }
     }
@@ -183,15 +203,10 @@ void launch_heads(HeadArgs a, bool wide, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const int lph = wide ? a.D / (2 * V) : 64;
     const int iters = (a.heads[0] + a.heads[1] + a.heads[2] + 64 / lph - 1) / (64 / lph);
-    // A token's heads are shared by as many waves as it takes to give every CU eight of them.
-    const int64_t want = int64_t{8} * device_cu_count();
-    a.split = static_cast<int>(std::min<int64_t>(iters, std::max<int64_t>(1, want / a.n_tokens)));
-    const int64_t waves = static_cast<int64_t>(a.n_tokens) * a.split;
-    int64_t blocks = std::min<int64_t>((waves + kHeadWaves - 1) / kHeadWaves, int64_t{8} * device_cu_count());
-    // (the token loop steps by waves / split, so the waves have to be a multiple of split)
-    const int64_t step = a.split;
-    blocks = (blocks + step - 1) / step * step;
-    const dim3 grid(static_cast<unsigned>(blocks));
+    // A wave takes up to kHeadRounds rounds of heads, fewer where that gives every CU eight waves.
+    const int64_t want = int64_t{8} * device_cu_count() / a.n_tokens;
+    a.split = static_cast<int>(std::max<int64_t>((iters + kHeadRounds - 1) / kHeadRounds, std::min<int64_t>(iters, want)));
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.n_tokens) * a.split + kHeadWaves - 1) / kHeadWaves));
     if (!wide) {
         heads_kernel<T, C, 1, 64, APPEND><<<grid, kHeadThreads, 0, s>>>(a);
         return;
@@ -235,6 +250,7 @@ int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip
                 (lanes & (lanes - 1)) == 0;
     for (int i = 0; i < 3; ++i)
         if (a.heads[i]) wide = wide && aligned(a.in[i], a.in_stride[i], bytes);
+    for (const float *f : {p.q_bias, p.k_bias, p.v_bias, p.q_norm, p.k_norm}) wide = wide && aligned(f, 0, 4);
     if (q) wide = wide && aligned(p.q_out, a.out_stride[0], bytes);
     if (!cache) {
         if (k) wide = wide && aligned(p.k_out, a.out_stride[1], bytes);

@@ -129,13 +129,6 @@ __device__ inline bool make_finite(vec<C, 8> &x) {
     return finite;
 }
 
-// LDS that only one wave uses: what its lanes wrote is there for all of them (a wave's LDS accesses complete in order; this
-// keeps the compiler from reordering them).
-__device__ inline void wave_lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Weights are 2^(s c + bias): with fp16 terms they are held 2^8 times larger, above fp16's subnormals.
 template <typename E>
 constexpr float kWeightShift = std::is_same_v<E, f16> ? 8.0f : 0.0f;
@@ -675,11 +668,8 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
 template <typename T, int D>
 __global__ __launch_bounds__(64) void attn_join(AttnArgs a) {
     const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-    const int b = last_start_at_or_before(a.q_start, a.n_seqs, token);
-    if (b < 0) return;
-    const int end = a.q_start[b + 1];
-    if (token >= end) return;
-    const int pos = a.kv_len[b] - (end - token);
+    int b, pos;
+    if (!find_token(a.q_start, a.kv_len, a.n_seqs, token, b, pos)) return;
     const int len = min(a.kv_len[b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
     const int lo = key_lo(a, pos), hi = key_hi(a, pos, len);
     const int z0 = min(lo / a.span, a.parts - 1), z1 = hi > lo ? min((hi - 1) / a.span + 1, a.parts) : z0;
