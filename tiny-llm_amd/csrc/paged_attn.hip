@@ -129,6 +129,24 @@ __device__ inline bool make_finite(vec<C, 8> &x) {
     return finite;
 }
 
+// 16 bytes per lane from global memory to LDS, lane after lane from `to` (the same in all lanes), without passing through
+// registers; wait_loads waits for all that the wave has under way.
+__device__ const int kZeros[4] = {0, 0, 0, 0};
+template <typename T, typename E>
+__device__ inline void global_to_lds(const T *from, E *to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+__device__ inline void wait_loads() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// A row's sums are brought down to a new maximum only once it exceeds the one they stand at by 2^kHeadroom: the weights stay
+// within fp16's range, and what their sums lose by it is nothing, since a factor of a power of two is common to all of them.
+constexpr float kHeadroom = 7.0f;
+
 // Weights are 2^(s c + bias): with fp16 terms they are held 2^8 times larger, above fp16's subnormals.
 template <typename E>
 constexpr float kWeightShift = std::is_same_v<E, f16> ? 8.0f : 0.0f;
@@ -314,7 +332,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kt][i]);
         mx = fmaxf(mx, lane_xor<16>(mx, lane));
         mx = fmaxf(mx, lane_xor<32>(mx, lane));
-        if (__ballot(mx != m)) {
+        if (__ballot((mx - m) * c > kHeadroom)) {
             const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
             const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
             m = mx;
@@ -441,10 +459,13 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     using E = typename Tm::E;
     constexpr int QT = Tm::QT, KT = Tm::KT, BN = TileShape<T, C, D>::BN;
     constexpr int NCH = BN * (D / 8) / 256;  // chunks of 8 elements per thread
-    constexpr int KS = D + 8, VS = D + 16;   // row strides: reads of 16 rows touch every bank once
-    constexpr int NK = BN / 32, ND = D / 32;
-    __shared__ __attribute__((aligned(16))) E ks[KT][BN][KS];
-    __shared__ __attribute__((aligned(16))) E vs[KT][BN][VS];
+    constexpr int NK = BN / 32, ND = D / 32, CH = D / 8;
+    // The tile's rows as they are, two buffers, when the cache holds the instruction's type; else one buffer of terms. A row's chunks
+    // of 16 bytes are permuted by an exclusive or (key_swap, value_swap) so that the reads below meet every bank once.
+    constexpr bool kDirect = KT == 1;
+    constexpr int kPlanes = kDirect ? 2 : KT;
+    __shared__ __attribute__((aligned(16))) E ks[kPlanes][BN][D];
+    __shared__ __attribute__((aligned(16))) E vs[kPlanes][BN][D];
     __shared__ int64_t offs[2][BN];
     __shared__ unsigned long long here[2];  // which of the tile's keys exist
     __shared__ unsigned long long wild[2];  // keys of a partly masked tile whose values are not all finite
@@ -484,17 +505,32 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
                                                      [&](float x) { return fmaxf(x, lane_xor<32>(x, lane)); });
     const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride;
     const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride;
-    vec<C, 8> kr[NCH], vr[NCH];
-    const auto load_tile = [&](int buf) {
+    const auto key_swap = [](int row) { return (D == 64 ? row >> 1 : row) & (D == 64 ? 7 : 15); };
+    const auto value_swap = [](int row) { return (row & 3) << 1; };
+    vec<C, 8> kr[kDirect ? 1 : NCH], vr[kDirect ? 1 : NCH];
+    // A tile's rows (at the offsets `from`) on their way: straight into LDS, 64 chunks in order per instruction, the lane choosing the
+    // global chunk that belongs at its place (a row that does not exist: zeros), or into registers.
+    const auto load_tile = [&](const int64_t *__restrict__ from, E *__restrict__ k_to, E *__restrict__ v_to)
+                               __attribute__((always_inline)) {
+        int64_t o[NCH];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) o[i] = from[(tid + 256 * i) / CH];
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int ch = tid + 256 * i;
-            const int64_t o = offs[buf][ch / (D / 8)];
-            kr[i] = vec<C, 8>{};
-            vr[i] = vec<C, 8>{};
-            if (o >= 0) {
-                kr[i] = *reinterpret_cast<const vec<C, 8> *>(kc + o + ch % (D / 8) * 8);
-                vr[i] = *reinterpret_cast<const vec<C, 8> *>(vc + o + ch % (D / 8) * 8);
+            const int ch = tid + 256 * i, row = ch / CH, at = ch % CH;
+            if constexpr (kDirect) {
+                const int first = (wave * 64 + 256 * i) * 8;  // element of the wave's first chunk
+                const C *k = o[i] >= 0 ? kc + o[i] + (at ^ key_swap(row)) * 8 : reinterpret_cast<const C *>(kZeros);
+                const C *v = o[i] >= 0 ? vc + o[i] + (at ^ value_swap(row)) * 8 : reinterpret_cast<const C *>(kZeros);
+                global_to_lds(k, k_to + first);
+                global_to_lds(v, v_to + first);
+            } else {
+                kr[i] = vec<C, 8>{};
+                vr[i] = vec<C, 8>{};
+                if (o[i] >= 0) {
+                    kr[i] = *reinterpret_cast<const vec<C, 8> *>(kc + o[i] + at * 8);
+                    vr[i] = *reinterpret_cast<const vec<C, 8> *>(vc + o[i] + at * 8);
+                }
             }
         }
     };
@@ -517,35 +553,19 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
 
     put_offset(0, key_offset(kb + tid));
     __syncthreads();
-    if (kb < ke) load_tile(0);
+    if (kb < ke) load_tile(offs[0], &ks[0][0][0], &vs[0][0][0]);
     int64_t next_off = key_offset(kb + BN + tid);
-    int buf = 0;
-    for (int k0 = kb; k0 < ke; k0 += BN, buf ^= 1) {
-        if (k0 != kb) __syncthreads();  // the last tile has been read
-        const bool partial = k0 < full_lo || k0 + BN > full_hi;  // some row of the block masks some key
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int ch = tid + 256 * i, row = ch / (D / 8), at = ch % (D / 8) * 8;
-            if (partial) {
-                // An infinite or NaN value would reach rows that mask its key through a product with their weight of zero.
-                // It goes into the products as zero and is added below where its key is seen.
-                if (!make_finite<C>(vr[i])) atomicOr(&wild[buf], 1ull << row);
-            }
-            vec<E, 8> terms[KT];
-            as_terms<C, E, KT>(kr[i], terms);
-#pragma unroll
-            for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&ks[n][row][at]) = terms[n];
-            as_terms<C, E, KT>(vr[i], terms);
-#pragma unroll
-            for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&vs[n][row][at]) = terms[n];
-        }
-        put_offset(buf ^ 1, next_off);
-        __syncthreads();
+    constexpr int kPlane = BN * D;
+    const auto step = [&](int k0, bool partial, const E *__restrict__ kcur, const E *__restrict__ vcur, const int64_t *__restrict__ offs_cur,
+                          const int64_t *__restrict__ offs_next, const unsigned long long *__restrict__ here_cur,
+                          const unsigned long long *__restrict__ wild_cur, E *__restrict__ knext, E *__restrict__ vnext)
+                          __attribute__((always_inline)) {
+        const unsigned long long exist = *here_cur;
         if (k0 + BN < ke) {
-            load_tile(buf ^ 1);
+            load_tile(offs_next, knext, vnext);
             next_off = key_offset(k0 + 2 * BN + tid);
         }
-        if (!wave_live || k0 >= w_hi || k0 + BN <= w_lo) continue;
+        if (!wave_live || k0 >= w_hi || k0 + BN <= w_lo) return;
 
         // S^T: keys down, queries across; the lane holds its query's keys 32 kt + (i % 4) + 8 (i / 4) + 4 h
         f32x16 s[NK];
@@ -556,14 +576,15 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
             for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
                 for (int kj = 0; kj < KT; ++kj) {
-                    const vec<E, 8> kf = *reinterpret_cast<const vec<E, 8> *>(&ks[kj][32 * kt + col][16 * i + 8 * h]);
+                    const vec<E, 8> kf =
+                        *reinterpret_cast<const vec<E, 8> *>(kcur + kj * kPlane + (32 * kt + col) * D + ((2 * i + h) ^ key_swap(col)) * 8);
 #pragma unroll
                     for (int qi = 0; qi < QT; ++qi)
                         if (qi + kj < Tm::kMost) s[kt] = mfma32(kf, q[qi][i], s[kt]);
                 }
             }
         }
-        const unsigned long long exist = here[buf];
+        
         const bool all_here = BN == 64 ? exist == ~0ull : (exist & 0xffffffffull) == 0xffffffffull;
         if (k0 < wf_lo || k0 + BN > wf_hi || !all_here) {
             // which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
@@ -582,7 +603,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
         mx = fmaxf(mx, lane_xor<32>(mx, lane));
-        if (__ballot(mx != m)) {  // a row's maximum moved: what is summed is brought down to the new one
+        if (__ballot((mx - m) * c > kHeadroom)) {
             const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
             const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
             m = mx;
@@ -612,9 +633,10 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
                     for (int d = 0; d < ND; ++d) {
 #pragma unroll
                         for (int kj = 0; kj < KT; ++kj) {
-                            const E *v0 = &vs[kj][32 * kt + 16 * half + 4 * h + (lane & 15) / 4]
-                                             [32 * d + (lane & 16) + 4 * (lane & 3)];
-                            const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * VS);
+                            const int i = lane & 15, row = 32 * kt + 16 * half + 4 * h + i / 4;
+                            const int ch = (4 * d + (lane & 16) / 8 + (i & 3) / 2) ^ value_swap(i / 4);
+                            const E *v0 = vcur + kj * kPlane + row * D + ch * 8 + 4 * (i & 1);
+                            const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * D);
                             const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                             for (int qi = 0; qi < QT; ++qi)
@@ -622,10 +644,10 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
                         }
                     }
                 }
-        for (unsigned long long w = partial ? wild[buf] : 0; w; w &= w - 1) {
+        for (unsigned long long w = partial ? *wild_cur : 0; w; w &= w - 1) {
             const int j = __builtin_ctzll(w), key = k0 + j;
             if (key < lo || key >= hi) continue;
-            const C *v0 = vc + offs[buf][j] + 4 * h;
+            const C *v0 = vc + offs_cur[j] + 4 * h;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -634,6 +656,49 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
                     if (!is_finite<C>(x)) acc[d][e] += static_cast<float>(x);
                 }
         }
+    };
+    int buf = 0;
+    for (int k0 = kb; k0 < ke; k0 += BN, buf ^= 1) {
+        // An infinite or NaN value would reach rows that mask its key through a product with their weight of zero: where some
+        // row of the block masks some key, it goes into the products as zero and is added below where its key is seen.
+        const bool partial = k0 < full_lo || k0 + BN > full_hi;
+        if constexpr (kDirect) {
+            put_offset(buf ^ 1, next_off);
+            wait_loads();  // the wave's part of this tile
+            __syncthreads();
+            if (partial) {
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const int ch = tid + 256 * i;
+                    vec<C, 8> *p = reinterpret_cast<vec<C, 8> *>(&vs[buf][0][0]) + ch;
+                    vec<C, 8> x = *p;
+                    if (!make_finite<C>(x)) {
+                        *p = x;
+                        atomicOr(&wild[buf], 1ull << (ch / CH));
+                    }
+                }
+                __syncthreads();
+            }
+        } else {
+            if (k0 != kb) __syncthreads();  // the last tile has been read
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int ch = tid + 256 * i, row = ch / CH, at = ch % CH;
+                if (partial && !make_finite<C>(vr[i])) atomicOr(&wild[buf], 1ull << row);
+                vec<E, 8> terms[KT];
+                as_terms<C, E, KT>(kr[i], terms);
+#pragma unroll
+                for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&ks[n][row][(at ^ key_swap(row)) * 8]) = terms[n];
+                as_terms<C, E, KT>(vr[i], terms);
+#pragma unroll
+                for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&vs[n][row][(at ^ value_swap(row)) * 8]) = terms[n];
+            }
+            put_offset(buf ^ 1, next_off);
+            __syncthreads();
+        }
+        // (distinct restrict pointers: without them the compiler waits for the next tile before it reads this one)
+        step(k0, partial, &ks[kDirect ? buf : 0][0][0], &vs[kDirect ? buf : 0][0][0], offs[buf], offs[buf ^ 1], &here[buf], &wild[buf],
+             &ks[kDirect ? buf ^ 1 : 0][0][0], &vs[kDirect ? buf ^ 1 : 0][0][0]);
     }
     if (wr0 + col >= rows) return;
     l += lane_xor<32>(l, lane);
