@@ -116,15 +116,18 @@ struct Pages {
     int64_t page_stride, token_stride, head_stride;
 };
 
-// Element offset of position p of sequence b (head 0), or -1 where it does not exist.
-__device__ inline int64_t row_offset(const Pages &g, int b, int p) {
-    if (p < 0) return -1;
-    const int i = g.page_size.quot(p);
-    if (i >= g.table_stride) return -1;
-    const int page = g.table[static_cast<int64_t>(b) * g.table_stride + i];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(g.n_pages)) return -1;
-    return page * g.page_stride + (p - i * static_cast<int>(g.page_size.d)) * g.token_stride;
+// The page number of position p of sequence b as the table has it (-1 past the table and before position 0), and the element
+// offset (head 0) of the position's row, -1 where it does not exist. Two steps, so that a kernel can have the page under way
+// while it computes: what is done with a loaded value, even a comparison, waits for it and for every load before it.
+__device__ inline int page_number(const Pages &g, int b, int p) {
+    const int i = p < 0 ? 0x7fffffff : g.page_size.quot(p);
+    return i < g.table_stride ? g.table[static_cast<int64_t>(b) * g.table_stride + i] : -1;
 }
+__device__ inline int64_t row_in_page(const Pages &g, int page, int p) {
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(g.n_pages)) return -1;
+    return page * g.page_stride + (p - g.page_size.quot(p) * static_cast<int>(g.page_size.d)) * g.token_stride;
+}
+__device__ inline int64_t row_offset(const Pages &g, int b, int p) { return row_in_page(g, page_number(g, b, p), p); }
 
 // The cache's strides with the contiguous layout for zeros; false: not a layout in which every row is apart.
 inline bool cache_strides(const tqhip_kv_cache &c, int64_t *page, int64_t *token, int64_t *head) {

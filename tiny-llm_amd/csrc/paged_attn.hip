@@ -85,6 +85,20 @@ __device__ inline f32x16 mfma32(vec<bf16, 8> a, vec<bf16, 8> b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+// l plus the eight elements, two at a time.
+__device__ inline float add_all(vec<f16, 8> p, float l) {
+    const vec<f16, 2> ones{static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(vec<f16, 2>{p[i], p[i + 1]}, ones, l, false);
+    return l;
+}
+__device__ inline float add_all(vec<bf16, 8> p, float l) {
+    const vec<bf16, 2> ones{static_cast<bf16>(1.0f), static_cast<bf16>(1.0f)};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2_f32_bf16(vec<bf16, 2>{p[i], p[i + 1]}, ones, l, false);
+    return l;
+}
+
 // Four rows of 16 elements each, held 4 elements a lane by 16 lanes, as columns: lane i gets column i's four.
 template <typename E>
 __device__ inline vec<E, 4> lds_columns(const E *p) {
@@ -98,6 +112,13 @@ __device__ inline bool is_finite(C x) {
         return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
     constexpr unsigned short kExp = std::is_same_v<C, f16> ? 0x7c00 : 0x7f80;
     return (__builtin_bit_cast(vec<unsigned short, sizeof(C) / 2>, x)[0] & kExp) != kExp;
+}
+
+// A value that all lanes of the wave hold.
+__device__ inline unsigned long long scalar(unsigned long long v) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
+    const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v >> 32));
+    return static_cast<unsigned long long>(hi) << 32 | lo;
 }
 
 // Bits below n (none for n <= 0, all from 32 on).
@@ -131,7 +152,6 @@ __device__ inline bool make_finite(vec<C, 8> &x) {
 
 // 16 bytes per lane from global memory to LDS, lane after lane from `to` (the same in all lanes), without passing through
 // registers; wait_loads waits for all that the wave has under way.
-__device__ const int kZeros[4] = {0, 0, 0, 0};
 template <typename T, typename E>
 __device__ inline void global_to_lds(const T *from, E *to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
@@ -255,12 +275,16 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride + 8 * g;
     vec<C, 8> kr[2][NS], vr[2][NS];
     // the lane's keys of a step: k0 + col and k0 + 16 + col
-    const auto offsets = [&](int k0, int64_t *o) {
+    const auto pages_of = [&](int k0, int *page) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             const int key = k0 + 16 * kt + col;
-            o[kt] = key < ke ? row_offset(a.pages, t.b, key) : -1;
+            page[kt] = key < ke ? page_number(a.pages, t.b, key) : -1;
         }
+    };
+    const auto offsets = [&](int k0, const int *page, int64_t *o) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) o[kt] = row_in_page(a.pages, page[kt], k0 + 16 * kt + col);
     };
     const auto load_rows = [&](const C *base, const int64_t *o, vec<C, 8> (*x)[NS]) {
 #pragma unroll
@@ -274,12 +298,14 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
         }
     };
 
-    int64_t off[2], next[2];
+    int64_t off[2];
+    int next[2];
     int k0 = kb + wave * kFewKeys;
-    offsets(k0, off);
+    pages_of(k0, next);
+    offsets(k0, next, off);
+    pages_of(k0 + kFewStep, next);
     load_rows(kc, off, kr);
     load_rows(vc, off, vr);
-    offsets(k0 + kFewStep, next);
     vec<E, 8> q[QT][NS];
     const float c = load_query<T, E, QT, NS, 32>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * g, q,
                                                  [&](float x) {
@@ -312,10 +338,9 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
                                static_cast<unsigned>(__ballot(off[1] >= 0) & 0xffff) << 16;
         const bool partial = k0 < full_lo || k0 + kFewKeys > full_hi;
         const int64_t was[2] = {off[0], off[1]};
-        off[0] = next[0];
-        off[1] = next[1];
+        offsets(k0 + kFewStep, next, off);
+        pages_of(k0 + 2 * kFewStep, next);
         load_rows(kc, off, kr);
-        offsets(k0 + 2 * kFewStep, next);
         if (partial || exist != ~0u) {
             const int k1 = k0 + 4 * g;
             const unsigned may = (exist >> (4 * g)) & below(hi - k1) & ~below(lo - k1);
@@ -459,18 +484,22 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     using E = typename Tm::E;
     constexpr int QT = Tm::QT, KT = Tm::KT, BN = TileShape<T, C, D>::BN;
     constexpr int NCH = BN * (D / 8) / 256;  // chunks of 8 elements per thread
-    constexpr int NK = BN / 32, ND = D / 32, CH = D / 8;
+    constexpr int NK = BN / 32, ND = D / 32, CH = D / 8, kTiles = 256 / BN;
     // The tile's rows as they are, two buffers, when the cache holds the instruction's type; else one buffer of terms. A row's chunks
     // of 16 bytes are permuted by an exclusive or (key_swap, value_swap) so that the reads below meet every bank once.
     constexpr bool kDirect = KT == 1;
     constexpr int kPlanes = kDirect ? 2 : KT;
-    __shared__ __attribute__((aligned(16))) E ks[kPlanes][BN][D];
-    __shared__ __attribute__((aligned(16))) E vs[kPlanes][BN][D];
-    __shared__ int64_t offs[2][BN];
-    __shared__ unsigned long long here[2];  // which of the tile's keys exist
-    __shared__ unsigned long long wild[2];  // keys of a partly masked tile whose values are not all finite
+    // (One object: with several, the compiler holds the transfers to one of them against the reads of the others, and waits for the
+    // next tile before it reads this one. What has to be waited for is waited for below.)
+    __shared__ struct {
+        __attribute__((aligned(16))) E k[kPlanes][BN][D];
+        __attribute__((aligned(16))) E v[kPlanes][BN][D];
+        int64_t offs[2][256];           // element offsets of the rows of 256 keys, several tiles, and of the next 256
+        unsigned long long here[2][4];  // which of those keys exist
+        unsigned long long wild[2];     // keys of a partly masked tile whose values are not all finite
+    } sh;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, col = lane & 31;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, col = lane & 31;
     const int kv_heads = a.n_heads / a.group;
     const int kvh = blockIdx.x % kv_heads;
     const int tile = gridDim.x / kv_heads - 1 - static_cast<int>(blockIdx.x) / kv_heads;  // the longest first
@@ -498,7 +527,6 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     const bool wave_live = wr0 < rows;
     const int wp_first = t.pos0 + min(wr0, rows - 1) / a.group, wp_last = t.pos0 + min(wr0 + 31, rows - 1) / a.group;
     const int w_lo = key_lo(a, wp_first), w_hi = key_hi(a, wp_last, t.len);
-    const int wf_lo = key_lo(a, wp_last), wf_hi = key_hi(a, wp_first, t.len);
 
     vec<E, 8> q[QT][D / 16];
     const float c = load_query<T, E, QT, D / 16, 16>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * h, q,
@@ -508,10 +536,10 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     const auto key_swap = [](int row) { return (D == 64 ? row >> 1 : row) & (D == 64 ? 7 : 15); };
     const auto value_swap = [](int row) { return (row & 3) << 1; };
     vec<C, 8> kr[kDirect ? 1 : NCH], vr[kDirect ? 1 : NCH];
-    // A tile's rows (at the offsets `from`) on their way: straight into LDS, 64 chunks in order per instruction, the lane choosing the
-    // global chunk that belongs at its place (a row that does not exist: zeros), or into registers.
-    const auto load_tile = [&](const int64_t *__restrict__ from, E *__restrict__ k_to, E *__restrict__ v_to)
-                               __attribute__((always_inline)) {
+    // A tile's rows on their way: straight into LDS, 64 chunks in order per instruction, the lane choosing the global chunk that belongs
+    // at its place, or into registers. For a key that does not exist row 0 of page 0 is loaded.
+    const auto load_tile = [&](int n, E *__restrict__ k_to, E *__restrict__ v_to) __attribute__((always_inline)) {
+        const int64_t *from = sh.offs[n / kTiles & 1] + n % kTiles * BN;
         int64_t o[NCH];
 #pragma unroll
         for (int i = 0; i < NCH; ++i) o[i] = from[(tid + 256 * i) / CH];
@@ -520,30 +548,24 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
             const int ch = tid + 256 * i, row = ch / CH, at = ch % CH;
             if constexpr (kDirect) {
                 const int first = (wave * 64 + 256 * i) * 8;  // element of the wave's first chunk
-                const C *k = o[i] >= 0 ? kc + o[i] + (at ^ key_swap(row)) * 8 : reinterpret_cast<const C *>(kZeros);
-                const C *v = o[i] >= 0 ? vc + o[i] + (at ^ value_swap(row)) * 8 : reinterpret_cast<const C *>(kZeros);
-                global_to_lds(k, k_to + first);
-                global_to_lds(v, v_to + first);
+                global_to_lds(kc + o[i] + (at ^ key_swap(row)) * 8, k_to + first);
+                global_to_lds(vc + o[i] + (at ^ value_swap(row)) * 8, v_to + first);
             } else {
-                kr[i] = vec<C, 8>{};
-                vr[i] = vec<C, 8>{};
-                if (o[i] >= 0) {
-                    kr[i] = *reinterpret_cast<const vec<C, 8> *>(kc + o[i] + at * 8);
-                    vr[i] = *reinterpret_cast<const vec<C, 8> *>(vc + o[i] + at * 8);
-                }
+                kr[i] = *reinterpret_cast<const vec<C, 8> *>(kc + o[i] + at * 8);
+                vr[i] = *reinterpret_cast<const vec<C, 8> *>(vc + o[i] + at * 8);
             }
         }
     };
-    const auto key_offset = [&](int key) { return tid < BN && key < ke ? row_offset(a.pages, t.b, key) : -1; };
-    const auto put_offset = [&](int buf, int64_t o) {
-        if (wave == 0) {
-            const unsigned long long m = __ballot(o >= 0);
-            if (tid < BN) offs[buf][tid] = o;
-            if (tid == 0) {
-                here[buf] = m;
-                wild[buf] = 0;
-            }
-        }
+    // 256 keys' pages are looked up while the tiles of the 256 before run, and their offsets put into LDS before the last of those.
+    const auto key_page = [&](int n) {
+        const int key = kb + n * 256 + tid;
+        return key < ke ? page_number(a.pages, t.b, key) : -1;
+    };
+    const auto put_offsets = [&](int n, int page) {
+        const int64_t o = row_in_page(a.pages, page, kb + n * 256 + tid);
+        const unsigned long long m = __ballot(o >= 0);
+        sh.offs[n & 1][tid] = max(o, int64_t{0});
+        if (lane == 0) sh.here[n & 1][wave] = m;
     };
 
     f32x16 acc[ND];
@@ -551,103 +573,95 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     for (int i = 0; i < ND; ++i) acc[i] = f32x16{};
     float m = -INFINITY, bias = 0.0f, l = 0.0f;
 
-    put_offset(0, key_offset(kb + tid));
+    put_offsets(0, key_page(0));
+    if (tid < 2) sh.wild[tid] = 0;
     __syncthreads();
-    if (kb < ke) load_tile(offs[0], &ks[0][0][0], &vs[0][0][0]);
-    int64_t next_off = key_offset(kb + BN + tid);
-    constexpr int kPlane = BN * D;
-    const auto step = [&](int k0, bool partial, const E *__restrict__ kcur, const E *__restrict__ vcur, const int64_t *__restrict__ offs_cur,
-                          const int64_t *__restrict__ offs_next, const unsigned long long *__restrict__ here_cur,
-                          const unsigned long long *__restrict__ wild_cur, E *__restrict__ knext, E *__restrict__ vnext)
-                          __attribute__((always_inline)) {
-        const unsigned long long exist = *here_cur;
-        if (k0 + BN < ke) {
-            load_tile(offs_next, knext, vnext);
-            next_off = key_offset(k0 + 2 * BN + tid);
-        }
+    if (kb < ke) load_tile(0, &sh.k[0][0][0], &sh.v[0][0][0]);
+    int next_page = key_page(1);
+    // (The restrict pointers tell the compiler that the next tile's transfers do not touch the values that are read meanwhile.)
+    const auto step = [&](int n, int k0, bool partial, unsigned long long exist, const E *__restrict__ v_now, E *__restrict__ k_next,
+                          E *__restrict__ v_next) __attribute__((always_inline)) {
+        const int buf = n & 1;
+        if (k0 + BN < ke) load_tile(n + 1, k_next, v_next);
         if (!wave_live || k0 >= w_hi || k0 + BN <= w_lo) return;
 
-        // S^T: keys down, queries across; the lane holds its query's keys 32 kt + (i % 4) + 8 (i / 4) + 4 h
-        f32x16 s[NK];
-#pragma unroll
-        for (int kt = 0; kt < NK; ++kt) {
-            s[kt] = f32x16{};
+        // 32 keys at a time: the score products of the next 32 run on the matrix cores while the vector units form the weights of
+        // these. S^T, keys down, queries across: the lane holds its query's keys (i % 4) + 8 (i / 4) + 4 h.
+        const auto scores = [&](int kt) {
+            f32x16 s{};
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
                 for (int kj = 0; kj < KT; ++kj) {
-                    const vec<E, 8> kf =
-                        *reinterpret_cast<const vec<E, 8> *>(kcur + kj * kPlane + (32 * kt + col) * D + ((2 * i + h) ^ key_swap(col)) * 8);
+                    const vec<E, 8> kf = *reinterpret_cast<const vec<E, 8> *>(
+                        &sh.k[kDirect ? buf : kj][32 * kt + col][((2 * i + h) ^ key_swap(col)) * 8]);
 #pragma unroll
                     for (int qi = 0; qi < QT; ++qi)
-                        if (qi + kj < Tm::kMost) s[kt] = mfma32(kf, q[qi][i], s[kt]);
+                        if (qi + kj < Tm::kMost) s = mfma32(kf, q[qi][i], s);
                 }
             }
-        }
-        
-        const bool all_here = BN == 64 ? exist == ~0ull : (exist & 0xffffffffull) == 0xffffffffull;
-        if (k0 < wf_lo || k0 + BN > wf_hi || !all_here) {
-            // which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
-#pragma unroll
-            for (int kt = 0; kt < NK; ++kt) {
-                const int k1 = k0 + 32 * kt + 4 * h;
-                const unsigned may = static_cast<unsigned>(exist >> (32 * kt + 4 * h)) & below(hi - k1) & ~below(lo - k1);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[kt][i] = -INFINITY;
-            }
-        }
-        float mx = m;
-#pragma unroll
-        for (int kt = 0; kt < NK; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
-        mx = fmaxf(mx, lane_xor<32>(mx, lane));
-        if (__ballot((mx - m) * c > kHeadroom)) {
-            const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
-            const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
-            m = mx;
-            bias = nb;
-            l *= f;
-#pragma unroll
-            for (int i = 0; i < ND; ++i) acc[i] *= f;
-        }
+            return s;
+        };
+        f32x16 s = scores(0), ahead{};
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt) {
+            const int k1 = k0 + 32 * kt;
+            const unsigned exists = static_cast<unsigned>(exist >> (32 * kt));
+            if (partial) {
+                // which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
+                const unsigned may = (exists >> (4 * h)) & below(hi - k1 - 4 * h) & ~below(lo - k1 - 4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = -INFINITY;
+            }
+            float mx = m;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+            mx = fmaxf(mx, lane_xor<32>(mx, lane));
+            if (__ballot((mx - m) * c > kHeadroom)) {
+                const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
+                const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
+                m = mx;
+                bias = nb;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) acc[i] *= f;
+            }
+            if (kt + 1 < NK) ahead = scores(kt + 1);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[kt][i] = __builtin_amdgcn_exp2f(fmaf(s[kt][i], c, bias));
-                l += s[kt][i];
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, bias));
+                if (QT > 1) l += s[i];
             }
-        }
 #pragma unroll
-            for (int kt = 0; kt < NK; ++kt)
+            for (int half = 0; half < 2; ++half) {
+                float x[8];
+                vec<E, 8> p[QT];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float x[8];
-                    vec<E, 8> p[QT];
+                for (int e = 0; e < 8; ++e) x[e] = s[8 * half + e];
+                split<E, QT>(x, p);
+                if (QT == 1) l = add_all(p[0], l);  // (what the products sum, so the rounding of the weights cancels in part)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = s[kt][8 * half + e];
-                    split<E, QT>(x, p);
+                for (int d = 0; d < ND; ++d) {
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) {
+                    for (int kj = 0; kj < KT; ++kj) {
+                        const int i = lane & 15, row = 32 * kt + 16 * half + 4 * h + i / 4;
+                        const int ch = (4 * d + (lane & 16) / 8 + (i & 3) / 2) ^ value_swap(i / 4);
+                        const E *v0 = v_now + kj * BN * D + row * D + ch * 8 + 4 * (i & 1);
+                        const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * D);
+                        const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                        for (int kj = 0; kj < KT; ++kj) {
-                            const int i = lane & 15, row = 32 * kt + 16 * half + 4 * h + i / 4;
-                            const int ch = (4 * d + (lane & 16) / 8 + (i & 3) / 2) ^ value_swap(i / 4);
-                            const E *v0 = vcur + kj * kPlane + row * D + ch * 8 + 4 * (i & 1);
-                            const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * D);
-                            const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                            for (int qi = 0; qi < QT; ++qi)
-                                if (qi + kj < Tm::kMost) acc[d] = mfma32(vf, p[qi], acc[d]);
-                        }
+                        for (int qi = 0; qi < QT; ++qi)
+                            if (qi + kj < Tm::kMost) acc[d] = mfma32(vf, p[qi], acc[d]);
                     }
                 }
-        for (unsigned long long w = partial ? *wild_cur : 0; w; w &= w - 1) {
+            }
+            s = ahead;
+        }
+        for (unsigned long long w = partial ? sh.wild[buf] : 0; w; w &= w - 1) {
             const int j = __builtin_ctzll(w), key = k0 + j;
-            if (key < lo || key >= hi) continue;
-            const C *v0 = vc + offs_cur[j] + 4 * h;
+            if (key < lo || key >= hi || !(exist >> j & 1)) continue;
+            const C *v0 = vc + sh.offs[n / kTiles & 1][n % kTiles * BN + j] + 4 * h;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -657,48 +671,52 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
                 }
         }
     };
-    int buf = 0;
-    for (int k0 = kb; k0 < ke; k0 += BN, buf ^= 1) {
+    for (int n = 0, k0 = kb; k0 < ke; k0 += BN, ++n) {
+        const int buf = n & 1;
+        const unsigned long long all = BN == 64 ? ~0ull : 0xffffffffull;
+        const unsigned long long exist = scalar(sh.here[n / kTiles & 1][n % kTiles * BN / 64]) >> (BN == 64 ? 0 : n % 2 * 32) & all;
         // An infinite or NaN value would reach rows that mask its key through a product with their weight of zero: where some
         // row of the block masks some key, it goes into the products as zero and is added below where its key is seen.
-        const bool partial = k0 < full_lo || k0 + BN > full_hi;
+        const bool partial = k0 < full_lo || k0 + BN > full_hi || exist != all;
+        if (n % kTiles == kTiles - 1) {
+            put_offsets(n / kTiles + 1, next_page);
+            next_page = key_page(n / kTiles + 2);
+        }
         if constexpr (kDirect) {
-            put_offset(buf ^ 1, next_off);
             wait_loads();  // the wave's part of this tile
             __syncthreads();
             if (partial) {
 #pragma unroll
                 for (int i = 0; i < NCH; ++i) {
                     const int ch = tid + 256 * i;
-                    vec<C, 8> *p = reinterpret_cast<vec<C, 8> *>(&vs[buf][0][0]) + ch;
+                    vec<C, 8> *p = reinterpret_cast<vec<C, 8> *>(&sh.v[buf][0][0]) + ch;
                     vec<C, 8> x = *p;
                     if (!make_finite<C>(x)) {
                         *p = x;
-                        atomicOr(&wild[buf], 1ull << (ch / CH));
+                        atomicOr(&sh.wild[buf], 1ull << (ch / CH));
                     }
                 }
                 __syncthreads();
             }
+            if (tid == 0) sh.wild[buf ^ 1] = 0;
         } else {
             if (k0 != kb) __syncthreads();  // the last tile has been read
+            if (tid == 0) sh.wild[buf ^ 1] = 0;
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 const int ch = tid + 256 * i, row = ch / CH, at = ch % CH;
-                if (partial && !make_finite<C>(vr[i])) atomicOr(&wild[buf], 1ull << row);
+                if (partial && !make_finite<C>(vr[i])) atomicOr(&sh.wild[buf], 1ull << row);
                 vec<E, 8> terms[KT];
                 as_terms<C, E, KT>(kr[i], terms);
 #pragma unroll
-                for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&ks[n][row][(at ^ key_swap(row)) * 8]) = terms[n];
+                for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&sh.k[n][row][(at ^ key_swap(row)) * 8]) = terms[n];
                 as_terms<C, E, KT>(vr[i], terms);
 #pragma unroll
-                for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&vs[n][row][(at ^ value_swap(row)) * 8]) = terms[n];
+                for (int n = 0; n < KT; ++n) *reinterpret_cast<vec<E, 8> *>(&sh.v[n][row][(at ^ value_swap(row)) * 8]) = terms[n];
             }
-            put_offset(buf ^ 1, next_off);
             __syncthreads();
         }
-        // (distinct restrict pointers: without them the compiler waits for the next tile before it reads this one)
-        step(k0, partial, &ks[kDirect ? buf : 0][0][0], &vs[kDirect ? buf : 0][0][0], offs[buf], offs[buf ^ 1], &here[buf], &wild[buf],
-             &ks[kDirect ? buf ^ 1 : 0][0][0], &vs[kDirect ? buf ^ 1 : 0][0][0]);
+        step(n, k0, partial, exist, &sh.v[kDirect ? buf : 0][0][0], &sh.k[kDirect ? buf ^ 1 : 0][0][0], &sh.v[kDirect ? buf ^ 1 : 0][0][0]);
     }
     if (wr0 + col >= rows) return;
     l += lane_xor<32>(l, lane);
