@@ -747,34 +747,56 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
 
 // ---- the join of the parts ----------------------------------------------------------------------
 
-// One workgroup of 64 lanes per token and head: out = sum of parts 2^(least bias - bias) o / the same of l.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void attn_join(AttnArgs a) {
-    const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+// out = sum over parts of 2^(least bias - bias) o, over the same sum of l. A lane of each wave holds a part's bias and sum (64 at a
+// time) and its factor. W waves share a token's head: with many parts (few rows) their outputs are dealt to four waves, whose
+// loads do not wait for one another and which meet in LDS; with few parts (many rows) one wave takes them all. (One wave with
+// a loop over the parts took 0.4 us a part; four waves for two parts cost a 2048-token prompt 20 us.)
+template <typename T, int D, int W>
+__global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
+    constexpr int V = D / 64;
+    __shared__ float meet[W][64][V];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+    const int row = blockIdx.x * (4 / W) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
+    const int token = row / a.n_heads, head = row - token * a.n_heads;
+    if (token >= a.n_tokens) return;
     int b, pos;
     if (!find_token(a.q_start, a.kv_len, a.n_seqs, token, b, pos)) return;
     const int len = min(a.kv_len[b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
     const int lo = key_lo(a, pos), hi = key_hi(a, pos, len);
     const int z0 = min(lo / a.span, a.parts - 1), z1 = hi > lo ? min((hi - 1) / a.span + 1, a.parts) : z0;
     const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts;
-    float least = INFINITY;
-    for (int z = z0; z < z1; ++z) {
-        const float2 ml = a.part_ml[at + z];
-        if (ml.y != 0.0f) least = fminf(least, ml.x);
-    }
-    float acc[D / 64] = {}, l = 0.0f;
-    for (int z = z0; z < z1; ++z) {
-        const float2 ml = a.part_ml[at + z];
-        if (ml.y == 0.0f) continue;
-        const float f = exp2f(least - ml.x);
-        l += ml.y * f;
-        const float *o = a.part_o + (at + z) * D;
+    float acc[V] = {}, l = 0.0f, bias = INFINITY;  // of the parts so far: their least bias
+    for (int z = z0; z < z1; z += 64) {
+        const float2 ml = z + lane < z1 ? a.part_ml[at + z + lane] : make_float2(INFINITY, 0.0f);
+        const float mine = ml.y != 0.0f ? ml.x : INFINITY;
+        const float least = fminf(bias, -xor_max_wave(-mine));
+        const float f = ml.y != 0.0f ? exp2f(least - mine) : 0.0f;
+        const float old = bias == INFINITY ? 0.0f : exp2f(least - bias);
+        bias = least;
+        l = l * old + sum_wave(ml.y * f);
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) acc[i] += o[lane + 64 * i] * f;
-    }
-    T *o = static_cast<T *>(a.out) + token * a.out_stride + head * D;
+        for (int i = 0; i < V; ++i) acc[i] *= old;
+        const int n = min(64, z1 - z);
+        for (int j = wave; j < n; j += W) {
+            const float fj = __shfl(f, j);
+            float o[V];
+            load_as_float<float, V>(a.part_o + (at + z + j) * D + lane * V, o);
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[lane + 64 * i] = static_cast<T>(l == 0.0f ? 0.0f : acc[i] / l);
+            for (int i = 0; i < V; ++i) acc[i] += fj != 0.0f ? o[i] * fj : 0.0f;
+        }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) meet[wave][lane][i] = acc[i];
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = (meet[0][lane][i] + meet[1][lane][i]) + (meet[2][lane][i] + meet[3][lane][i]);
+    }
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = l == 0.0f ? 0.0f : acc[i] / l;
+    store_rounded<T, V>(static_cast<T *>(a.out) + token * a.out_stride + head * D + lane * V, o);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -793,13 +815,23 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
     n.tiles = static_cast<int>(rows / (n.few ? kFewRows : kTileRows)) + s.n_seqs;
     const int64_t most = static_cast<int64_t>(s.table_stride) * c.page_size;
     const int64_t kv = s.max_kv > 0 ? std::min<int64_t>(s.max_kv, most) : most;
-    const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads;
+    // keys that one tile reads
+    const int64_t seen = p.causal && p.window > 0 ? std::min<int64_t>(kv, p.window + (n.few ? kFewRows : kTileRows)) : kv;
+    const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads, cus = device_cu_count();
+    const auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
     if (n.few) {
-        const int64_t want = kv * blocks / (8 * device_cu_count());
-        n.span = static_cast<int>(std::clamp<int64_t>((want + kFewStep - 1) / kFewStep * kFewStep, kFewStep, 1024));
+        // A workgroup's start and end cost as much as 500 keys, so parts are as long as one workgroup per CU makes them, up to
+        // 1024 keys, which evens out ragged lengths. One token of 32 heads over 30000 keys: 33 us in parts of 1024, 61 of
+        // 128; of 14 heads over 3000: 14 of 128, 31 of 1024; 64 sequences of up to 16000: 423, 455 of 512, 428 of 4096.
+        n.span = static_cast<int>(std::clamp<int64_t>(up(seen * blocks / cus, kFewStep), kFewStep, 1024));
     } else {
-        const int64_t parts = std::min<int64_t>(std::max<int64_t>(1, 2 * device_cu_count() / blocks), std::max<int64_t>(1, kv / 256));
-        n.span = static_cast<int>(((kv + parts - 1) / parts + 63) / 64 * 64);
+        // Two workgroups are resident per CU. With fewer tiles than 1.5 rounds of them, parts give three rounds, which evens out
+        // ragged lengths too; of 512 keys at least, for a part's output is written and read again. Chunks of 257 over up
+        // to 8000 (28 tiles of 8 heads): 206 us in parts of 1536, 243 of 4096, 334 whole; 512 over 16000: 302, 281, 612;
+        // a prompt of 5000 of 14 heads (514 tiles of 2 heads): 130 whole, 159 of 4096.
+        const int64_t slots = 2 * cus;
+        const int64_t parts = 2 * blocks >= 3 * slots ? 1 : (3 * slots + blocks - 1) / blocks;
+        n.span = static_cast<int>(parts == 1 ? kv : std::min(kv, std::max<int64_t>(512, up((seen + parts - 1) / parts, 64))));
     }
     n.parts = static_cast<int>((kv + n.span - 1) / n.span);
     return n;
@@ -819,7 +851,12 @@ void launch_dim(const AttnArgs &a, const Plan &n, hipStream_t s) {
         attn_few<T, C, D><<<grid, 256, 0, s>>>(a);
     else
         attn_tiles<T, C, D><<<grid, 256, 0, s>>>(a);
-    if (n.parts > 1) attn_join<T, D><<<dim3(a.n_tokens, a.n_heads), 64, 0, s>>>(a);
+    if (n.parts == 1) return;
+    const int rows = a.n_tokens * a.n_heads;
+    if (n.parts > 8)
+        attn_join<T, D, 4><<<rows, 256, 0, s>>>(a);
+    else
+        attn_join<T, D, 1><<<(rows + 3) / 4, 256, 0, s>>>(a);
 }
 
 template <typename T, typename C>
