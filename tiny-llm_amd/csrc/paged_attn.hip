@@ -152,10 +152,11 @@ __device__ inline bool make_finite(vec<C, 8> &x) {
 
 // 16 bytes per lane from global memory to LDS, lane after lane from `to` (the same in all lanes), without passing through
 // registers; wait_loads waits for all that the wave has under way.
-template <typename T, typename E>
+// STREAM: rows that are read once, past the caches' other contents.
+template <bool STREAM, typename T, typename E>
 __device__ inline void global_to_lds(const T *from, E *to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, STREAM ? 2 : 0);
 }
 __device__ inline void wait_loads() {
     __builtin_amdgcn_sched_barrier(0);
@@ -233,10 +234,10 @@ __device__ inline float load_query(const AttnArgs &a, const T *qp, vec<E, 8> (*q
 
 // ---- few rows: tiles of 16 rows ------------------------------------------------------------------
 
-// A tile's keys are dealt to the four waves 32 at a time; each wave keeps a softmax of its own, and the four meet at the end.
-// K goes from the cache straight into operand registers; V passes through LDS of the wave's own, which turns rows into columns.
-// Both registers are filled again as soon as they have been used, so K's loads are under way during the softmax and the
-// value product and V's during the next scores, with no wave waiting for another.
+// A tile's keys are dealt to the four waves 32 at a time; each wave keeps a softmax of its own, and the four meet at the end, so no
+// wave waits for another. K goes from the cache straight into operand registers, V into LDS of the wave's own, whose
+// transposing reads turn its rows into columns. Reading the cache is the work (a query row takes 2 to 4 flops a byte), so the loads of
+// the next step are issued as soon as this step's have arrived, before anything is computed on them.
 constexpr int kFewRows = 16;
 constexpr int kFewKeys = 32;   // per wave and step
 constexpr int kFewStep = 4 * kFewKeys;
@@ -246,12 +247,19 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     using Tm = Terms<T, C>;
     using E = typename Tm::E;
     constexpr int QT = Tm::QT, KT = Tm::KT;
-    constexpr int VS = D + 16, ND = D / 16, NS = D / 32;
-    static_assert(4 * kFewKeys * VS * sizeof(E) >= 4 * kFewRows * D * sizeof(float), "the waves' outputs fit where V was");
-    __shared__ __attribute__((aligned(16))) E vs[4][kFewKeys][VS];
-    __shared__ float meet[2][4][kFewRows];
+    // V of a step: as it is in two buffers (chunks of 16 bytes permuted as in attn_tiles) when the cache holds the instruction's
+    // type; else one of its terms after the other in one buffer.
+    constexpr bool kDirect = KT == 1;
+    constexpr int VS = kDirect ? D : D + 16, ND = D / 16, NS = D / 32, CH = D / 8, NV = kFewKeys * CH / 64;
+    __shared__ struct {
+        union {
+            __attribute__((aligned(16))) E v[4][kDirect ? 2 : 1][kFewKeys][VS];
+            float o[4][kFewRows][D];
+        };
+        float meet[2][4][kFewRows];
+    } sh;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, col = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
     const int kv_heads = a.n_heads / a.group;
     const int kvh = blockIdx.x % kv_heads;
     TileRows t;
@@ -273,28 +281,45 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
 
     const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride + 8 * g;
     const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride + 8 * g;
-    vec<C, 8> kr[2][NS], vr[2][NS];
-    // the lane's keys of a step: k0 + col and k0 + 16 + col
+    vec<C, 8> kr[2][2][NS], vr[kDirect ? 1 : 2][NS];
+    // The lane's keys of a step are k0 + col and k0 + 16 + col. All loads of the loop are unconditional (a page past the table is its
+    // last entry, a row that does not exist is row 0 of page 0): the compiler counts the loads that may stay under way at
+    // a wait, and a load under a branch counts as none, so every wait would be for all of them.
     const auto pages_of = [&](int k0, int *page) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const int key = k0 + 16 * kt + col;
-            page[kt] = key < ke ? page_number(a.pages, t.b, key) : -1;
+            const int i = min(a.pages.page_size.quot(k0 + 16 * kt + col), a.pages.table_stride - 1);
+            page[kt] = a.pages.table[static_cast<int64_t>(t.b) * a.pages.table_stride + i];
         }
     };
     const auto offsets = [&](int k0, const int *page, int64_t *o) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) o[kt] = row_in_page(a.pages, page[kt], k0 + 16 * kt + col);
+        for (int kt = 0; kt < 2; ++kt) {
+            const int key = k0 + 16 * kt + col;
+            o[kt] = key < ke ? row_in_page(a.pages, page[kt], key) : -1;
+        }
     };
     const auto load_rows = [&](const C *base, const int64_t *o, vec<C, 8> (*x)[NS]) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
+            const C *row = base + max(o[kt], int64_t{0});
 #pragma unroll
-            for (int i = 0; i < NS; ++i) x[kt][i] = vec<C, 8>{};
-            if (o[kt] >= 0) {
+            for (int i = 0; i < NS; ++i) x[kt][i] = *reinterpret_cast<const vec<C, 8> *>(row + 32 * i);
+        }
+    };
+
+    const auto load_values = [&](const int64_t *o, E *__restrict__ to) __attribute__((always_inline)) {
+        if constexpr (kDirect) {
 #pragma unroll
-                for (int i = 0; i < NS; ++i) x[kt][i] = *reinterpret_cast<const vec<C, 8> *>(base + o[kt] + 32 * i);
+            for (int i = 0; i < NV; ++i) {  // 64 chunks in order; the row's offset is held by lane `row % 16`
+                const int first = 64 * i / CH, row = first + lane / CH;
+                const int64_t ro = __shfl(static_cast<long long>(max(o[first / 16], int64_t{0})), row & 15);
+                // (streamed: a decode step of 64 requests takes 397 us so, 420 without. K's lines are read in two halves, which
+                // streaming fetches twice: 451 us.)
+                global_to_lds<true>(vc - 8 * g + ro + ((lane % CH) ^ ((row & 3) << 1)) * 8, to + 64 * i * 8);
             }
+        } else {
+            load_rows(vc, o, vr);
         }
     };
 
@@ -304,8 +329,8 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     pages_of(k0, next);
     offsets(k0, next, off);
     pages_of(k0 + kFewStep, next);
-    load_rows(kc, off, kr);
-    load_rows(vc, off, vr);
+    load_rows(kc, off, kr[0]);
+    load_values(off, &sh.v[wave][0][0][0]);
     vec<E, 8> q[QT][NS];
     const float c = load_query<T, E, QT, NS, 32>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 8 * g, q,
                                                  [&](float x) {
@@ -317,7 +342,18 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     for (int i = 0; i < ND; ++i) acc[i] = f32x4{};
     float m = -INFINITY, bias = 0.0f, l = 0.0f;
 
-    for (; k0 < ke; k0 += kFewStep) {
+    // (The restrict pointers tell the compiler that the next step's transfers do not touch the values that are read meanwhile.)
+    const auto step = [&](const vec<C, 8> (*k_now)[NS], vec<C, 8> (*k_next)[NS], const E *__restrict__ v_now, E *__restrict__ v_next)
+                          __attribute__((always_inline)) {
+        const unsigned exist = static_cast<unsigned>(__ballot(off[0] >= 0) & 0xffff) |
+                               static_cast<unsigned>(__ballot(off[1] >= 0) & 0xffff) << 16;
+        const bool partial = k0 < full_lo || k0 + kFewKeys > full_hi || exist != ~0u;
+        const int64_t was[2] = {off[0], off[1]};
+        wait_loads();
+        offsets(k0 + kFewStep, next, off);
+        pages_of(k0 + 2 * kFewStep, next);
+        load_rows(kc, off, k_next);
+        if constexpr (kDirect) load_values(off, v_next);
         // S^T: the lane holds its row's scores of keys 16 kt + 4 g + i
         f32x4 s[2];
 #pragma unroll
@@ -326,7 +362,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 vec<E, 8> kf[KT];
-                as_terms<C, E, KT>(kr[kt][i], kf);
+                as_terms<C, E, KT>(k_now[kt][i], kf);
 #pragma unroll
                 for (int kj = 0; kj < KT; ++kj)
 #pragma unroll
@@ -334,14 +370,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
                         if (qi + kj < Tm::kMost) s[kt] = mfma16(kf[kj], q[qi][i], s[kt]);
             }
         }
-        const unsigned exist = static_cast<unsigned>(__ballot(off[0] >= 0) & 0xffff) |
-                               static_cast<unsigned>(__ballot(off[1] >= 0) & 0xffff) << 16;
-        const bool partial = k0 < full_lo || k0 + kFewKeys > full_hi;
-        const int64_t was[2] = {off[0], off[1]};
-        offsets(k0 + kFewStep, next, off);
-        pages_of(k0 + 2 * kFewStep, next);
-        load_rows(kc, off, kr);
-        if (partial || exist != ~0u) {
+        if (partial) {
             const int k1 = k0 + 4 * g;
             const unsigned may = (exist >> (4 * g)) & below(hi - k1) & ~below(lo - k1);
 #pragma unroll
@@ -376,42 +405,60 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
         split<E, QT>(w, p);
         unsigned wild = 0;
         if (partial) {  // infinite and NaN values as in attn_tiles
+            if constexpr (kDirect) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                bool finite = true;
+                for (int i = 0; i < NV; ++i) {
+                    vec<C, 8> *at = reinterpret_cast<vec<C, 8> *>(const_cast<E *>(v_now)) + 64 * i + lane;
+                    vec<C, 8> x = *at;
+                    const bool finite = make_finite<C>(x);
+                    if (!finite) *at = x;
+                    unsigned long long bad = __ballot(!finite);  // by chunk: CH of them a row
+                    for (int row = 64 * i / CH; bad; ++row, bad >>= CH)
+                        if (bad & ((1ull << CH) - 1)) wild |= 1u << row;
+                }
+                wave_lds_order();
+            } else {
 #pragma unroll
-                for (int i = 0; i < NS; ++i) finite = make_finite<C>(vr[kt][i]) && finite;
-                const unsigned long long bad = __ballot(!finite);
-                wild |= static_cast<unsigned>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff) << (16 * kt);
+                for (int kt = 0; kt < 2; ++kt) {
+                    bool finite = true;
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) finite = make_finite<C>(vr[kt][i]) && finite;
+                    const unsigned long long bad = __ballot(!finite);
+                    wild |= static_cast<unsigned>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff) << (16 * kt);
+                }
             }
         }
 #pragma unroll
         for (int kj = 0; kj < KT; ++kj) {
+            if constexpr (!kDirect) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+                for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    vec<E, 8> vf[KT];
-                    as_terms<C, E, KT>(vr[kt][i], vf);
-                    *reinterpret_cast<vec<E, 8> *>(&vs[wave][16 * kt + col][32 * i + 8 * g]) = vf[kj];
-                }
-            wave_lds_order();
-            if (kj == KT - 1) load_rows(vc, off, vr);
+                    for (int i = 0; i < NS; ++i) {
+                        vec<E, 8> vf[KT];
+                        as_terms<C, E, KT>(vr[kt][i], vf);
+                        *reinterpret_cast<vec<E, 8> *>(&sh.v[wave][0][16 * kt + col][32 * i + 8 * g]) = vf[kj];
+                    }
+                wave_lds_order();
+                if (kj == KT - 1) load_values(off, v_next);
+            }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const E *v0 = &vs[wave][4 * g + (lane & 15) / 4][16 * d + 4 * (lane & 3)];
+                const int i = lane & 15, row = 4 * g + i / 4;
+                const int ch = (2 * d + (i & 3) / 2) ^ (kDirect ? (row & 3) << 1 : 0);
+                const E *v0 = (kDirect ? v_now : &sh.v[wave][0][0][0]) + row * VS + ch * 8 + 4 * (i & 1);
                 const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 16 * VS);
                 const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int qi = 0; qi < QT; ++qi)
                     if (qi + kj < Tm::kMost) acc[d] = mfma16(vf, p[qi], acc[d]);
             }
-            wave_lds_order();
+            if constexpr (!kDirect) wave_lds_order();
         }
         for (; wild; wild &= wild - 1) {
             const int j = __builtin_ctz(wild), key = k0 + j;
             const int64_t o = __shfl(static_cast<long long>(j < 16 ? was[0] : was[1]), j & 15);
-            if (key < lo || key >= hi) continue;
+            if (key < lo || key >= hi || o < 0) continue;
             const C *v0 = vc + o - 8 * g + 4 * g;
 #pragma unroll
             for (int d = 0; d < ND; ++d)
@@ -419,30 +466,37 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
                 for (int e = 0; e < 4; ++e)
                     if (!is_finite<C>(v0[16 * d + e])) acc[d][e] += static_cast<float>(v0[16 * d + e]);
         }
+        k0 += kFewStep;
+    };
+    E *v0 = &sh.v[wave][0][0][0], *v1 = &sh.v[wave][kDirect ? 1 : 0][0][0];
+    while (k0 < ke) {
+        step(kr[0], kr[1], v0, v1);
+        if (k0 >= ke) break;
+        step(kr[1], kr[0], v1, v0);
     }
+    wait_loads();  // (the loads past the last step: into LDS that is used for other things below)
     l += lane_xor<16>(l, lane);
     l += lane_xor<32>(l, lane);
     // the four waves' sums, brought to the least exponent bias among those that have any
     if (g == 0) {
-        meet[0][wave][col] = bias;
-        meet[1][wave][col] = l;
+        sh.meet[0][wave][col] = bias;
+        sh.meet[1][wave][col] = l;
     }
     __syncthreads();  // (and every wave is done with V)
     float least = INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-        if (meet[1][w][col] != 0.0f) least = fminf(least, meet[0][w][col]);
+        if (sh.meet[1][w][col] != 0.0f) least = fminf(least, sh.meet[0][w][col]);
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-        if (meet[1][w][col] != 0.0f) total += meet[1][w][col] * exp2f(least - meet[0][w][col]);
+        if (sh.meet[1][w][col] != 0.0f) total += sh.meet[1][w][col] * exp2f(least - sh.meet[0][w][col]);
     const float f = l != 0.0f ? exp2f(least - bias) : 0.0f;
-    float(*os)[kFewRows][D] = reinterpret_cast<float(*)[kFewRows][D]>(&vs[0][0][0]);
     if (l != 0.0f) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] *= f;
     }
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&os[wave][col][16 * d + 4 * g]) = acc[d];
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&sh.o[wave][col][16 * d + 4 * g]) = acc[d];
     __syncthreads();
     // thread: row tid / 16, every 16th group of four dimensions
     const int row = tid >> 4;
@@ -455,9 +509,9 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         const int d = 4 * (tid & 15) + 64 * i;
-        f32x4 o = *reinterpret_cast<f32x4 *>(&os[0][row][d]);
+        f32x4 o = *reinterpret_cast<f32x4 *>(&sh.o[0][row][d]);
 #pragma unroll
-        for (int w = 1; w < 4; ++w) o += *reinterpret_cast<f32x4 *>(&os[w][row][d]);
+        for (int w = 1; w < 4; ++w) o += *reinterpret_cast<f32x4 *>(&sh.o[w][row][d]);
         if (a.parts > 1) {
             *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) = o;
         } else {
@@ -548,8 +602,8 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
             const int ch = tid + 256 * i, row = ch / CH, at = ch % CH;
             if constexpr (kDirect) {
                 const int first = (wave * 64 + 256 * i) * 8;  // element of the wave's first chunk
-                global_to_lds(kc + o[i] + (at ^ key_swap(row)) * 8, k_to + first);
-                global_to_lds(vc + o[i] + (at ^ value_swap(row)) * 8, v_to + first);
+                global_to_lds<false>(kc + o[i] + (at ^ key_swap(row)) * 8, k_to + first);
+                global_to_lds<false>(vc + o[i] + (at ^ value_swap(row)) * 8, v_to + first);
             } else {
                 kr[i] = *reinterpret_cast<const vec<C, 8> *>(kc + o[i] + at * 8);
                 vr[i] = *reinterpret_cast<const vec<C, 8> *>(vc + o[i] + at * 8);
