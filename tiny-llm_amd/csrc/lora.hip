@@ -23,7 +23,7 @@ struct LoraArgs {
     const int *q_start, *adapter;
     float *u;  // [splits][n_tokens][rank]: parts of scale A x, over the parts of K
     int n_tokens, K, M, rank, n_adapters, n_seqs;
-    int splits, m_per_block;
+    int splits;
 };
 
 using f32x4 = vec<float, 4>;
@@ -53,12 +53,15 @@ __device__ inline void bf16_terms(const float *x, bf16x8 *out) {
     }
 }
 
-// Elements at .. at + 7 of a row of n, zeros past its end. WIDE: n is a multiple of 8 and rows are 16-byte aligned.
+// Elements at .. at + 7 of a row of n, zeros past its end. WIDE: n is a multiple of 8 and rows are 16-byte aligned; the load is
+// then unconditional, so that the compiler can count it among those that may stay under way at a wait.
 template <bool WIDE, typename T>
 __device__ inline vec<T, 8> load8(const T *row, int at, int n) {
     vec<T, 8> v{};
     if constexpr (WIDE) {
-        if (at < n) v = *reinterpret_cast<const vec<T, 8> *>(row + at);
+        v = *reinterpret_cast<const vec<T, 8> *>(row + min(at, n - 8));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = at < n ? v[i] : static_cast<T>(0.0f);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -83,101 +86,144 @@ __device__ inline int adapter_of(const LoraArgs &p, int b) {
     return static_cast<unsigned>(a) < static_cast<unsigned>(p.n_adapters) ? a : -1;
 }
 
-// u^T = A x^T for a tile of 16 TT tokens: the lane holds ranks 16 n + 4 g + i of token 16 t + lane % 16. The steps of 32 along K are
-// dealt to gridDim.y blocks of four waves; the waves' sums meet in LDS, the blocks' in lora_expand. x is read once.
-template <typename W, int NR, int TT, bool WIDE>
-__global__ __launch_bounds__(256) void lora_shrink(LoraArgs p) {
-    constexpr int BM = 16 * TT;
-    __shared__ float sum[4][BM][16 * NR + 4];
+// u^T = A x^T for a tile of 16 tokens: the lane holds ranks 16 n + 4 g + i of token lane % 16. The steps of 32 along K are dealt to
+// the workgroup's waves, whose sums meet in LDS, and to gridDim.y workgroups where there are fewer tiles than CUs, whose sums
+// meet in lora_expand. x is read once. The launch lasts as long as one wave's loads one after the other, so the waves are many and
+// their steps few: 16 waves of 5 steps at K = 2560. (4 waves, 32 tokens and 4 workgroups a tile took 21 us for 3700 tokens, and
+// the four sums of u cost every workgroup of lora_expand as many bytes as its outputs.)
+template <int NR>
+constexpr int kShrinkWaves = NR <= 4 ? 16 : 8;
+
+template <typename W, int NR, bool WIDE>
+__global__ __launch_bounds__(64 * kShrinkWaves<NR>) void lora_shrink(LoraArgs p) {
+    constexpr int BM = 16, NW = kShrinkWaves<NR>;
+    __shared__ float sum[NW][BM][16 * NR + 4];
     Run t;
     if (!find_run<BM>(p.q_start, p.n_seqs, p.n_tokens, 1, blockIdx.x, t)) return;
-    const int ad = adapter_of(p, t.b);
-    if (ad < 0) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
-    const int steps = (p.K + 31) / 32, workers = 4 * p.splits, worker = blockIdx.y * 4 + wave;
+    const int steps = (p.K + 31) / 32, workers = NW * p.splits, worker = blockIdx.y * NW + wave;
     const int s0 = static_cast<int>(static_cast<int64_t>(steps) * worker / workers);
     const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (worker + 1) / workers);
-    const float *x[TT];
+    const float *x = p.x + static_cast<int64_t>(t.first + min(t.r0 + col, t.n - 1)) * p.K;
+    vec<float, 8> xv = load8<WIDE>(x, 32 * s0 + 8 * g, p.K);  // (under way while the adapter is looked up)
+    const int ad = adapter_of(p, t.b);
+    if (ad < 0) return;
+    const W *a = static_cast<const W *>(p.a) + static_cast<int64_t>(ad) * p.rank * p.K;
+    vec<W, 8> av[NR];
+    const auto load_weights = [&](int s) {
 #pragma unroll
-    for (int j = 0; j < TT; ++j) x[j] = p.x + static_cast<int64_t>(t.first + min(t.r0 + 16 * j + col, t.n - 1)) * p.K;
-    const W *a[NR];
+        for (int n = 0; n < NR; ++n)
+            av[n] = load8<WIDE>(a + static_cast<int64_t>(min(16 * n + col, p.rank - 1)) * p.K, 32 * s + 8 * g, p.K);
+    };
+    load_weights(s0);
+    f32x4 acc[NR];
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
-        a[n] = static_cast<const W *>(p.a) + (static_cast<int64_t>(ad) * p.rank + min(16 * n + col, p.rank - 1)) * p.K;
-    f32x4 acc[NR][TT];
-#pragma unroll
-    for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int j = 0; j < TT; ++j) acc[n][j] = f32x4{};
+    for (int n = 0; n < NR; ++n) acc[n] = f32x4{};
     for (int s = s0; s < s1; ++s) {
-        const int k = 32 * s + 8 * g;
-        bf16x8 xt[TT][kUTerms];
+        bf16x8 xt[kUTerms];
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            const vec<float, 8> v = load8<WIDE>(x[j], k, p.K);
-            float f[8];
+        for (int e = 0; e < 8; ++e) f[e] = xv[e];
+        bf16_terms<kUTerms>(f, xt);
+        const int ahead = min(s + 1, s1 - 1);  // the next step's operands are under way during this step's products
+        xv = load8<WIDE>(x, 32 * ahead + 8 * g, p.K);
+        vec<W, 8> now[NR];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = v[e];
-            bf16_terms<kUTerms>(f, xt[j]);
-        }
+        for (int n = 0; n < NR; ++n) now[n] = av[n];
+        load_weights(ahead);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             bf16x8 wt[kWTerms<W>];
-            weight_terms<W>(load8<WIDE>(a[n], k, p.K), wt);
+            weight_terms<W>(now[n], wt);
 #pragma unroll
             for (int w = 0; w < kWTerms<W>; ++w)
 #pragma unroll
                 for (int u = 0; u < kUTerms; ++u)
-                    if (w + u < 3) {
-#pragma unroll
-                        for (int j = 0; j < TT; ++j) acc[n][j] = mfma16(wt[w], xt[j][u], acc[n][j]);
-                    }
+                    if (w + u < 3) acc[n] = mfma16(wt[w], xt[u], acc[n]);
         }
     }
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int j = 0; j < TT; ++j) *reinterpret_cast<f32x4 *>(&sum[wave][16 * j + col][16 * n + 4 * g]) = acc[n][j];
+    for (int n = 0; n < NR; ++n) *reinterpret_cast<f32x4 *>(&sum[wave][col][16 * n + 4 * g]) = acc[n];
     __syncthreads();
     const float scale = p.scale[ad];
     const int live = min(BM, t.n - t.r0);
     float *u = p.u + (static_cast<int64_t>(blockIdx.y) * p.n_tokens + t.first + t.r0) * p.rank;
-    for (int i = threadIdx.x; i < live * p.rank; i += 256) {
+    for (int i = threadIdx.x; i < live * p.rank; i += 64 * NW) {
         const int row = i / p.rank, c = i - row * p.rank;
-        u[i] = scale * ((sum[0][row][c] + sum[1][row][c]) + (sum[2][row][c] + sum[3][row][c]));
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += sum[w][row][c];
+        u[i] = scale * v;
     }
 }
 
-// y = base + u B^T for a tile of 16 TT tokens and m_per_block outputs, 32 of them per wave and step. Rows of the matrix instruction
-// are dealt so that a lane holds outputs 8 g .. 8 g + 7 of the 32 for its token, and four lanes a whole 128-byte line.
-template <typename W, int KS, int TT, bool WIDE, bool WIDE_Y>
+// y = base + u B^T for a tile of 16 TT tokens and 128 S outputs, 32 of them per wave and step: the lane holds outputs
+// 4 g + 16 h .. + 3 of a step for token 16 j + lane % 16. All of the wave's base is requested first and under way while u is put
+// together, and nothing is stored before it is all there: with the next step's base requested between the stores, in fewer and longer
+// workgroups, 8 prompts of up to 600 tokens beside 9728x2560 took 125 us instead of 99 (a load waits for the stores before it,
+// and reads and writes take turns at the memory).
+template <typename W, int KS, int TT, int S, bool WIDE, bool WIDE_Y>
 __global__ __launch_bounds__(256) void lora_expand(LoraArgs p) {
     constexpr int BM = 16 * TT, US = 32 * KS + 8;
     __shared__ __attribute__((aligned(16))) bf16 ut[kUTerms][BM][US];
     Run t;
     if (!find_run<BM>(p.q_start, p.n_seqs, p.n_tokens, 1, blockIdx.x, t)) return;
-    const int ad = adapter_of(p, t.b);
-    if (ad < 0 && p.base == p.y) return;
     const int live = min(BM, t.n - t.r0);
-    const int m_first = blockIdx.y * p.m_per_block, m_end = min(m_first + p.m_per_block, p.M);
+    const int m_first = blockIdx.y * 128 * S, m_end = min(m_first + 128 * S, p.M);
     const int64_t token0 = t.first + t.r0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
+    f32x4 acc[S][2][TT];
+#pragma unroll
+    for (int j = 0; j < TT; ++j) {
+        const float *src = p.base + (token0 + min(16 * j + col, live - 1)) * p.M;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int m = m_first + 128 * i + 32 * wave + 16 * h + 4 * g;
+                acc[i][h][j] = f32x4{};
+                if (!p.base) continue;
+                if constexpr (WIDE_Y) {
+                    acc[i][h][j] = *reinterpret_cast<const f32x4 *>(src + min(m, p.M - 4));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][h][j][e] = src[min(m + e, p.M - 1)];
+                }
+            }
+    }
+    const int ad = adapter_of(p, t.b);
     if (ad < 0) {
-        for (int row = threadIdx.x >> 6; row < live; row += 4)
-            for (int m = m_first + (threadIdx.x & 63); m < m_end; m += 64) {
+        if (p.base == p.y) return;
+        for (int row = wave; row < live; row += 4)
+            for (int m = m_first + lane; m < m_end; m += 64) {
                 const int64_t at = (token0 + row) * p.M + m;
                 p.y[at] = p.base ? p.base[at] : 0.0f;
             }
         return;
     }
+    const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(ad) * p.M * p.rank;
+    vec<W, 8> bv[S][2][KS];
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                bv[i][h][s] = load8<WIDE>(b + static_cast<int64_t>(min(m_first + 128 * i + 32 * wave + 16 * h + col, p.M - 1)) * p.rank,
+                                          32 * s + 8 * g, p.rank);
     for (int i = threadIdx.x; i < BM * KS * 4; i += 256) {
         const int row = i / (KS * 4), c = i % (KS * 4) * 8;
         float f[8] = {};
         if (row < live) {
-            for (int z = 0; z < p.splits; ++z) {
-                const float *u = p.u + (static_cast<int64_t>(z) * p.n_tokens + token0 + row) * p.rank;
-                const vec<float, 8> v = load8<WIDE>(u, c, p.rank);
+            for (int z = 0; z < p.splits; z += 4) {  // four parts' loads at a time
+                vec<float, 8> v[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] += v[e];
+                for (int y = 0; y < 4; ++y)
+                    v[y] = load8<WIDE>(p.u + (static_cast<int64_t>(min(z + y, p.splits - 1)) * p.n_tokens + token0 + row) * p.rank, c, p.rank);
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] += z + y < p.splits ? v[y][e] : 0.0f;
             }
         }
         bf16x8 terms[kUTerms];
@@ -186,7 +232,6 @@ __global__ __launch_bounds__(256) void lora_expand(LoraArgs p) {
         for (int n = 0; n < kUTerms; ++n) *reinterpret_cast<bf16x8 *>(&ut[n][row][c]) = terms[n];
     }
     __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
     bf16x8 u[TT][KS][kUTerms];
 #pragma unroll
     for (int j = 0; j < TT; ++j)
@@ -194,81 +239,63 @@ __global__ __launch_bounds__(256) void lora_expand(LoraArgs p) {
         for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int n = 0; n < kUTerms; ++n) u[j][s][n] = *reinterpret_cast<bf16x8 *>(&ut[n][16 * j + col][32 * s + 8 * g]);
-    const W *b = static_cast<const W *>(p.b) + static_cast<int64_t>(ad) * p.M * p.rank;
-    for (int m0 = m_first + 32 * wave; m0 < m_end; m0 += 128) {
-        f32x4 acc[2][TT];
-        const int m = m0 + 8 * g;  // the lane's outputs m .. m + 7
 #pragma unroll
-        for (int j = 0; j < TT; ++j) {
-            const float *src = p.base ? p.base + (token0 + min(16 * j + col, live - 1)) * p.M : nullptr;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                acc[h][j] = f32x4{};
-                if (!src) continue;
-                if (WIDE_Y && m + 4 * h < p.M) acc[h][j] = *reinterpret_cast<const f32x4 *>(src + m + 4 * h);
-                if constexpr (!WIDE_Y) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (m + 4 * h + e < p.M) acc[h][j][e] = src[m + 4 * h + e];
-                }
-            }
-        }
+    for (int i = 0; i < S; ++i) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            // row col of the instruction is output 8 (col / 4) + 4 h + col % 4 of the 32
-            const int row = m0 + 8 * (col >> 2) + 4 * h + (col & 3);
-            const W *br = b + static_cast<int64_t>(min(row, p.M - 1)) * p.rank;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 bf16x8 wt[kWTerms<W>];
-                weight_terms<W>(load8<WIDE>(br, 32 * s + 8 * g, p.rank), wt);
+                weight_terms<W>(bv[i][h][s], wt);
 #pragma unroll
                 for (int w = 0; w < kWTerms<W>; ++w)
 #pragma unroll
                     for (int n = 0; n < kUTerms; ++n)
                         if (w + n < 3) {
 #pragma unroll
-                            for (int j = 0; j < TT; ++j) acc[h][j] = mfma16(wt[w], u[j][s][n], acc[h][j]);
+                            for (int j = 0; j < TT; ++j) acc[i][h][j] = mfma16(wt[w], u[j][s][n], acc[i][h][j]);
                         }
             }
         }
+    }
+#pragma unroll
+    for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
             if (16 * j + col >= live) continue;
             float *dst = p.y + (token0 + 16 * j + col) * p.M;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (WIDE_Y && m + 4 * h < p.M) *reinterpret_cast<f32x4 *>(dst + m + 4 * h) = acc[h][j];
+                const int m = m_first + 128 * i + 32 * wave + 16 * h + 4 * g;
+                if (WIDE_Y && m < p.M) *reinterpret_cast<f32x4 *>(dst + m) = acc[i][h][j];
                 if constexpr (!WIDE_Y) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (m + 4 * h + e < p.M) dst[m + 4 * h + e] = acc[h][j][e];
+                        if (m + e < p.M) dst[m + e] = acc[i][h][j][e];
                 }
             }
         }
-    }
 }
 
 // ---- host ----------------------------------------------------------------------------------------
 
 struct LoraPlan {
-    int few;             // sequences of a token or a few: tiles of 16 tokens
-    int shrink_tiles, splits;
-    int expand_tiles, m_per_block;
+    bool few;  // sequences of a token or a few: tiles of 16 tokens
+    int shrink_tiles, splits, expand_tiles;
 };
 
-int expand_tokens(int rank, bool few) { return few || rank > 128 ? 16 : rank > 64 ? 32 : 64; }
+constexpr int kLoraSteps = 2;  // of a wave in lora_expand, 1 with few tokens
+
+int expand_tokens(int rank, bool few) { return few || rank > 128 ? 16 : 32; }
 
 LoraPlan lora_plan(const tqhip_lora &l) {
     LoraPlan n{};
     n.few = l.n_tokens <= 16 * static_cast<int64_t>(l.n_seqs);
-    n.shrink_tiles = l.n_tokens / (n.few ? 16 : 32) + l.n_seqs;
-    // about two workgroups per CU, of at least two steps of 32 per wave
-    const int most = std::max(1, (l.in_dim + 31) / 32 / 8);
-    n.splits = std::clamp(2 * device_cu_count() / n.shrink_tiles, 1, most);
+    n.shrink_tiles = l.n_tokens / 16 + l.n_seqs;
+    // fewer tiles than CUs: several workgroups a tile, of at least a step of 32 per wave
+    const int most = std::max(1, (l.in_dim + 31) / 32 / (l.rank <= 64 ? kShrinkWaves<4> : kShrinkWaves<8>));
+    n.splits = std::clamp(device_cu_count() / n.shrink_tiles, 1, std::min(most, 8));
     n.expand_tiles = l.n_tokens / expand_tokens(l.rank, n.few) + l.n_seqs;
-    const int64_t want = static_cast<int64_t>(l.out_dim) * n.expand_tiles / (4 * device_cu_count());
-    n.m_per_block = static_cast<int>(std::clamp<int64_t>((want + 127) / 128 * 128, 128, 2048));
     return n;
 }
 
@@ -288,25 +315,22 @@ int check_lora(const tqhip_lora &l) {
 
 template <typename W, int NR, bool WIDE>
 void launch_shrink(const LoraArgs &p, const LoraPlan &n, hipStream_t s) {
-    const dim3 grid(n.shrink_tiles, n.splits);
-    if (n.few)
-        lora_shrink<W, NR, 1, WIDE><<<grid, 256, 0, s>>>(p);
-    else
-        lora_shrink<W, NR, 2, WIDE><<<grid, 256, 0, s>>>(p);
+    lora_shrink<W, NR, WIDE><<<dim3(n.shrink_tiles, n.splits), 64 * kShrinkWaves<NR>, 0, s>>>(p);
 }
 
 template <typename W, int KS, bool WIDE>
 void launch_expand(const LoraArgs &p, const LoraPlan &n, bool wide_y, hipStream_t s) {
-    constexpr int TT = KS <= 2 ? 4 : KS == 4 ? 2 : 1;
-    const dim3 grid(n.expand_tiles, (p.M + p.m_per_block - 1) / p.m_per_block);
+    constexpr int TT = KS <= 4 ? 2 : 1, S = kLoraSteps;
+    const int steps = n.few ? 1 : S;
+    const dim3 grid(n.expand_tiles, (p.M + 128 * steps - 1) / (128 * steps));
     if (n.few && wide_y)
-        lora_expand<W, KS, 1, WIDE, true><<<grid, 256, 0, s>>>(p);
+        lora_expand<W, KS, 1, 1, WIDE, true><<<grid, 256, 0, s>>>(p);
     else if (n.few)
-        lora_expand<W, KS, 1, WIDE, false><<<grid, 256, 0, s>>>(p);
+        lora_expand<W, KS, 1, 1, WIDE, false><<<grid, 256, 0, s>>>(p);
     else if (wide_y)
-        lora_expand<W, KS, TT, WIDE, true><<<grid, 256, 0, s>>>(p);
+        lora_expand<W, KS, TT, S, WIDE, true><<<grid, 256, 0, s>>>(p);
     else
-        lora_expand<W, KS, TT, WIDE, false><<<grid, 256, 0, s>>>(p);
+        lora_expand<W, KS, TT, S, WIDE, false><<<grid, 256, 0, s>>>(p);
 }
 
 template <typename W>
@@ -355,7 +379,7 @@ int run_lora(const tqhip_lora &l, hipStream_t s) {
     if (!ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
     const LoraPlan n = lora_plan(l);
     const LoraArgs p{l.x, l.base, l.y, l.a, l.b, l.scale, l.q_start, l.adapter, static_cast<float *>(ws), l.n_tokens,
-                     l.in_dim, l.out_dim, l.rank, l.n_adapters, l.n_seqs, n.splits, n.m_per_block};
+                     l.in_dim, l.out_dim, l.rank, l.n_adapters, l.n_seqs, n.splits};
     switch (l.dtype) {
         case TQHIP_F32: launch_lora<float>(p, n, s); break;
         case TQHIP_F16: launch_lora<f16>(p, n, s); break;
