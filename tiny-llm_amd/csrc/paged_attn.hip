@@ -164,9 +164,11 @@ __device__ inline void wait_loads() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// A row's sums are brought down to a new maximum only once it exceeds the one they stand at by 2^kHeadroom: the weights stay
+// A row's sums are brought down to a new maximum only once it exceeds the one they stand at by that power of two: the weights stay
 // within fp16's range, and what their sums lose by it is nothing, since a factor of a power of two is common to all of them.
-constexpr float kHeadroom = 7.0f;
+// (With fp32 results 2^1: an exponent of up to 7 has three bits less behind its point than one near 0.)
+template <int QT>
+constexpr float kHeadroom = QT == 1 ? 7.0f : 1.0f;
 
 // Weights are 2^(s c + bias): with fp16 terms they are held 2^8 times larger, above fp16's subnormals.
 template <typename E>
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kt][i]);
         mx = fmaxf(mx, lane_xor<16>(mx, lane));
         mx = fmaxf(mx, lane_xor<32>(mx, lane));
-        if (__ballot((mx - m) * c > kHeadroom)) {
+        if (__ballot((mx - m) * c > kHeadroom<QT>)) {
             const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
             const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
             m = mx;
@@ -672,7 +674,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
             mx = fmaxf(mx, lane_xor<32>(mx, lane));
-            if (__ballot((mx - m) * c > kHeadroom)) {
+            if (__ballot((mx - m) * c > kHeadroom<QT>)) {
                 const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
                 const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
                 m = mx;
@@ -865,7 +867,11 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
     const int group = p.n_heads / c.n_kv_heads;
     const int64_t rows = static_cast<int64_t>(s.n_tokens) * group;
     Plan n{};
-    n.few = rows <= int64_t{2} * kFewRows * s.n_seqs;
+    // Tiles of 16 rows read the cache once for each; they win up to 32 rows a sequence (64 sequences of up to 4000 keys, 32 heads of
+    // 128: 16 rows 140 us, against 182 with tiles of 128; 32 rows 195 and 189; 64 rows 294 and 223), and, whatever the rows, as long
+    // as there are few of them in all, because there they come in shorter parts (one sequence of 64 rows on 8 K/V heads 22 us and 32,
+    // 128 rows 34 and 34; 448 rows on 2 heads of 64 30 and 41, 1792 rows 79 and 47; 1024 on one of 256 52 and 81).
+    n.few = rows <= int64_t{2} * kFewRows * s.n_seqs || (rows + kFewRows - 1) / kFewRows * c.n_kv_heads <= 56;
     n.tiles = static_cast<int>(rows / (n.few ? kFewRows : kTileRows)) + s.n_seqs;
     const int64_t most = static_cast<int64_t>(s.table_stride) * c.page_size;
     const int64_t kv = s.max_kv > 0 ? std::min<int64_t>(s.max_kv, most) : most;
@@ -874,10 +880,11 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
     const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads, cus = device_cu_count();
     const auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
     if (n.few) {
-        // A workgroup's start and end cost as much as 500 keys, so parts are as long as one workgroup per CU makes them, up to
-        // 1024 keys, which evens out ragged lengths. One token of 32 heads over 30000 keys: 33 us in parts of 1024, 61 of
-        // 128; of 14 heads over 3000: 14 of 128, 31 of 1024; 64 sequences of up to 16000: 423, 455 of 512, 428 of 4096.
-        n.span = static_cast<int>(std::clamp<int64_t>(up(seen * blocks / cus, kFewStep), kFewStep, 1024));
+        // A workgroup's start and end cost as much as some 500 keys, so parts are as long as two workgroups per CU make them, up to
+        // 1024 keys, which evens out ragged lengths. One token of 32 heads over 30000 keys: 35 us in parts of 512, 61 of
+        // 128; of 14 heads over 3000: 14 of 128, 31 of 1024; 64 sequences of up to 16000: 423 of 1024, 455 of 512, 428 of 4096.
+        const int64_t full = std::max<int64_t>(s.n_seqs, (rows + kFewRows - 1) / kFewRows) * c.n_kv_heads;  // tiles that there are
+        n.span = static_cast<int>(std::clamp<int64_t>(up(seen * full / (2 * cus), kFewStep), kFewStep, 1024));
     } else {
         // Two workgroups are resident per CU. With fewer tiles than 1.5 rounds of them, parts give three rounds, which evens out
         // ragged lengths too; of 512 keys at least, for a part's output is written and read again. Chunks of 257 over up
