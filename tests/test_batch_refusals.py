@@ -79,6 +79,30 @@ def test_lora_refuses(calls, kw):
 def test_too_large(calls):
     assert calls["attention"](s=dict(table_stride=INT_MAX)) == -3
     assert calls["append"](s=dict(table_stride=INT_MAX)) == -3
+    assert calls["rope"](n_tokens=INT_MAX, n_heads=2) == -3
+    assert calls["rope"](n_heads=INT_MAX // 64) == -3
+    assert calls["rope"](n_heads=8193, head_dim=2, rotary_dim=2) == -3
+    assert calls["append"](p=dict(n_tokens=INT_MAX), s=dict(n_tokens=INT_MAX)) == -3
+    assert calls["attention"](s=dict(n_tokens=INT_MAX)) == -3
+    assert calls["attention"](s=dict(n_seqs=INT_MAX)) == -3
+    assert calls["lora"](n_tokens=INT_MAX) == -3
+    assert calls["lora"](n_seqs=INT_MAX) == -3
+
+
+def test_misaligned_workspace(calls):
+    assert calls["attention"](a=dict(workspace=AT + 16, workspace_bytes=1 << 40)) == -1
+    assert calls["lora"](workspace=AT + 16, workspace_bytes=1 << 40) == -1
+
+
+def test_workspace_of_a_short_window_in_a_long_cache(calls):
+    """The split of the keys is bounded: a table of 2^30 positions and one token ask for some hundred parts, not for millions."""
+    import tiny_llm_amd as tqa
+    a = tqa.Attn(dtype=F32, n_heads=4, q=AT, out=AT, scale=0.125, causal=1, window=16)
+    c = tqa.KvCache(k=AT, v=AT, dtype=F16, n_pages=1, page_size=1 << 20, n_kv_heads=2, head_dim=64)
+    s = tqa.Seqs(n_seqs=1, n_tokens=1, q_start=AT, kv_len=AT, block_table=AT, table_stride=1023)
+    assert 0 < tqa.paged_attention_workspace(a, c, s) <= 1 << 20
+    a.window = INT_MAX
+    assert 0 < tqa.paged_attention_workspace(a, c, s) <= 1 << 20
 
 
 def test_too_small_a_workspace(calls):

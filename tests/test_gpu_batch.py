@@ -216,6 +216,13 @@ def test_attention_chunks(gpu, act, cache, Hq, Hk, D):
     check_attention(gpu, b, act, Hq, 1, 0)
 
 
+@pytest.mark.parametrize("new", [[1, 1], [40, 3]])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_attention_scale_of_zero_and_below(gpu, new, scale):
+    b = Batch(gpu, new, [150, 60], 16, 1, 64, F16, seed=20)
+    check_attention(gpu, b, F32, 3, 1, 0, scale=scale)
+
+
 @pytest.mark.parametrize("page", [1, 7, 40, 64, 1000])
 def test_attention_page_sizes(gpu, page):
     b = Batch(gpu, [33, 1, 3], [200, 333, 70], page, 2, 64, F16, seed=page)
@@ -340,3 +347,288 @@ def test_attention_masked_infinities_and_nan(gpu, cache, D):
     assert np.linalg.norm((got - want)[one][..., keep]) <= 2.0 ** -17 * np.linalg.norm(want[one][..., keep])
     assert not np.isfinite(got[one][..., 5]).any()
     assert np.isnan(got[[t for t in range(n) if first + t >= 133]]).all()
+
+
+def test_kv_append_keys_alone_at_given_positions(gpu):
+    """No queries, angles of the caller's positions, no rotation of the rest of the head."""
+    b = Batch(gpu, [2, 1, 4], [9, 30, 4], 8, 2, 64, F32, seed=30)
+    T = b.tokens
+    s = head_inputs(gpu, b.rng, T, 4, 2, 64, F32, False, True)
+    pos = np.array([1000, 3, 70000, 0, 5, 6, 9])
+    d_pos = ints(gpu, pos)
+    p = proj_of(gpu, s, T, 4, 2, 64, F32, 32, None, None, d_pos)
+    p.q = None
+    gpu.kv_append_dev(p, b.c, b.s)
+    gpu.synchronize()
+    want, size = ref.finish_heads(s["k"][2], None, s["k_norm"][0], pos, 32, 1e-6, 1e6)
+    got_k, got_v = b.k.read(), b.v.read()
+    for t, at in b.token_positions().items():
+        check_heads(got_k[b.place(*at)], want[t], size[t], F32, f"k of token {t}")
+        assert np.array_equal(got_v[b.place(*at)], s["v"][2][t])
+
+
+def test_positions_past_the_table_do_not_exist(gpu):
+    """A cached length beyond the table's pages: the rows past them are neither written nor attended to."""
+    b = Batch(gpu, [3, 1], [32, 20], 16, 1, 64, F16, seed=31)  # (the table has three entries a sequence)
+    b.kv = [50, 20]
+    b.d_kv = ints(gpu, b.kv)
+    b.s.kv_len, b.s.max_kv = b.d_kv.ptr, 50
+    before = b.k.read_bits()
+    s = head_inputs(gpu, b.rng, b.tokens, 2, 1, 64, F32, False, False)
+    q_out = Dev(gpu, np.full((b.tokens, 2, 64), 7.0), F32)
+    gpu.kv_append_dev(proj_of(gpu, s, b.tokens, 2, 1, 64, F32, 64, q_out), b.c, b.s)
+    gpu.synchronize()
+    after = b.k.read_bits()
+    changed = np.argwhere((before != after).any((2, 3)))
+    assert [tuple(c) for c in changed] == [b.place(1, 19)]  # positions 47..49 of sequence 0 are past its pages
+    b.k.values, b.v.values = b.k.read(), b.v.read()
+    check_attention(gpu, b, F32, 2, 1, 0)
+
+
+@pytest.mark.parametrize("new,kv", [([1, 1], [700, 2600]), ([300, 64], [900, 2600])])
+@pytest.mark.parametrize("window", [0, 50, 2 ** 31 - 1])
+@pytest.mark.parametrize("max_kv", [1, 300, 2 ** 31 - 1])
+def test_attention_split_by_a_wrong_length(gpu, new, kv, window, max_kv):
+    """max_kv decides how the work is split and nothing else, too small and too large ones too."""
+    b = Batch(gpu, new, kv, 16, 1, 64, F16, seed=35)
+    b.s.max_kv = max_kv
+    check_attention(gpu, b, F32, 2, 1, window)
+
+
+def test_many_sequences(gpu):
+    """More sequences than two rounds of the search cover, most without tokens, and their tokens found by all the calls."""
+    rng = np.random.default_rng(32)
+    B, D = 5000, 64
+    new = (rng.random(B) < 0.03).astype(int)
+    new[[0, 63, 64, 4095, 4096, 4999]] = [2, 1, 3, 1, 17, 1]
+    kv = np.where(new > 0, rng.integers(0, 12, B) + new, 0)
+    b = Batch(gpu, new, kv, 4, 1, D, F32, seed=33, tail=1)
+    s = head_inputs(gpu, b.rng, b.tokens, 2, 1, D, F32, False, True)
+    q_out = Dev(gpu, np.full((b.tokens, 2, D), 7.0), F32)
+    gpu.kv_append_dev(proj_of(gpu, s, b.tokens, 2, 1, D, F32, D, q_out), b.c, b.s)
+    gpu.synchronize()
+    at = b.token_positions()
+    assert len(at) == b.tokens - 1
+    pos = np.array([at.get(t, (0, 0))[1] for t in range(b.tokens)])
+    want, size = ref.finish_heads(s["k"][2], None, s["k_norm"][0], pos, D, 1e-6, 1e6)
+    got = b.k.read()
+    for t, a in at.items():
+        check_heads(got[b.place(*a)], want[t], size[t], F32, f"token {t}")
+    b.k.values, b.v.values = b.k.read(), b.v.read()
+    check_attention(gpu, b, F32, 2, 1, 0)
+    K, M, r, n = 32, 20, 4, 3
+    x, base = rng.standard_normal((b.tokens, K)).astype(np.float32), rng.standard_normal((b.tokens, M)).astype(np.float32)
+    a_, b_ = Dev(gpu, rng.standard_normal((n, r, K)), F16), Dev(gpu, rng.standard_normal((n, M, r)), F16)
+    scale, of = np.float32([1, 2, 0.5]), rng.integers(-1, n, B)
+    dx, db, ds, dof, dy = f32_buffer(gpu, x), f32_buffer(gpu, base), f32_buffer(gpu, scale), ints(gpu, of), f32_buffer(gpu, base)
+    gpu.lora_add_dev(gpu.Lora(dtype=F16, n_tokens=b.tokens, in_dim=K, out_dim=M, rank=r, n_adapters=n, n_seqs=B, x=dx.ptr, base=db.ptr, y=dy.ptr,
+                              a=a_.ptr, b=b_.ptr, scale=ds.ptr, q_start=b.d_start.ptr, adapter=dof.ptr))
+    gpu.synchronize()
+    want, size = ref.lora(x.astype(np.float64), base.astype(np.float64), a_.values, b_.values, scale, b.starts, of, b.tokens)
+    assert np.all(np.abs(dy.download(np.float32, base.size).reshape(base.shape) - want) <= (K + r + 8) * U * size)
+
+
+def test_rows_past_4_gib(gpu):
+    """Pages more than 2^31 elements apart in one allocation: appended to and attended to."""
+    D, page, far = 64, 16, (1 << 31) + 4096
+    room = gpu.DeviceBuffer(2 * (far + 2 * page * D))
+    start, kv, table = ints(gpu, [0, 20]), ints(gpu, [20]), ints(gpu, [[1, 0]])
+    cache = gpu.KvCache(k=room.ptr, v=room.ptr + 2 * page * D, dtype=F16, n_pages=2, page_size=page, n_kv_heads=1, head_dim=D, page_stride=far,
+                        token_stride=D, head_stride=D)
+    seqs = gpu.Seqs(n_seqs=1, n_tokens=20, q_start=start.ptr, kv_len=kv.ptr, block_table=table.ptr, table_stride=2, max_kv=20)
+    rng = np.random.default_rng(34)
+    s = head_inputs(gpu, rng, 20, 2, 1, D, F32, False, False)
+    q_out, out = Dev(gpu, np.zeros((20, 2, D)), F32), Dev(gpu, np.zeros((20, 2, D)), F32)
+    gpu.kv_append_dev(proj_of(gpu, s, 20, 2, 1, D, F32, 0, q_out), cache, seqs)
+    gpu.paged_attention_dev(gpu.Attn(dtype=F32, n_heads=2, q=q_out.ptr, out=out.ptr, scale=0.125, causal=1), cache, seqs)
+    gpu.synchronize()
+    k, v = (s[n][2][:, 0].astype(np.float16).astype(np.float64) for n in ("k", "v"))
+    for h in range(2):
+        w = np.where(np.tri(20) > 0, s["q"][2][:, h] @ k.T / 8, -np.inf)
+        w = np.exp(w - w.max(-1, keepdims=True))
+        want = w / w.sum(-1, keepdims=True) @ v
+        assert np.linalg.norm(out.read()[:, h] - want) <= 2.0 ** -17 * np.linalg.norm(want)
+
+
+def test_same_bits_again_and_on_two_streams(gpu):
+    """Calls that overlap on two streams, each with scratch of its own, give what each gives alone, again and again."""
+    cases = []
+    for seed, new, kv in ((40, [1] * 6, [3000, 10, 700, 1, 64, 2100]), (41, [150, 20], [2500, 900])):
+        b = Batch(gpu, new, kv, 16, 2, 128, F16, seed=seed)
+        q = Dev(gpu, b.rng.standard_normal((b.tokens, 8, 128)), F32)
+        out = Dev(gpu, np.zeros((b.tokens, 8, 128)), F32)
+        x, y = f32_buffer(gpu, b.rng.standard_normal((b.tokens, 512))), f32_buffer(gpu, np.zeros((b.tokens, 260)))
+        a_, b_ = Dev(gpu, b.rng.standard_normal((2, 24, 512)), BF16), Dev(gpu, b.rng.standard_normal((2, 260, 24)), BF16)
+        sc, of = f32_buffer(gpu, [1.0, 2.0]), ints(gpu, [i % 2 for i in range(len(new))])
+        lo = gpu.Lora(dtype=BF16, n_tokens=b.tokens, in_dim=512, out_dim=260, rank=24, n_adapters=2, n_seqs=len(new), x=x.ptr, y=y.ptr, a=a_.ptr,
+                      b=b_.ptr, scale=sc.ptr, q_start=b.d_start.ptr, adapter=of.ptr)
+        at = gpu.Attn(dtype=F32, n_heads=8, q=q.ptr, out=out.ptr, scale=0.1, causal=1)
+        cases.append((b, at, lo, out, y, gpu.Stream(), (q, x, a_, b_, sc, of)))
+    first = []
+    for b, at, lo, out, y, stream, _ in cases:
+        gpu.paged_attention_dev(at, b.c, b.s, stream)
+        gpu.lora_add_dev(lo, stream)
+        stream.synchronize()
+        first.append((out.read_bits(), y.download(np.int32, b.tokens * 260)))
+    for _ in range(4):
+        for b, at, lo, out, y, stream, _ in cases * 3:
+            gpu.paged_attention_dev(at, b.c, b.s, stream)
+            gpu.lora_add_dev(lo, stream)
+        for (b, at, lo, out, y, stream, _), (o1, y1) in zip(cases, first):
+            stream.synchronize()
+            assert np.array_equal(out.read_bits(), o1) and np.array_equal(y.download(np.int32, b.tokens * 260), y1)
+
+
+def layer_ops(gpu, b, w, bufs, T, Hq, Hk, D, H, act_stride=None):
+    """One attention block of a layer for the T tokens of the batch as an op list: q, k, v projections with an adapter beside q, k and v
+    appended, attention, o projection. Returns the ops and the structs that they name."""
+    proj = gpu.HeadProj(dtype=F32, n_tokens=T, n_heads=Hq, n_kv_heads=Hk, head_dim=D, rotary_dim=D, q=bufs["q"].ptr, k=bufs["k"].ptr, v=bufs["v"].ptr,
+                        q_out=bufs["q"].ptr, q_norm=w["qn"].ptr, k_norm=w["kn"].ptr, eps=1e-6, theta=1e6)
+    attn = gpu.Attn(dtype=F32, n_heads=Hq, q=bufs["q"].ptr, out=bufs["attn"].ptr, scale=D ** -0.5, causal=1)
+    lora = gpu.Lora(dtype=F16, n_tokens=T, in_dim=H, out_dim=Hq * D, rank=8, n_adapters=2, n_seqs=len(b.new), x=bufs["x"].ptr, base=bufs["q"].ptr,
+                    y=bufs["q"].ptr, a=w["a"].ptr, b=w["b"].ptr, scale=w["s"].ptr, q_start=b.d_start.ptr, adapter=w["of"].ptr)
+    mm = lambda name, x, y, m, k: gpu.Op(gpu.OP_I4_MATMUL, w[name].ptr, bufs[x].ptr, bufs[y].ptr, m, k, T, 64, None, None, None, None, 0)  # noqa: E731
+    ops = [mm("wq", "x", "q", Hq * D, H), mm("wk", "x", "k", Hk * D, H), mm("wv", "x", "v", Hk * D, H), gpu.batch_op(gpu.OP_LORA_ADD, lora),
+           gpu.batch_op(gpu.OP_KV_APPEND, proj, b.c, b.s), gpu.batch_op(gpu.OP_PAGED_ATTENTION, attn, b.c, b.s), mm("wo", "attn", "y", H, Hq * D)]
+    return ops, (proj, attn, lora)
+
+
+def test_attention_block_of_prompts_and_decode_steps(gpu, orc):
+    """The calls together, as a runtime makes them: prompts in one batch, then decode steps replayed from a captured op list whose
+    device arrays (lengths, activations) change between replays. Each replay equals the eager list bit for bit, and each stage
+    what the stage's plain form gives on the stage's own inputs."""
+    Hq, Hk, D, H, steps = 4, 2, 64, 256, 3
+    lens = [5, 33, 1]
+    rng = np.random.default_rng(50)
+    w = {n: gpu.synth_i4(m, k, 64, seed=60 + i) for i, (n, m, k) in enumerate((("wq", Hq * D, H), ("wk", Hk * D, H), ("wv", Hk * D, H), ("wo", H, Hq * D)))}
+    host = dict(w)
+    w = {n: gpu.DeviceBuffer.from_array(x) for n, x in w.items()}
+    a_, b_ = Dev(gpu, rng.standard_normal((2, 8, H)) / 16, F16), Dev(gpu, 0.3 * rng.standard_normal((2, Hq * D, 8)), F16)
+    qn, kn = (1 + 0.1 * rng.standard_normal((2, D))).astype(np.float32)
+    sc, of = np.float32([1.5, 0.5]), [1, -1, 0]
+    w.update(a=a_, b=b_, qn=f32_buffer(gpu, qn), kn=f32_buffer(gpu, kn), s=f32_buffer(gpu, sc), of=ints(gpu, of))
+
+    def plain(b, bufs, x, T):
+        """q, k, v after the projections and the adapter, then everything after them, from the i4 oracle and the plain forms."""
+        m = lambda n, v, rows, cols: orc.matmul_i4(host[n], np.ascontiguousarray(v, np.float32).ravel(), rows, cols, T, 64).reshape(T, rows)  # noqa: E731
+        q = ref.lora(x.astype(np.float64), m("wq", x, Hq * D, H).astype(np.float64), a_.values, b_.values, sc, b.starts, of, T)[0]
+        k, v = m("wk", x, Hk * D, H), m("wv", x, Hk * D, H)
+        at = b.token_positions()
+        pos = np.array([at[t][1] for t in range(T)])
+        q = ref.finish_heads(q.reshape(T, Hq, D), None, qn, pos, D, 1e-6, 1e6)[0]
+        k = ref.finish_heads(k.astype(np.float64).reshape(T, Hk, D), None, kn, pos, D, 1e-6, 1e6)[0]
+        for t in range(T):
+            pl = b.place(*at[t])
+            b.k.values[pl], b.v.values[pl] = k[t], v[t].reshape(Hk, D)
+        o = ref.attention(b, q, D ** -0.5, 1, 0)[0]
+        return m("wo", o.reshape(T, Hq * D), H, Hq * D)
+
+    def buffers(T):
+        return {n: gpu.DeviceBuffer(4 * T * m) for n, m in (("x", H), ("q", Hq * D), ("k", Hk * D), ("v", Hk * D), ("attn", Hq * D), ("y", H))}
+
+    # prompts: the pages have room for the steps after them
+    b = Batch(gpu, lens, [n + steps for n in lens], 16, Hk, D, F16, seed=51, fill=0.0)
+    b.kv = list(lens)
+    b.d_kv.upload(np.int32(b.kv))
+    T = b.tokens
+    bufs = buffers(T)
+    x = rng.standard_normal((T, H)).astype(np.float32)
+    bufs["x"].upload(x)
+    stream = gpu.Stream()
+    ops, keep = layer_ops(gpu, b, w, bufs, T, Hq, Hk, D, H)
+    gpu.run_ops(ops, 1, stream)
+    stream.synchronize()
+    want = plain(b, bufs, x, T)
+    got = bufs["y"].download(np.float32, T * H).reshape(T, H)
+    # fp16 operands in the projections: 4e-4 of them in L2 (1e-3 at most), through two of them, and fp16 rows in the cache
+    assert np.linalg.norm(got - want) <= 4e-3 * np.linalg.norm(want)
+
+    # decode steps
+    b.new, b.starts, b.tokens = [1, 1, 1], np.arange(4), 3
+    b.d_start = ints(gpu, b.starts)
+    b.s = gpu.Seqs(n_seqs=3, n_tokens=3, q_start=b.d_start.ptr, kv_len=b.d_kv.ptr, block_table=b.d_table.ptr, table_stride=b.stride, max_kv=0)
+    bufs = buffers(3)
+    ops, keep = layer_ops(gpu, b, w, bufs, 3, Hq, Hk, D, H)
+    b.kv = [n + 1 for n in lens]
+    b.d_kv.upload(np.int32(b.kv))
+    bufs["x"].upload(np.zeros((3, H), np.float32))
+    graph = gpu.OpsGraph(ops, stream)
+    for step in range(steps):
+        b.kv = [n + 1 + step for n in lens]
+        b.d_kv.upload(np.int32(b.kv))
+        x = rng.standard_normal((3, H)).astype(np.float32)
+        bufs["x"].upload(x)
+        gpu.run_ops(ops, 1, stream)
+        stream.synchronize()
+        eager = [bufs["y"].download(np.int32, 3 * H), b.k.read_bits(), b.v.read_bits()]
+        for _ in range(2):
+            bufs["x"].upload(x)
+            graph.launch()
+            stream.synchronize()
+            again = [bufs["y"].download(np.int32, 3 * H), b.k.read_bits(), b.v.read_bits()]
+            assert all(np.array_equal(p, q) for p, q in zip(eager, again)), f"step {step}"
+        want = plain(b, bufs, x, 3)
+        got = bufs["y"].download(np.float32, 3 * H).reshape(3, H)
+        assert np.linalg.norm(got - want) <= 4e-3 * np.linalg.norm(want), f"step {step}"
+    graph.close()
+
+
+class Hip:
+    """The runtime's capture calls, which the library does not wrap (a caller that captures for itself has them)."""
+
+    def __init__(self):
+        import ctypes
+        self.c = ctypes
+        self.lib = ctypes.CDLL("libamdhip64.so")
+
+    def begin(self, stream):
+        assert self.lib.hipStreamBeginCapture(self.c.c_void_p(stream.ptr), 2) == 0  # relaxed
+
+    def end(self, stream):
+        g = self.c.c_void_p()
+        assert self.lib.hipStreamEndCapture(self.c.c_void_p(stream.ptr), self.c.byref(g)) == 0
+        return g
+
+    def replay(self, g, stream, times):
+        e = self.c.c_void_p()
+        assert self.lib.hipGraphInstantiate(self.c.byref(e), g, None, None, self.c.c_size_t(0)) == 0
+        for _ in range(times):
+            assert self.lib.hipGraphLaunch(e, self.c.c_void_p(stream.ptr)) == 0
+            stream.synchronize()
+        assert self.lib.hipGraphExecDestroy(e) == 0 and self.lib.hipGraphDestroy(g) == 0
+
+
+def test_own_capture_needs_a_workspace(gpu):
+    """Under the caller's own capture the calls that need scratch are refused without a workspace, and run with one."""
+    hip, stream = Hip(), gpu.Stream()
+    b = Batch(gpu, [1, 1], [3000, 1200], 16, 1, 64, F16, seed=70)
+    q, out = Dev(gpu, b.rng.standard_normal((2, 4, 64)), F32), Dev(gpu, np.zeros((2, 4, 64)), F32)
+    attn = gpu.Attn(dtype=F32, n_heads=4, q=q.ptr, out=out.ptr, scale=0.125, causal=1)
+    x, y = f32_buffer(gpu, b.rng.standard_normal((2, 64))), f32_buffer(gpu, np.zeros((2, 32)))
+    a_, b_ = Dev(gpu, b.rng.standard_normal((1, 4, 64)), F16), Dev(gpu, b.rng.standard_normal((1, 32, 4)), F16)
+    sc, of = f32_buffer(gpu, [1.0]), ints(gpu, [0, 0])
+    lora = gpu.Lora(dtype=F16, n_tokens=2, in_dim=64, out_dim=32, rank=4, n_adapters=1, n_seqs=2, x=x.ptr, y=y.ptr, a=a_.ptr, b=b_.ptr,
+                    scale=sc.ptr, q_start=b.d_start.ptr, adapter=of.ptr)
+    gpu.paged_attention_dev(attn, b.c, b.s, stream)
+    gpu.lora_add_dev(lora, stream)
+    stream.synchronize()
+    want = out.read_bits(), y.download(np.int32, 64)
+    out.buf.upload(np.zeros((2, 4, 64), np.float32))
+    y.upload(np.zeros(64, np.float32))
+    need = gpu.paged_attention_workspace(attn, b.c, b.s), gpu.lora_workspace(lora)
+    assert need[0] > 0 and need[1] > 0
+    spaces = [gpu.DeviceBuffer(n) for n in need]
+    lib = gpu.lib()
+    hip.begin(stream)
+    refused = lib.tqhip_paged_attention_dev(attn, b.c, b.s, stream.ptr), lib.tqhip_lora_add_dev(lora, stream.ptr)
+    for struct, space, n in ((attn, spaces[0], need[0]), (lora, spaces[1], need[1])):
+        struct.workspace, struct.workspace_bytes = space.ptr, n
+    ran = lib.tqhip_paged_attention_dev(attn, b.c, b.s, stream.ptr), lib.tqhip_lora_add_dev(lora, stream.ptr)
+    g = hip.end(stream)
+    assert refused == (gpu.ENOSCRATCH, gpu.ENOSCRATCH) and ran == (0, 0)
+    hip.replay(g, stream, 3)
+    assert np.array_equal(out.read_bits(), want[0]) and np.array_equal(y.download(np.int32, 64), want[1])
+    attn.workspace_bytes -= 1
+    lora.workspace_bytes -= 1
+    assert lib.tqhip_paged_attention_dev(attn, b.c, b.s, stream.ptr) == gpu.ENOSCRATCH
+    assert lib.tqhip_lora_add_dev(lora, stream.ptr) == gpu.ENOSCRATCH

@@ -199,24 +199,24 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a) {
 }
 
 template <typename T, typename C, bool APPEND>
-void launch_heads(HeadArgs a, bool wide, hipStream_t s) {
+int launch_heads(HeadArgs a, bool wide, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const int lph = wide ? a.D / (2 * V) : 64;
     const int iters = (a.heads[0] + a.heads[1] + a.heads[2] + 64 / lph - 1) / (64 / lph);
     // A wave takes up to kHeadRounds rounds of heads, fewer where that gives every CU eight waves.
     const int64_t want = int64_t{8} * device_cu_count() / a.n_tokens;
     a.split = static_cast<int>(std::max<int64_t>((iters + kHeadRounds - 1) / kHeadRounds, std::min<int64_t>(iters, want)));
-    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.n_tokens) * a.split + kHeadWaves - 1) / kHeadWaves));
-    if (!wide) {
-        heads_kernel<T, C, 1, 64, APPEND><<<grid, kHeadThreads, 0, s>>>(a);
-        return;
-    }
-    switch (lph) {
+    const int64_t groups = (static_cast<int64_t>(a.n_tokens) * a.split + kHeadWaves - 1) / kHeadWaves;
+    if (groups > INT32_MAX / kHeadThreads) return kTooLarge;
+    const dim3 grid(static_cast<unsigned>(groups));
+    switch (wide ? lph : 0) {
+        case 0: heads_kernel<T, C, 1, 64, APPEND><<<grid, kHeadThreads, 0, s>>>(a); break;
         case 4: heads_kernel<T, C, V, 4, APPEND><<<grid, kHeadThreads, 0, s>>>(a); break;
         case 8: heads_kernel<T, C, V, 8, APPEND><<<grid, kHeadThreads, 0, s>>>(a); break;
         case 16: heads_kernel<T, C, V, 16, APPEND><<<grid, kHeadThreads, 0, s>>>(a); break;
         default: heads_kernel<T, C, V, 32, APPEND><<<grid, kHeadThreads, 0, s>>>(a); break;
     }
+    return hipGetLastError() == hipSuccess ? kOk : kLaunchFailed;
 }
 
 bool aligned(const void *p, int64_t stride, int bytes) {
@@ -233,7 +233,7 @@ int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip
     if (!cache && !p.positions && p.rotary_dim) return kBadShape;
     if (p.rotary_dim && !p.inv_freq && !(p.theta > 0.0 && std::isfinite(p.theta))) return kBadShape;
     if (!(p.eps >= 0.0f)) return kBadShape;
-    if (static_cast<int64_t>(std::max(p.n_heads, p.n_kv_heads)) * p.head_dim > INT32_MAX / 4) return kTooLarge;
+    if (std::max(p.n_heads, p.n_kv_heads) > 8192) return kTooLarge;  // (rounds of all heads times their parts fit 32 bits)
     HeadArgs a{{p.q, p.k, p.v}, {}, {p.q_bias, p.k_bias, p.v_bias}, {p.q_norm, p.k_norm}, {p.q_out, p.k_out}, {},
                {nullptr, nullptr}, {q ? p.n_heads : 0, k ? p.n_kv_heads : 0, cache ? p.n_kv_heads : 0}, p.n_tokens,
                p.head_dim, p.rotary_dim, p.eps, p.rotary_dim && !p.inv_freq ? std::log2(p.theta) : 0.0, p.inv_freq,
@@ -255,11 +255,10 @@ int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip
     if (!cache) {
         if (k) wide = wide && aligned(p.k_out, a.out_stride[1], bytes);
         switch (p.dtype) {
-            case TQHIP_F32: launch_heads<float, float, false>(a, wide, s); break;
-            case TQHIP_F16: launch_heads<f16, f16, false>(a, wide, s); break;
-            default: launch_heads<bf16, bf16, false>(a, wide, s); break;
+            case TQHIP_F32: return launch_heads<float, float, false>(a, wide, s);
+            case TQHIP_F16: return launch_heads<f16, f16, false>(a, wide, s);
+            default: return launch_heads<bf16, bf16, false>(a, wide, s);
         }
-        return hipGetLastError() == hipSuccess ? kOk : kLaunchFailed;
     }
     const int st = check_cache(*cache, *seqs);
     if (st != kOk) return st;
@@ -277,18 +276,13 @@ int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip
     const int cb = type_bytes(cache->dtype);
     for (const void *c : {cache->k, cache->v}) wide = wide && aligned(c, a.pages.page_stride, cb);
     wide = wide && a.pages.token_stride * cb % 16 == 0 && a.pages.head_stride * cb % 16 == 0;
-    if (p.dtype == TQHIP_F16) {
-        launch_heads<f16, f16, true>(a, wide, s);
-    } else if (p.dtype == TQHIP_BF16) {
-        launch_heads<bf16, bf16, true>(a, wide, s);
-    } else {
-        switch (cache->dtype) {
-            case TQHIP_F32: launch_heads<float, float, true>(a, wide, s); break;
-            case TQHIP_F16: launch_heads<float, f16, true>(a, wide, s); break;
-            default: launch_heads<float, bf16, true>(a, wide, s); break;
-        }
+    if (p.dtype == TQHIP_F16) return launch_heads<f16, f16, true>(a, wide, s);
+    if (p.dtype == TQHIP_BF16) return launch_heads<bf16, bf16, true>(a, wide, s);
+    switch (cache->dtype) {
+        case TQHIP_F32: return launch_heads<float, float, true>(a, wide, s);
+        case TQHIP_F16: return launch_heads<float, f16, true>(a, wide, s);
+        default: return launch_heads<float, bf16, true>(a, wide, s);
     }
-    return hipGetLastError() == hipSuccess ? kOk : kLaunchFailed;
 }
 
 }  // namespace

@@ -307,8 +307,9 @@ int check_lora(const tqhip_lora &l) {
     if (!type_known(l.dtype) || l.n_tokens < 1 || l.in_dim < 1 || l.out_dim < 1 || l.rank < 1 || l.rank > 256 ||
         l.n_adapters < 1 || l.n_seqs < 1 || !l.x || !l.y || !l.a || !l.b || !l.scale || !l.q_start || !l.adapter)
         return kBadShape;
-    // tiles in grid.x, blocks of outputs in grid.y; everything else is addressed in 64 bits
-    if (static_cast<int64_t>(l.n_tokens) + l.n_seqs > INT32_MAX / 256 || l.out_dim > 65535 * 128 || l.in_dim > INT32_MAX - 64)
+    // tiles of at least 16 tokens in grid.x, of up to 1024 threads, blocks of outputs in grid.y; everything else is addressed in 64 bits
+    if (static_cast<int64_t>(l.n_tokens) / 16 + l.n_seqs > INT32_MAX / 1024 || l.n_tokens > INT32_MAX / 16 || l.out_dim > 65535 * 128 ||
+        l.in_dim > INT32_MAX - 64)
         return kTooLarge;
     return kOk;
 }
@@ -336,7 +337,7 @@ void launch_expand(const LoraArgs &p, const LoraPlan &n, bool wide_y, hipStream_
 template <typename W>
 void launch_lora(const LoraArgs &p, const LoraPlan &n, hipStream_t s) {
     const auto on16 = [](const void *q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
-    const bool wide_a = p.K % 8 == 0 && on16(p.x) && on16(p.a), wide_b = p.rank % 8 == 0 && on16(p.b) && on16(p.u);
+    const bool wide_a = p.K % 8 == 0 && on16(p.x) && on16(p.a), wide_b = p.rank % 8 == 0 && on16(p.b);
     const bool wide_y = p.M % 4 == 0 && on16(p.y) && on16(p.base);
     const auto shrink = [&](auto wide) {
         if (p.rank <= 16)
@@ -375,6 +376,7 @@ int run_lora(const tqhip_lora &l, hipStream_t s) {
     if (st != kOk) return st;
     const size_t bytes = lora_bytes(l);
     void *ws = l.workspace;
+    if (reinterpret_cast<uintptr_t>(ws) % 256) return kBadShape;
     if (ws && l.workspace_bytes < bytes) return kNoScratch;
     if (!ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
     const LoraPlan n = lora_plan(l);

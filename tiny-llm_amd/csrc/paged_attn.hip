@@ -858,6 +858,8 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
 // ---- host ----------------------------------------------------------------------------------------
 
 // How the work is cut, from the host's numbers alone.
+constexpr int kMaxParts = 512;  // (a short window in a long cache asks for many, most of them empty)
+
 struct Plan {
     bool few;
     int tiles, parts, span;
@@ -876,7 +878,7 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
     const int64_t most = static_cast<int64_t>(s.table_stride) * c.page_size;
     const int64_t kv = s.max_kv > 0 ? std::min<int64_t>(s.max_kv, most) : most;
     // keys that one tile reads
-    const int64_t seen = p.causal && p.window > 0 ? std::min<int64_t>(kv, p.window + (n.few ? kFewRows : kTileRows)) : kv;
+    const int64_t seen = p.causal && p.window > 0 ? std::min<int64_t>(kv, int64_t{p.window} + (n.few ? kFewRows : kTileRows)) : kv;
     const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads, cus = device_cu_count();
     const auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
     if (n.few) {
@@ -894,6 +896,7 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
         const int64_t parts = 2 * blocks >= 3 * slots ? 1 : (3 * slots + blocks - 1) / blocks;
         n.span = static_cast<int>(parts == 1 ? kv : std::min(kv, std::max<int64_t>(512, up((seen + parts - 1) / parts, 64))));
     }
+    if (kv > int64_t{kMaxParts} * n.span) n.span = static_cast<int>(up(kv, int64_t{kMaxParts} * 128) / kMaxParts);
     n.parts = static_cast<int>((kv + n.span - 1) / n.span);
     return n;
 }
@@ -914,7 +917,7 @@ void launch_dim(const AttnArgs &a, const Plan &n, hipStream_t s) {
         attn_tiles<T, C, D><<<grid, 256, 0, s>>>(a);
     if (n.parts == 1) return;
     const int rows = a.n_tokens * a.n_heads;
-    if (n.parts > 8)
+    if (n.parts > 8 && rows <= INT32_MAX / 256)  // (a launch has less than 2^32 threads along x)
         attn_join<T, D, 4><<<rows, 256, 0, s>>>(a);
     else
         attn_join<T, D, 1><<<(rows + 3) / 4, 256, 0, s>>>(a);
@@ -934,7 +937,7 @@ int check_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s
     const int st = check_cache(c, s);
     if (st != kOk) return st;
     if (!p.q || !p.out || !type_known(p.dtype) || p.n_heads < 1 || p.n_heads % c.n_kv_heads || p.window < 0 ||
-        !std::isfinite(p.scale) || (p.dtype != TQHIP_F32 && c.dtype != p.dtype))
+        !std::isfinite(p.scale * 1.4426950408889634f) || (p.dtype != TQHIP_F32 && c.dtype != p.dtype))
         return kBadShape;
     if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return kBadShape;
     const int qb = type_bytes(p.dtype), cb = type_bytes(c.dtype);
@@ -946,8 +949,8 @@ int check_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s
         return kBadShape;
     const int64_t row = static_cast<int64_t>(p.n_heads) * c.head_dim;
     if (s.n_tokens > 1 && ((p.q_stride && p.q_stride < row) || (p.out_stride && p.out_stride < row))) return kBadShape;
-    if (p.n_heads > 65535 || static_cast<int64_t>(s.n_tokens) * p.n_heads > INT32_MAX / 4 ||
-        static_cast<int64_t>(s.n_seqs) * p.n_heads > INT32_MAX / 4)
+    // workgroups along x, of 256 threads: a sixteenth of the rows and one a sequence and key/value head, then a quarter of the rows
+    if (static_cast<int64_t>(s.n_tokens) * p.n_heads > INT32_MAX / 32 || static_cast<int64_t>(s.n_seqs) * p.n_heads > INT32_MAX / 256)
         return kTooLarge;
     return kOk;
 }
@@ -958,6 +961,7 @@ int run_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &b, 
     const Plan n = plan(p, c, b);
     const size_t bytes = plan_bytes(n, p, c, b);
     void *ws = p.workspace;
+    if (reinterpret_cast<uintptr_t>(ws) % 256) return kBadShape;
     if (ws && p.workspace_bytes < bytes) return kNoScratch;
     if (bytes && !ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
     const int64_t row = static_cast<int64_t>(p.n_heads) * c.head_dim;
