@@ -395,6 +395,24 @@ def test_attention_split_by_a_wrong_length(gpu, new, kv, window, max_kv):
     check_attention(gpu, b, F32, 2, 1, window)
 
 
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 30, -2 ** 31, -1, 0])
+@pytest.mark.parametrize("new", [[1, 1], [120, 30]])
+@pytest.mark.parametrize("page", [1, 16])
+def test_lengths_that_no_table_holds(gpu, length, new, page):
+    """A sequence whose window lies past its table, or whose length is no length, gets zeros; the other one is as ever."""
+    b = Batch(gpu, new, [150, 140], page, 1, 64, F16, seed=36)
+    q, out = Dev(gpu, b.rng.standard_normal((b.tokens, 2, 64)), F32), Dev(gpu, np.full((b.tokens, 2, 64), 7.0), F32)
+    attn = gpu.Attn(dtype=F32, n_heads=2, q=q.ptr, out=out.ptr, scale=0.125, causal=1, window=20)
+    gpu.paged_attention_dev(attn, b.c, b.s)
+    gpu.synchronize()
+    want = out.read()
+    want[: new[0]] = 0
+    b.d_kv.upload(np.int32([length, 140]))
+    gpu.paged_attention_dev(attn, b.c, b.s)
+    gpu.synchronize()
+    assert np.array_equal(out.read(), want)
+
+
 def test_many_sequences(gpu):
     """More sequences than two rounds of the search cover, most without tokens, and their tokens found by all the calls."""
     rng = np.random.default_rng(32)

@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     const int rows = t.n * a.group;
     const int last = min(t.r0 + kFewRows, rows) - 1;
     const int p_first = t.pos0 + t.r0 / a.group, p_last = t.pos0 + last / a.group;
-    int kb = key_lo(a, p_first), ke = key_hi(a, p_last, t.len);
+    int ke = key_hi(a, p_last, t.len), kb = max(min(key_lo(a, p_first), ke), 0);  // (a window past the table is empty)
     if (a.parts > 1) {
         kb = max(kb, static_cast<int>(blockIdx.y) * a.span);
         if (static_cast<int>(blockIdx.y) < a.parts - 1) ke = min(ke, (static_cast<int>(blockIdx.y) + 1) * a.span);
@@ -564,7 +564,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     const int rows = t.n * a.group;
     const int last = min(t.r0 + kTileRows, rows) - 1;
     const int p_first = t.pos0 + t.r0 / a.group, p_last = t.pos0 + last / a.group;
-    int kb = key_lo(a, p_first), ke = key_hi(a, p_last, t.len);
+    int ke = key_hi(a, p_last, t.len), kb = max(min(key_lo(a, p_first), ke), 0);  // (a window past the table is empty)
     if (a.parts > 1) {
         kb = max(kb, static_cast<int>(blockIdx.y) * a.span);
         if (static_cast<int>(blockIdx.y) < a.parts - 1) ke = min(ke, (static_cast<int>(blockIdx.y) + 1) * a.span);
