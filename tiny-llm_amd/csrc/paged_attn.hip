@@ -283,6 +283,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
 
     const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride + 8 * g;
     const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride + 8 * g;
+    const auto swap = [](int row) { return (D == 64 ? row >> 1 & 3 : row & 7) << 1; };  // of a value row's chunks
     vec<C, 8> kr[2][2][NS], vr[kDirect ? 1 : 2][NS];
     // The lane's keys of a step are k0 + col and k0 + 16 + col. All loads of the loop are unconditional (a page past the table is its
     // last entry, a row that does not exist is row 0 of page 0): the compiler counts the loads that may stay under way at
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
                 const int64_t ro = __shfl(static_cast<long long>(max(o[first / 16], int64_t{0})), row & 15);
                 // (streamed: a decode step of 64 requests takes 397 us so, 420 without. K's lines are read in two halves, which
                 // streaming fetches twice: 451 us.)
-                global_to_lds<true>(vc - 8 * g + ro + ((lane % CH) ^ ((row & 3) << 1)) * 8, to + 64 * i * 8);
+                global_to_lds<true>(vc - 8 * g + ro + ((lane % CH) ^ swap(row)) * 8, to + 64 * i * 8);
             }
         } else {
             load_rows(vc, o, vr);
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const int i = lane & 15, row = 4 * g + i / 4;
-                const int ch = (2 * d + (i & 3) / 2) ^ (kDirect ? (row & 3) << 1 : 0);
+                const int ch = (2 * d + (i & 3) / 2) ^ (kDirect ? swap(row) : 0);
                 const E *v0 = (kDirect ? v_now : &sh.v[wave][0][0][0]) + row * VS + ch * 8 + 4 * (i & 1);
                 const vec<E, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 16 * VS);
                 const vec<E, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
     const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride;
     const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride;
     const auto key_swap = [](int row) { return (D == 64 ? row >> 1 : row) & (D == 64 ? 7 : 15); };
-    const auto value_swap = [](int row) { return (row & 3) << 1; };
+    const auto value_swap = [](int row) { return (row & 3) << (D == 64 ? 1 : 2); };
     vec<C, 8> kr[kDirect ? 1 : NCH], vr[kDirect ? 1 : NCH];
     // A tile's rows on their way: straight into LDS, 64 chunks in order per instruction, the lane choosing the global chunk that belongs
     // at its place, or into registers. For a key that does not exist row 0 of page 0 is loaded.
