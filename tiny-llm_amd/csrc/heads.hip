@@ -9,7 +9,12 @@
 // A head lies in D / (2 V) lanes of a wave, each holding V elements at u V and the V partners at
 // r/2 + u V in 16-byte loads, so norm and rotation stay in registers: the norm is a butterfly over
 // the head's lanes. A wave takes several heads of one token side by side and goes on to the token's
-// next heads with the same cosines and sines, and to its next token with the same frequencies.
+// next heads with the same cosines and sines. All of its loads go out before anything waits for one (a
+// load behind a store waits for that store: loads between the rounds' stores took 96 us where this takes 69).
+//
+// 8191 tokens of 32 + 8 heads of 128 in fp32, 335 MB read and written: 69 us, 4.85 TB/s, which is what a copy of such a
+// size reaches here (4.8 to 5.3). One token: 3.5 us, a launch and two dependent loads. 12520 tokens of 14 + 2 + 2
+// heads of 64 into bf16 pages, 109 MB: 26 us, 4.2 TB/s.
 //
 // Angles: turns = pos * freq / 2 pi in fp64, reduced to the nearest whole turn there (exact to 2^-53 of
 // the turns, so positions in the millions keep 30 bits of angle), then an fp32 sine of the remainder.

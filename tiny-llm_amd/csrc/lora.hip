@@ -6,6 +6,10 @@
 // Both are products on the matrix cores in bf16 terms: an fp32 operand (x, u, fp32 weights) is three
 // of them (24 bits), an fp16 weight two (all 11 bits, and fp16's range), a bf16 weight one; products below 2^-24 are
 // left out. So fp32 results keep fp32's precision at 3 to 6 matrix instructions a product, where the fp32 ones take 16.
+//
+// Both launches are bound by HBM (x once; base and y once; A and B stay in L2) or, with few tokens, by latency. 3555 tokens of 8
+// requests, rank 64 in bf16 beside 9728x2560: 26 and 73 us for 38 and 287 MB. 64 requests of a token, rank 16 in fp16 beside
+// 4096x2560: 5.7 and 7 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -89,7 +93,7 @@ __device__ inline int adapter_of(const LoraArgs &p, int b) {
 // u^T = A x^T for a tile of 16 tokens: the lane holds ranks 16 n + 4 g + i of token lane % 16. The steps of 32 along K are dealt to
 // the workgroup's waves, whose sums meet in LDS, and to gridDim.y workgroups where there are fewer tiles than CUs, whose sums
 // meet in lora_expand. x is read once. The launch lasts as long as one wave's loads one after the other, so the waves are many and
-// their steps few: 16 waves of 5 steps at K = 2560. (4 waves, 32 tokens and 4 workgroups a tile took 21 us for 3700 tokens, and
+// their steps few: 16 waves of 5 steps at K = 2560. (4 waves, 32 tokens and 4 workgroups a tile took 21 us for 3555 tokens, and
 // the four sums of u cost every workgroup of lora_expand as many bytes as its outputs.)
 template <int NR>
 constexpr int kShrinkWaves = NR <= 4 ? 16 : 8;
