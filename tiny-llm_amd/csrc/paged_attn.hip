@@ -18,9 +18,9 @@
 // (Every XCD taking all heads: 878 us instead of 789 for the prompts below.)
 //   64 tokens of 32 heads on 8 of 128, up to 16000 fp16 keys each (2.06 GB):        395 us, 5.2 TB/s
 //   two prompts of up to 8192, the same heads, all in bf16 (706 GFLOP):             789 us, 0.90 PFLOP/s
-//   four chunks of up to 257 fp32 tokens over up to 8000 fp16 keys, the same heads:  204 us (72 GFLOP of two terms each), 18 of them the join
+//   four chunks of up to 257 fp32 tokens over up to 8000 fp16 keys, the same heads:  204 us (72 GFLOP of two terms each), 17 of them the join
 //   three prompts of up to 5001 fp32 tokens, a window of 1000 bf16 keys, 14 heads on 2 of 64: 130 us (33.5 GFLOP of three terms each)
-//   one fp32 token of 14 heads on 2 of 64 over 3000 fp32 keys:                        9.5 us and 4.6 for the join
+//   one fp32 token of 14 heads on 2 of 64 over 3000 fp32 keys:                        9.4 us and 4.0 for the join
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -835,7 +835,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
 // out = sum over parts of 2^(least bias - bias) o, over the same sum of l. A lane of each wave holds a part's bias and sum (64 at a
 // time) and its factor. W waves share a token's head: with many parts (few rows) their outputs are dealt to four waves, whose
 // loads do not wait for one another and which meet in LDS; with few parts (many rows) one wave takes them all. (One wave with
-// a loop over the parts took 0.4 us a part; four waves for two parts cost a 2048-token prompt 20 us.)
+// a loop over the parts, a load at a time, took 0.4 us a part; four waves for two parts cost a 2048-token prompt 20 us.)
 template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     constexpr int V = D / 64;
@@ -844,12 +844,12 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     const int row = blockIdx.x * (4 / W) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
     const int token = row / a.n_heads, head = row - token * a.n_heads;
     if (token >= a.n_tokens) return;
+    const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts;
     int b, pos;
     if (!find_token(a.q_start, a.kv_len, a.n_seqs, token, b, pos)) return;
     const int len = min(a.kv_len[b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
     const int lo = key_lo(a, pos), hi = key_hi(a, pos, len);
     const int z0 = min(lo / a.span, a.parts - 1), z1 = hi > lo ? min((hi - 1) / a.span + 1, a.parts) : z0;
-    const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts;
     float acc[V] = {}, l = 0.0f, bias = INFINITY;  // of the parts so far: their least bias
     for (int z = z0; z < z1; z += 64) {
         const float2 ml = z + lane < z1 ? a.part_ml[at + z + lane] : make_float2(INFINITY, 0.0f);
@@ -862,12 +862,17 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] *= old;
         const int n = min(64, z1 - z);
-        for (int j = wave; j < n; j += W) {
-            const float fj = __shfl(f, j);
-            float o[V];
-            load_as_float<float, V>(a.part_o + (at + z + j) * D + lane * V, o);
+        for (int j = wave; j < n; j += 4 * W) {  // four parts' loads at a time
+            float o[4][V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += fj != 0.0f ? o[i] * fj : 0.0f;
+            for (int y = 0; y < 4; ++y)
+                load_as_float<float, V>(a.part_o + (at + z + min(j + y * W, n - 1)) * D + lane * V, o[y]);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const float fj = j + y * W < n ? __shfl(f, min(j + y * W, n - 1)) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] += fj != 0.0f ? o[y][i] * fj : 0.0f;
+            }
         }
     }
     if constexpr (W > 1) {
