@@ -650,3 +650,26 @@ def test_own_capture_needs_a_workspace(gpu):
     lora.workspace_bytes -= 1
     assert lib.tqhip_paged_attention_dev(attn, b.c, b.s, stream.ptr) == gpu.ENOSCRATCH
     assert lib.tqhip_lora_add_dev(lora, stream.ptr) == gpu.ENOSCRATCH
+
+
+@pytest.mark.parametrize("T", [1, 37])
+def test_qk_norm_rope_in_an_op_list(gpu, T):
+    """Finishing heads out of place as an op, eager and replayed from a graph with other positions: the direct call's bits."""
+    rng = np.random.default_rng(80 + T)
+    Hq, Hk, D = 5, 2, 64
+    s = head_inputs(gpu, rng, T, Hq, Hk, D, F32, True, True)
+    pos = ints(gpu, np.arange(T) + 11)
+    outs = [[Dev(gpu, np.zeros((T, h, D)), F32) for h in (Hq, Hk)] for _ in range(2)]
+    projs = [proj_of(gpu, s, T, Hq, Hk, D, F32, D, q, k, pos) for q, k in outs]
+    stream = gpu.Stream()
+    graph = gpu.OpsGraph([gpu.batch_op(gpu.OP_QK_NORM_ROPE, projs[1])], stream)
+    for first in (11, 40000, 0):
+        pos.upload(np.int32(np.arange(T) + first))
+        gpu.qk_norm_rope_dev(projs[0], stream)
+        graph.launch()
+        stream.synchronize()
+        for a, b in zip(*outs):
+            assert np.array_equal(a.read_bits(), b.read_bits()), first
+        want, size = ref.finish_heads(s["q"][2], s["q_bias"][0], s["q_norm"][0], np.arange(T) + first, D, 1e-6, 1e6)
+        check_heads(outs[1][0].read(), want, size, F32, f"q from position {first}")
+    graph.close()
