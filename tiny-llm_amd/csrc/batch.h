@@ -61,7 +61,7 @@ __device__ inline bool find_token(const int *start, const int *len, int n, int t
     if (c == 0) return false;
     b = lo + c - 1;
     const int e = __builtin_amdgcn_readlane(end, c - 1);
-    pos = __builtin_amdgcn_readlane(kv, c - 1) - (e - t);
+    pos = max(__builtin_amdgcn_readlane(kv, c - 1), 0) - (e - t);
     return t < e;
 }
 

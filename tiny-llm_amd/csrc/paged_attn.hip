@@ -205,13 +205,15 @@ struct TileRows : Run {
 template <int BM>
 __device__ inline bool find_tile(const AttnArgs &a, int tile, TileRows &t) {
     if (!find_run<BM>(a.q_start, a.n_seqs, a.n_tokens, a.group, tile, t)) return false;
-    t.pos0 = a.kv_len[t.b] - t.n;
-    t.len = min(a.kv_len[t.b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
+    const int kv = max(a.kv_len[t.b], 0);
+    t.pos0 = kv - t.n;
+    t.len = min(kv, a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
     return true;
 }
 
-// Keys [lo, hi) of the row's token at position p.
-__device__ inline int key_lo(const AttnArgs &a, int p) { return a.causal && a.window > 0 ? max(0, p + 1 - a.window) : 0; }
+// Keys [lo, hi) of the row's token at position p (p < 0 where a sequence has more new tokens than positions: a window of up to
+// INT_MAX is taken from 0 then, so that the difference fits).
+__device__ inline int key_lo(const AttnArgs &a, int p) { return a.causal && a.window > 0 ? max(0, max(p + 1, 0) - a.window) : 0; }
 __device__ inline int key_hi(const AttnArgs &a, int p, int len) { return a.causal ? min(p + 1, len) : len; }
 
 // A row's query as the operand of the score products: N chunks of 8 elements, STEP apart, in each of the lanes that hold the
@@ -847,7 +849,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts;
     int b, pos;
     if (!find_token(a.q_start, a.kv_len, a.n_seqs, token, b, pos)) return;
-    const int len = min(a.kv_len[b], a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
+    const int len = min(max(a.kv_len[b], 0), a.pages.table_stride * static_cast<int>(a.pages.page_size.d));
     const int lo = key_lo(a, pos), hi = key_hi(a, pos, len);
     const int z0 = min(lo / a.span, a.parts - 1), z1 = hi > lo ? min((hi - 1) / a.span + 1, a.parts) : z0;
     float acc[V] = {}, l = 0.0f, bias = INFINITY;  // of the parts so far: their least bias
