@@ -216,6 +216,10 @@ __device__ inline bool find_tile(const AttnArgs &a, int tile, TileRows &t) {
 __device__ inline int key_lo(const AttnArgs &a, int p) { return a.causal && a.window > 0 ? max(0, max(p + 1, 0) - a.window) : 0; }
 __device__ inline int key_hi(const AttnArgs &a, int p, int len) { return a.causal ? min(p + 1, len) : len; }
 
+// The factor that takes a score to a power of two's exponent is at least this: a masked score is minus infinity, and 0 times that is
+// no number. (What it adds to an exponent is nothing for scores below 1e30.)
+constexpr float kLeastScale = 1e-37f;
+
 // A row's query as the operand of the score products: N chunks of 8 elements, STEP apart, in each of the lanes that hold the
 // row (wide(x): the largest x over them). Returns the factor that takes a product to a power of two's exponent. fp32 rows
 // against fp16 keys are scaled into fp16's range by a power of two, which that factor takes back.
@@ -241,7 +245,7 @@ __device__ inline float load_query(const AttnArgs &a, const T *qp, vec<E, 8> (*q
             }
             mx = wide(mx);
             if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
-            c = ldexpf(c, ex);
+            c = fmaxf(ldexpf(c, ex), kLeastScale);
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -1001,7 +1005,7 @@ int run_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &b, 
     if (ws && p.workspace_bytes < bytes) return kNoScratch;
     if (bytes && !ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
     const int64_t row = static_cast<int64_t>(p.n_heads) * c.head_dim;
-    const float c2 = std::max(std::fabs(p.scale) * 1.4426950408889634f, 1e-37f);  // (> 0: 0 times an infinite score is no number)
+    const float c2 = std::max(std::fabs(p.scale) * 1.4426950408889634f, kLeastScale);
     const int64_t parts = static_cast<int64_t>(b.n_tokens) * p.n_heads * n.parts;
     float *po = static_cast<float *>(ws);
     const AttnArgs a{p.q, c.k, c.v, p.out, p.q_stride ? p.q_stride : row, p.out_stride ? p.out_stride : row, b.q_start,
