@@ -251,7 +251,10 @@ int tqhip_kv_append_dev(const tqhip_head_proj *proj, const tqhip_kv_cache *cache
  * token that may attend to nothing gets zeros. head_dim 64, 128 or 256; f16 / bf16 activations
  * take a cache of their own type, f32 activations any; q, out and the cache 16-byte aligned,
  * their strides multiples of 16 bytes. The keys and values of positions that are masked are
- * never used, whatever they hold (NaN and infinities too).
+ * never used, whatever they hold (NaN and infinities too). Infinities and NaN among those attended
+ * to go through the formula: a score of minus infinity is a weight of 0, and a key of weight 0 does
+ * not count whatever its value (where all are, the row gets zeros); a score of NaN or plus infinity makes
+ * the row NaN; an infinite value reaches its own dimension. Such rows take longer.
  *
  * workspace: NULL takes the stream's scratch (grown on demand like that of the other calls); a
  * caller that captures the call itself gives device memory of tqhip_paged_attention_workspace()

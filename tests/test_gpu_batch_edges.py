@@ -1,12 +1,15 @@
 """The batch calls on the GPU at the ends of their ranges. Tolerances as in test_gpu_batch.py."""
+import numpy as np
 import pytest
 
+import batch_ref as ref
 import test_gpu_batch as base
-from batch_ref import Batch
+from batch_ref import HALF, Batch, Dev
 
 pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = 0, 1, 2
+U = 2.0 ** -24
 
 # Sequences (new tokens, cached positions), query heads, key/value heads: 16 rows a tile and 128, in one part and in several.
 FEW_ONE = ([3, 9], [9, 100], 2, 1)
@@ -30,3 +33,98 @@ def test_scale_of_zero_and_tiny_queries(gpu, new, kv, Hq, Hk, scale, q_std):
     """Every weight is the same, whatever the size of the queries: rows are the mean of the values that they see."""
     b = Batch(gpu, new, kv, 16, Hk, 64, F16, seed=3)
     base.check_attention(gpu, b, F32, Hq, 1, 0, scale=scale, q_std=q_std)
+
+
+def seen(b, t_pos, g):
+    """Keys and values of head g at the positions that a causal row at position t_pos of sequence b sees."""
+    batch, seq, pos = b, *t_pos
+    places = [batch.place(seq, p) for p in range(0, min(batch.kv[seq], pos + 1))]
+    pg, r = np.array([p for p in places if p]).T
+    return batch.rows(batch.k.values)[pg, r, g], batch.rows(batch.v.values)[pg, r, g]
+
+
+def attend(gpu, b, act, Hq, scale, q):
+    out = Dev(gpu, np.full(q.shape, 7.0), act)
+    gpu.paged_attention_dev(gpu.Attn(dtype=act, n_heads=Hq, q=q.ptr, out=out.ptr, scale=scale, causal=1), b.c, b.s)
+    gpu.synchronize()
+    return out.read()
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("act,cache", base.TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinities_that_are_attended_to(gpu, new, kv, Hq, Hk, act, cache, D):
+    """As the formula has it, wherever tiles and parts end. A key of minus infinity in a dimension: weight 0 where the query is
+    positive there (the value does not count, infinite or not), no number where it is negative. An infinite value: an
+    infinity of its sign in its dimension, no number beside one of the other sign, and the other dimensions as ever."""
+    b = Batch(gpu, new, kv, 16, Hk, D, cache, seed=5)
+    k, v = b.k.values, b.v.values
+    for s, n in enumerate(b.kv):
+        for p, key, values in ((0, True, {1: np.inf}), (n // 2, False, {2: np.inf, 3: -np.inf}), (n // 3, False, {3: np.inf}), (n - 3, True, {}), (n - 2, False, {4: -np.inf})):
+            pg, r = b.place(s, p)
+            if key:
+                k[pg, r, :, 0] = -np.inf
+            for d, x in values.items():
+                v[pg, r, :, d] = x
+    b.k.buf.upload(ref.raw(k, cache)[0])
+    b.v.buf.upload(ref.raw(v, cache)[0])
+    q = Dev(gpu, 1.5 * b.rng.standard_normal((b.tokens, Hq, D)), act)
+    got = attend(gpu, b, act, Hq, D ** -0.5, q)
+    G, kinds = Hq // Hk, set()
+    err = size = 0.0
+    for t, at in b.token_positions().items():
+        for h in range(Hq):
+            kk, vv = seen(b, at, h // G)
+            with np.errstate(invalid="ignore"):
+                s = kk @ q.values[t, h] * float(np.float32(D ** -0.5))
+            if not np.all(s < np.inf):
+                assert np.isnan(got[t, h]).all(), (t, h, at)
+                kinds.add("nan")
+                continue
+            live = s > -np.inf
+            if not live.any():
+                assert np.all(got[t, h] == 0), (t, h, at)
+                continue
+            s, vv = s[live], vv[live]
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            with np.errstate(invalid="ignore"):
+                want = p @ vv
+            finite = np.isfinite(want)
+            assert np.array_equal(np.isnan(got[t, h]), np.isnan(want)) and np.array_equal(got[t, h][np.isinf(want)], want[np.isinf(want)]), (t, h, at, got[t, h, :6], want[:6])
+            kinds.update("+" if x > 0 else "-" for x in want[np.isinf(want)])
+            spread = p @ np.abs(np.where(np.isfinite(vv), vv, 0))
+            fin = np.where(np.isfinite(kk[live]), kk[live], 0)
+            score = (np.abs(fin) @ np.abs(q.values[t, h])).max() * D ** -0.5
+            bound = (2 * (D + 4) * score + 2 * len(s) + 32) * U * spread
+            if act != F32:
+                bound = bound + HALF[act] * (spread + np.abs(np.where(finite, want, 0))) + 2.0 ** -25
+            assert np.all(np.abs(got[t, h] - want)[finite] <= bound[finite]), (t, h, at)
+            err, size = err + np.sum((got[t, h] - want)[finite] ** 2), size + np.sum(want[finite] ** 2)
+    assert kinds == {"nan", "+", "-"}
+    if act == F32:
+        assert np.sqrt(err) <= 2.0 ** -17 * np.sqrt(size)
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("act,cache", base.TYPES)
+def test_queries_that_are_not_finite(gpu, new, kv, Hq, Hk, act, cache):
+    """A NaN or infinite query makes its own rows NaN where keys of either sign are seen, and no others: those stay within the bound that
+    every row has. (Not the same bits: rows of one wave bring their sums down to a new maximum together, so when one does,
+    all have another rounding of a factor and its products, which the N + 16 u of the sums count.)"""
+    D = 64
+    b = Batch(gpu, new, kv, 16, Hk, D, cache, seed=6)
+    x = Dev(gpu, 1.5 * b.rng.standard_normal((b.tokens, Hq, D)), act).values
+    want, spread, score, _ = ref.attention(b, x, 0.125, 1, 0)
+    bound = (2 * (D + 4) * score + 2 * max(kv) + 32) * U * spread
+    if act != F32:
+        bound = bound + HALF[act] * (spread + np.abs(want)) + 2.0 ** -25
+    last = b.tokens - 1
+    odd = (last, 0), (last - 1, 1), (last - 2, 0)
+    for (t, h), d, y in zip(odd, (7, 0, 63), (np.nan, np.inf, -np.inf)):
+        x[t, h, d] = y
+    got = attend(gpu, b, act, Hq, 0.125, Dev(gpu, x, act))
+    for t, h in odd:
+        assert np.isnan(got[t, h]).all(), (t, h)
+        got[t, h] = want[t, h]
+    assert np.all(np.abs(got - want) <= bound)

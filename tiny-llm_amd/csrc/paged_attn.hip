@@ -22,6 +22,7 @@
 //   three prompts of up to 5001 fp32 tokens, a window of 1000 bf16 keys, 14 heads on 2 of 64: 130 us (33.5 GFLOP of three terms each)
 //   one fp32 token of 14 heads on 2 of 64 over 3000 fp32 keys:                        9.4 us and 4.0 for the join
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -262,6 +263,84 @@ __device__ inline float load_query(const AttnArgs &a, const T *qp, vec<E, 8> (*q
     return c;
 }
 
+// ---- a row by the formula ------------------------------------------------------------------------
+
+// One row's keys [k0, k1) by one wave, in 64 bits, a key a lane for the scores and dimensions a lane for the values. The tiles take
+// numbers: in their terms an infinity is itself, then a zero or an infinity of the other sign, and a weight that rounds to zero
+// makes no number of an infinite value. So a row whose result there is not finite is done again here (nothing is
+// added to the tiles' loops for it), and what a row gives does not depend on where tiles and parts end: a key of weight zero (a
+// score of minus infinity) does not count whatever its value, a score of plus infinity or NaN makes the row NaN, an infinite value
+// its dimension's sum. A row of NaN ends at its first 64 keys. Writes the row's output, or its part's sums.
+template <typename T, typename C, int D>
+__device__ inline void formula_row(const AttnArgs &a, int b, int row, int token0, int kvh, int k0, int k1) {
+    constexpr int V = D / 64;
+    const int lane = threadIdx.x & 63, token = token0 + row / a.group, head = kvh * a.group + row % a.group;
+    const T *q = static_cast<const T *>(a.q) + token * a.q_stride + head * D;
+    const C *kc = static_cast<const C *>(a.k) + kvh * a.pages.head_stride;
+    const C *vc = static_cast<const C *>(a.v) + kvh * a.pages.head_stride + lane * V;
+    const double c = static_cast<double>(a.scale) * a.sign;
+    const auto offset = [&](int key) { return key < k1 ? row_offset(a.pages, b, key) : int64_t{-1}; };
+    const auto score = [&](int64_t o) {
+        double s = 0.0;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 8) {  // (unrolled, it would take more registers than the tiles)
+            float x[8], y[8];
+            load_as_float<T, 8>(q + d, x);
+            load_as_float<C, 8>(kc + max(o, int64_t{0}) + d, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += static_cast<double>(x[e]) * y[e];
+        }
+        return o < 0 ? static_cast<double>(-INFINITY) : s * c;
+    };
+    double m = -INFINITY;
+    bool number = true;
+    for (int k = k0; k < k1 && number; k += 64) {
+        const double s = score(offset(k + lane));
+        number = __ballot(!(s < INFINITY)) == 0;
+        m = fmax(m, s);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) m = fmax(m, __shfl_xor(m, d));
+    double l = 0.0, acc[V] = {};
+    for (int k = k0; k < k1 && number && m > -INFINITY; k += 64) {
+        const int64_t o = offset(k + lane);
+        const float w = exp2f(static_cast<float>(score(o) - m));
+        l += w;
+        for (int j = 0; j < min(64, k1 - k); ++j) {
+            const float wj = __shfl(w, j);
+            if (wj == 0.0f) continue;
+            float x[V];
+            load_as_float<C, V>(vc + __shfl(static_cast<long long>(o), j), x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += static_cast<double>(wj) * x[i];
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
+    if (!number) l = NAN;
+    float o[V];
+    if (a.parts > 1) {
+        const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts + blockIdx.y;
+        // (weights are 2^(score + bias); a bias that fp32 rounds is off by as much as fp32 scores of that size are)
+        if (lane == 0) a.part_ml[at] = make_float2(l > 0.0 ? static_cast<float>(fmin(fmax(-m, -FLT_MAX), FLT_MAX)) : 0.0f, static_cast<float>(l));
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = static_cast<float>(acc[i]);
+        store_rounded<float, V>(a.part_o + at * D + lane * V, o);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = l == 0.0 ? 0.0f : static_cast<float>(acc[i] / l);
+        store_rounded<T, V>(static_cast<T *>(a.out) + token * a.out_stride + head * D + lane * V, o);
+    }
+}
+
+// 0 where all numbers are finite, NaN where one is not.
+template <int N>
+__device__ inline float not_finite(const vec<float, N> &x, float z) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z = fmaf(x[i], 0.0f, z);
+    return z;
+}
+
 // ---- few rows: tiles of 16 rows ------------------------------------------------------------------
 
 // A tile's keys are dealt to the four waves 32 at a time; each wave keeps a softmax of its own, and the four meet at the end, so no
@@ -379,7 +458,6 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
         const unsigned exist = static_cast<unsigned>(__ballot(off[0] >= 0) & 0xffff) |
                                static_cast<unsigned>(__ballot(off[1] >= 0) & 0xffff) << 16;
         const bool partial = k0 < full_lo || k0 + kFewKeys > full_hi || exist != ~0u;
-        const int64_t was[2] = {off[0], off[1]};
         wait_loads();
         offsets(k0 + kFewStep, next, off);
         pages_of(k0 + 2 * kFewStep, next);
@@ -486,17 +564,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
             }
             if constexpr (!kDirect) wave_lds_order();
         }
-        for (; wild; wild &= wild - 1) {
-            const int j = __builtin_ctz(wild), key = k0 + j;
-            const int64_t o = __shfl(static_cast<long long>(j < 16 ? was[0] : was[1]), j & 15);
-            if (key < lo || key >= hi || o < 0) continue;
-            const C *v0 = vc + o - 8 * g + 4 * g;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (!is_finite<C>(v0[16 * d + e])) acc[d][e] += static_cast<float>(v0[16 * d + e]);
-        }
+        if (wild & exist & below(hi - k0) & ~below(lo - k0)) l = NAN;  // (formula_row takes the row)
         k0 += kFewStep;
     };
     E *v0 = &sh.v[wave][0][0][0], *v1 = &sh.v[wave][kDirect ? 1 : 0][0][0];
@@ -531,26 +599,39 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     __syncthreads();
     // thread: row tid / 16, every 16th group of four dimensions
     const int row = tid >> 4;
-    if (t.r0 + row >= rows) return;
     const int r2 = t.r0 + row, token2 = t.first + r2 / a.group, head2 = kvh * a.group + r2 % a.group;
     const float total2 = __shfl(total, row), least2 = __shfl(least, row);
-    const int64_t at = (static_cast<int64_t>(token2) * a.n_heads + head2) * a.parts + blockIdx.y;
-    if (a.parts > 1 && (tid & 15) == 0) a.part_ml[at] = make_float2(least2, total2);
-    const float inv = total2 == 0.0f ? 0.0f : 1.0f / total2;
+    f32x4 o[D / 64];
+    float z = total2 * 0.0f;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         const int d = 4 * (tid & 15) + 64 * i;
-        f32x4 o = *reinterpret_cast<f32x4 *>(&sh.o[0][row][d]);
+        o[i] = *reinterpret_cast<f32x4 *>(&sh.o[0][row][d]);
 #pragma unroll
-        for (int w = 1; w < 4; ++w) o += *reinterpret_cast<f32x4 *>(&sh.o[w][row][d]);
-        if (a.parts > 1) {
-            *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) = o;
-        } else {
-            o *= inv;
-            float x[4] = {o[0], o[1], o[2], o[3]};
-            store_rounded<T, 4>(static_cast<T *>(a.out) + token2 * a.out_stride + head2 * D + d, x);
+        for (int w = 1; w < 4; ++w) o[i] += *reinterpret_cast<f32x4 *>(&sh.o[w][row][d]);
+        z = not_finite<4>(o[i], z);
+    }
+    const unsigned long long odd = __ballot(r2 < rows && z != 0.0f);  // 16 lanes a row
+    if (r2 < rows && !(odd >> (lane & 48) & 0xffff)) {
+        const int64_t at = (static_cast<int64_t>(token2) * a.n_heads + head2) * a.parts + blockIdx.y;
+        if (a.parts > 1 && (tid & 15) == 0) a.part_ml[at] = make_float2(least2, total2);
+        const float inv = total2 == 0.0f ? 0.0f : 1.0f / total2;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            const int d = 4 * (tid & 15) + 64 * i;
+            if (a.parts > 1) {
+                *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) = o[i];
+            } else {
+                float x[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
+                store_rounded<T, 4>(static_cast<T *>(a.out) + token2 * a.out_stride + head2 * D + d, x);
+            }
         }
     }
+    for (int i = 0; odd && i < 4; ++i)
+        if (odd >> (16 * i) & 0xffff) {
+            const int ro = t.r0 + 4 * wave + i, p = t.pos0 + ro / a.group;
+            formula_row<T, C, D>(a, t.b, ro, t.first, kvh, max(kb, key_lo(a, p)), min(ke, key_hi(a, p, t.len)));
+        }
 }
 
 // ---- many rows: tiles of 128 rows ---------------------------------------------------------------
@@ -749,17 +830,9 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
             }
             s = ahead;
         }
-        for (unsigned long long w = partial ? sh.wild[buf] : 0; w; w &= w - 1) {
-            const int j = __builtin_ctzll(w), key = k0 + j;
-            if (key < lo || key >= hi || !(exist >> j & 1)) continue;
-            const C *v0 = vc + sh.offs[n / kTiles & 1][n % kTiles * BN + j] + 4 * h;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const C x = v0[32 * d + (e & 3) + 8 * (e >> 2)];
-                    if (!is_finite<C>(x)) acc[d][e] += static_cast<float>(x);
-                }
+        for (unsigned long long w = partial ? sh.wild[buf] & exist : 0; w; w &= w - 1) {
+            const int key = k0 + __builtin_ctzll(w);
+            if (key >= lo && key < hi) l = NAN;  // (formula_row takes the row)
         }
     };
     for (int n = 0, k0 = kb; k0 < ke; k0 += BN, ++n) {
@@ -767,7 +840,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
         const unsigned long long all = BN == 64 ? ~0ull : 0xffffffffull;
         const unsigned long long exist = scalar(sh.here[n / kTiles & 1][n % kTiles * BN / 64]) >> (BN == 64 ? 0 : n % 2 * 32) & all;
         // An infinite or NaN value would reach rows that mask its key through a product with their weight of zero: where some
-        // row of the block masks some key, it goes into the products as zero and is added below where its key is seen.
+        // row of the block masks some key, it goes into the products as zero, and the rows that see its key are done again.
         const bool partial = k0 < full_lo || k0 + BN > full_hi || exist != all;
         if (n % kTiles == kTiles - 1) {
             put_offsets(n / kTiles + 1, next_page);
@@ -809,31 +882,41 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
         }
         step(n, k0, partial, exist, &sh.v[kDirect ? buf : 0][0][0], &sh.k[kDirect ? buf ^ 1 : 0][0][0], &sh.v[kDirect ? buf ^ 1 : 0][0][0]);
     }
-    if (wr0 + col >= rows) return;
     l += lane_xor<32>(l, lane);
-    if (a.parts > 1) {
-        const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts + blockIdx.y;
-        if (h == 0) a.part_ml[at] = make_float2(bias, l);
-        float *o = a.part_o + at * D;
+    float z = l * 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d) z = not_finite<16>(acc[d], z);
+    unsigned long long odd = __ballot(wr0 + col < rows && z != 0.0f);
+    odd = (odd | odd >> 32) & 0xffffffffu;  // rows of the wave
+    if (wr0 + col < rows && !(odd >> col & 1)) {
+        if (a.parts > 1) {
+            const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts + blockIdx.y;
+            if (h == 0) a.part_ml[at] = make_float2(bias, l);
+            float *o = a.part_o + at * D;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4 *>(o + 32 * d + 8 * g + 4 * h) =
-                    make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T *o = static_cast<T *>(a.out) + token * a.out_stride + head * D;
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<float4 *>(o + 32 * d + 8 * g + 4 * h) =
+                        make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T *o = static_cast<T *>(a.out) + token * a.out_stride + head * D;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float x[4];
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[d][4 * g + e] * inv;
-            store_rounded<T, 4>(o + 32 * d + 8 * g + 4 * h, x);
+                for (int g = 0; g < 4; ++g) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = acc[d][4 * g + e] * inv;
+                    store_rounded<T, 4>(o + 32 * d + 8 * g + 4 * h, x);
+                }
         }
+    }
+    for (; odd; odd &= odd - 1) {
+        const int ro = wr0 + __builtin_ctzll(odd), p = t.pos0 + ro / a.group;
+        formula_row<T, C, D>(a, t.b, ro, t.first, kvh, max(kb, key_lo(a, p)), min(ke, key_hi(a, p, t.len)));
+    }
 }
 
 // ---- the join of the parts ----------------------------------------------------------------------
