@@ -128,3 +128,43 @@ def test_queries_that_are_not_finite(gpu, new, kv, Hq, Hk, act, cache):
         assert np.isnan(got[t, h]).all(), (t, h)
         got[t, h] = want[t, h]
     assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("act,cache,q_std,scale", [(F32, F16, 1e6, 1.0), (F32, F16, 1e9, 1.0), (F32, F16, 3.0, 1e13), (F32, BF16, 1e9, -1.0), (F32, F32, 1e15, 1.0),
+                                                   (F16, F16, 1e4, 1e2), (F16, F16, 1e4, 1e4), (BF16, BF16, 1e6, 1e4)])
+def test_scores_of_millions_and_beyond(gpu, new, kv, Hq, Hk, act, cache, q_std, scale):
+    """Scores whose exponents do not fit between two neighbouring fp32 numbers of their size. Keys repeat every 32 positions, so a row
+    is the mean of the values at its best key's repetitions, which lie in every tile and part, unless rounding can
+    decide between the two best keys (a row's scores are off by at most 2 (D + 4) u of their terms' sizes); such a row lies within its values."""
+    D = 64
+    b = Batch(gpu, new, kv, 16, Hk, D, cache, seed=int(q_std) % 97)
+    keys = ref.raw(b.rng.standard_normal((32, Hk, D)), cache)[1]
+    full = b.k.values
+    for s, n in enumerate(b.kv):
+        for p in range(n):
+            pg, r = b.place(s, p)
+            full[pg, r] = keys[p % 32]
+    b.k.buf.upload(ref.raw(full, cache)[0])
+    q = Dev(gpu, q_std * b.rng.standard_normal((b.tokens, Hq, D)), act)
+    got = attend(gpu, b, act, Hq, scale, q)
+    G, decided = Hq // Hk, 0
+    scale = float(np.float32(scale))
+    for t, at in b.token_positions().items():
+        for h in range(Hq):
+            kk, vv = seen(b, at, h // G)
+            s = kk @ q.values[t, h] * scale
+            top = s.max()
+            best = s >= top - 1e-9 * abs(top)
+            off = 2 * (D + 4) * U * (np.abs(kk) @ np.abs(q.values[t, h])).max() * abs(scale)
+            if best.all() or top - s[~best].max() > 2 * off + 100:
+                decided += 1
+                want, spread = vv[best].mean(0), np.abs(vv[best]).mean(0)
+                bound = (2 * len(vv) + 32) * U * spread
+                if act != F32:
+                    bound = bound + HALF[act] * (spread + np.abs(want)) + 2.0 ** -25
+                assert np.all(np.abs(got[t, h] - want) <= bound), (t, h, at)
+            else:
+                slack = 1e-5 + (0 if act == F32 else 4 * HALF[act]) * np.abs(vv).max()
+                assert np.all((got[t, h] >= vv.min(0) - slack) & (got[t, h] <= vv.max(0) + slack)), (t, h, at)
+    assert decided > 0.5 * b.tokens * Hq
