@@ -280,6 +280,7 @@ size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_ca
  * Tokens whose adapter is outside [0, n_adapters) (-1: none) get base_t; tokens of no sequence
  * keep their y. x is [n_tokens][in_dim] and base / y [n_tokens][out_dim], as matmul_i4 reads and
  * writes them; base may be y, or NULL for zeros. An adapter of a lower rank has zero rows.
+ * Infinities and NaN go through as the formula has them (such outputs take longer).
  * rank 1 to 256. workspace: as for the attention, tqhip_lora_workspace() bytes. */
 typedef struct tqhip_lora {
     int dtype;                       /* of a and b: TQHIP_F32 / F16 / BF16 */

@@ -4,7 +4,7 @@ import pytest
 
 import batch_ref as ref
 import test_gpu_batch as base
-from batch_ref import HALF, Batch, Dev
+from batch_ref import HALF, Batch, Dev, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,43 @@ def test_scores_of_millions_and_beyond(gpu, new, kv, Hq, Hk, act, cache, q_std, 
                 slack = 1e-5 + (0 if act == F32 else 4 * HALF[act]) * np.abs(vv).max()
                 assert np.all((got[t, h] >= vv.min(0) - slack) & (got[t, h] <= vv.max(0) + slack)), (t, h, at)
     assert decided > 0.5 * b.tokens * Hq
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,K,M,r", [([1] * 5, 96, 70, 1), ([1] * 5, 100, 33, 8), ([40, 30], 256, 300, 16), ([40, 30], 67, 35, 5), ([40], 2000, 130, 200)])
+def test_lora_of_infinities(gpu, dtype, new, K, M, r):
+    """Infinite activations and adapter weights go through as the formula has them: infinities of the sum's sign, no number where both
+    signs meet; every other token and output is as ever."""
+    rng = np.random.default_rng(K + r)
+    starts = np.concatenate(([0], np.cumsum(new)))
+    T = int(starts[-1])
+    x, y0 = rng.standard_normal((T, K)).astype(np.float32), rng.standard_normal((T, M)).astype(np.float32)
+    a, b = rng.standard_normal((2, r, K)) / np.sqrt(K), 0.3 * rng.standard_normal((2, M, r))
+    b[:, : M // 2] = np.abs(b[:, : M // 2]) * np.sign(a[:, None, :, K - 1])  # (half of the outputs: terms of one sign)
+    a, b = Dev(gpu, a, dtype), Dev(gpu, b, dtype)
+    x[1, K - 1], x[3, K - 1] = np.inf, -np.inf
+    y0[2, 3] = np.inf
+    b.values[1, M - 1, 0] = -np.inf
+    b.buf.upload(ref.raw(b.values, dtype)[0])
+    of = [i % 2 for i in range(len(new))]
+    scale = np.float32([1.5, 0.5])
+    dx, dy0, ds, dst, dad = base.f32_buffer(gpu, x), base.f32_buffer(gpu, y0), base.f32_buffer(gpu, scale), ints(gpu, starts), ints(gpu, of)
+    dy = base.f32_buffer(gpu, np.full((T, M), 7.0))
+    gpu.lora_add_dev(gpu.Lora(dtype=dtype, n_tokens=T, in_dim=K, out_dim=M, rank=r, n_adapters=2, n_seqs=len(new), x=dx.ptr, base=dy0.ptr, y=dy.ptr,
+                              a=a.ptr, b=b.ptr, scale=ds.ptr, q_start=dst.ptr, adapter=dad.ptr))
+    gpu.synchronize()
+    got = dy.download(np.float32, T * M).reshape(T, M).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want, size = ref.lora(x.astype(np.float64), y0.astype(np.float64), a.values, b.values, scale.astype(np.float64), starts, of, T)
+    finite = np.isfinite(want)
+    assert np.isinf(want[1, : M // 2]).all() and (r == 1 or np.isnan(want).any()) and np.isinf(want[2, 3])
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    assert np.all(np.abs(got - want)[finite] <= (K + r + 8) * U * size[finite])
+    # in place: the same bits
+    bits = dy.download(np.int32, T * M)
+    gpu.lora_add_dev(gpu.Lora(dtype=dtype, n_tokens=T, in_dim=K, out_dim=M, rank=r, n_adapters=2, n_seqs=len(new), x=dx.ptr, base=dy0.ptr, y=dy0.ptr,
+                              a=a.ptr, b=b.ptr, scale=ds.ptr, q_start=dst.ptr, adapter=dad.ptr))
+    gpu.synchronize()
+    same = (dy0.download(np.int32, T * M) == bits) | np.isnan(got.ravel())
+    assert same.all()

@@ -6,6 +6,8 @@
 // Both are products on the matrix cores in bf16 terms: an fp32 operand (x, u, fp32 weights) is three
 // of them (24 bits), an fp16 weight two (all 11 bits, and fp16's range), a bf16 weight one; products below 2^-24 are
 // left out. So fp32 results keep fp32's precision at 3 to 6 matrix instructions a product, where the fp32 ones take 16.
+// An infinity is its first term, and no number beside the zero or the other sign of the other operand's next one: results that
+// are not finite are formed again by the formula, in 64 bits, by the threads that have them. The loops carry nothing for it.
 //
 // Both launches are bound by HBM (x once; base and y once; A and B stay in L2) or, with few tokens, by latency. 3555 tokens of 8
 // requests, rank 64 in bf16 beside 9728x2560: 26 and 73 us for 38 and 287 MB. 64 requests of a token, rank 16 in fp16 beside
@@ -157,6 +159,16 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NR>) void lora_shrink(LoraArgs p)
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += sum[w][row][c];
+        if (v * 0.0f != 0.0f) {  // infinite or NaN: by the formula, over what the workgroup's waves had
+            const int64_t k0 = 32 * (static_cast<int64_t>(steps) * blockIdx.y * NW / workers);
+            const int64_t k1 = min(32 * (static_cast<int64_t>(steps) * (blockIdx.y + 1) * NW / workers), static_cast<int64_t>(p.K));
+            const float *xr = p.x + static_cast<int64_t>(t.first + t.r0 + row) * p.K;
+            const W *ar = a + static_cast<int64_t>(c) * p.K;
+            double w = 0.0;
+#pragma unroll 1
+            for (int64_t k = k0; k < k1 && w == w; ++k) w += static_cast<double>(xr[k]) * static_cast<float>(ar[k]);
+            v = static_cast<float>(w);
+        }
         u[i] = scale * v;
     }
 }
@@ -262,11 +274,41 @@ __global__ __launch_bounds__(256) void lora_expand(LoraArgs p) {
             }
         }
     }
+    // (a lane's outputs of a token are formed again together, and none of them is stored before: base may be y)
+    unsigned again = 0;
+#pragma unroll
+    for (int j = 0; j < TT; ++j) {
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z = fmaf(acc[i][h][j][e], 0.0f, z);
+        if (z != 0.0f && 16 * j + col < live) again |= 1u << j;
+    }
+    for (unsigned left = again; left; left &= left - 1) {
+        const int64_t token = token0 + 16 * __builtin_ctz(left) + col;
+#pragma unroll 1
+        for (int n = 0; n < 8 * S; ++n) {
+            const int m = m_first + 128 * (n >> 3) + 32 * wave + 16 * (n >> 2 & 1) + 4 * g + (n & 3);
+            if (m >= p.M) continue;
+            double v = p.base ? p.base[token * p.M + m] : 0.0f;
+#pragma unroll 1
+            for (int r = 0; r < p.rank && v == v; ++r) {
+                float u_r = 0.0f;
+#pragma unroll 1
+                for (int z = 0; z < p.splits; ++z) u_r += p.u[(static_cast<int64_t>(z) * p.n_tokens + token) * p.rank + r];
+                v += static_cast<double>(u_r) * static_cast<float>(b[static_cast<int64_t>(m) * p.rank + r]);
+            }
+            p.y[token * p.M + m] = static_cast<float>(v);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            if (16 * j + col >= live) continue;
+            if (16 * j + col >= live || again >> j & 1) continue;
             float *dst = p.y + (token0 + 16 * j + col) * p.M;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
