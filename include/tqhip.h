@@ -177,6 +177,8 @@ int tqhip_matvec_i4_generic_dev(const uint8_t *w, const float *x, float *y, int 
  * calls serve many requests at once, each with its own number of new tokens, on device
  * buffers like the _dev calls above: asynchronous on `stream`, status codes, no aborts. The
  * stream has to be one of the current device. The structs are read during the call.
+ * Host threads may call on one stream at the same time: a call enqueues all of its launches before
+ * another call that takes the stream's scratch does (a workspace of the caller's is the caller's to guard).
  *
  * Types: activations f32 (what the projections above read and write), or f16 / bf16; the
  * cache f32 / f16 / bf16. Arithmetic, norms and softmax statistics are in fp32, angles in

@@ -1138,6 +1138,7 @@ int launch_i4_matmul(const uint8_t *w, const float *x, float *y, int M, int K, i
                      hipStream_t stream) {
     if (M < 1 || K < 1 || N < 1 || group_size < 2 || (group_size & 1)) return kBadShape;
     if (!w || !x || !y) return kBadShape;  // nothing is launched on a null operand
+    ScratchCall call(stream);
     if (skinny_applies(x, K, N, group_size)) {
         const SkinnyGeom g = skinny_geom(M, K, device_cu_count());
         unsigned long long *slots = nullptr;  // zero between launches: the arrival counters

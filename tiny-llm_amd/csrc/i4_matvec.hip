@@ -1403,6 +1403,7 @@ int launch_split(const uint8_t *w, const float *x, float *y, Geom gm, int S, int
     const size_t lds = gm.tbuf + static_cast<size_t>(kTile * NWP) * 4 + 3 * kp + kp / 8 * 4 + ng * 4 + 16;
     if (lds > kLdsBytes) return kTooLarge;
     if (S < 2 || S > 4) return kTooLarge;  // the exchange tree has two levels
+    ScratchCall call(stream);
     unsigned long long *slots = nullptr;
     const int st = scratch_split_slots(stream, static_cast<size_t>(tiles) * 3 * kTile, &slots);
     if (st != kOk) return st;

@@ -13,6 +13,7 @@
 // requests, rank 64 in bf16 beside 9728x2560: 26 and 73 us for 38 and 287 MB. 64 requests of a token, rank 16 in fp16 beside
 // 4096x2560: 5.7 and 7 us.
 #include <algorithm>
+#include <optional>
 #include <type_traits>
 
 #include "batch.h"
@@ -424,7 +425,11 @@ int run_lora(const tqhip_lora &l, hipStream_t s) {
     void *ws = l.workspace;
     if (reinterpret_cast<uintptr_t>(ws) % 256) return kBadShape;
     if (ws && l.workspace_bytes < bytes) return kNoScratch;
-    if (!ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
+    std::optional<ScratchCall> call;
+    if (!ws) {
+        call.emplace(s);
+        if ((st = call->workspace(bytes, &ws)) != kOk) return st;
+    }
     const LoraPlan n = lora_plan(l);
     const LoraArgs p{l.x, l.base, l.y, l.a, l.b, l.scale, l.q_start, l.adapter, static_cast<float *>(ws), l.n_tokens,
                      l.in_dim, l.out_dim, l.rank, l.n_adapters, l.n_seqs, n.splits};

@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <optional>
 #include <type_traits>
 
 #include "batch.h"
@@ -1094,7 +1095,11 @@ int run_attn(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &b, 
     void *ws = p.workspace;
     if (reinterpret_cast<uintptr_t>(ws) % 256) return kBadShape;
     if (ws && p.workspace_bytes < bytes) return kNoScratch;
-    if (bytes && !ws && (st = scratch_batch(s, bytes, &ws)) != kOk) return st;
+    std::optional<ScratchCall> call;
+    if (bytes && !ws) {
+        call.emplace(s);
+        if ((st = call->workspace(bytes, &ws)) != kOk) return st;
+    }
     const int64_t row = static_cast<int64_t>(p.n_heads) * c.head_dim;
     const float c2 = std::max(std::fabs(p.scale) * 1.4426950408889634f, kLeastScale);
     const int64_t parts = static_cast<int64_t>(b.n_tokens) * p.n_heads * n.parts;

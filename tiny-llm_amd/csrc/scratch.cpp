@@ -16,6 +16,10 @@
 //     (the caller's own hipStreamBeginCapture around a _dev call) has recorded
 //     is marked and, when the stream later needs a larger one, retired instead
 //     of freed: that graph may still be replayed.
+//   * A call takes its buffers and enqueues its launches under one lock of the set
+//     (ScratchCall): a stream orders launches, not pairs of them, so another host thread's
+//     call on the stream could otherwise write a buffer between two launches of this one,
+//     or replace it before they are made.
 //   * A fixed set (the allocation-free entry point) has preset buffers and can
 //     not grow: a request beyond them is kTooLarge, which the launchers treat as
 //     "this kernel does not fit" (split-K falls back to a non-split kernel).
@@ -45,7 +49,7 @@ struct ScratchSet {
     ~ScratchSet() { --g_live_sets; }
     ScratchSet(const ScratchSet &) = delete;
     ScratchSet &operator=(const ScratchSet &) = delete;
-    std::mutex mu;
+    std::recursive_mutex mu;  // of one request, or of a whole call (ScratchCall)
     ScratchBuf split;  // split-K exchange slots / arrival counters: zero between launches
     ScratchBuf xws;    // prefill workspace
     std::vector<void *> retired;
@@ -114,7 +118,7 @@ int grow(ScratchSet &set, ScratchBuf &b, size_t need, size_t floor_bytes, bool z
 int scratch_split_slots(hipStream_t s, size_t nslots, unsigned long long **slots) {
     ScratchSet *set = set_for(s);
     if (!set) return kHipFailed;
-    std::lock_guard<std::mutex> lock(set->mu);
+    std::lock_guard<std::recursive_mutex> lock(set->mu);
     void *p = nullptr;
     const int st = grow(*set, set->split, nslots * sizeof(unsigned long long), (size_t{1} << 14) * 8, true, s, &p);
     *slots = static_cast<unsigned long long *>(p);
@@ -124,15 +128,8 @@ int scratch_split_slots(hipStream_t s, size_t nslots, unsigned long long **slots
 int scratch_prefill(hipStream_t s, size_t bytes, void **ws) {
     ScratchSet *set = set_for(s);
     if (!set) return kHipFailed;
-    std::lock_guard<std::mutex> lock(set->mu);
+    std::lock_guard<std::recursive_mutex> lock(set->mu);
     return grow(*set, set->xws, bytes, size_t{1} << 20, false, s, ws);
-}
-
-// The prefill workspace for a call that takes the caller's own workspace too: under a capture that
-// no scope owns it is refused, because two graphs captured on one stream would share the buffer.
-int scratch_batch(hipStream_t s, size_t bytes, void **ws) {
-    if (!t_scope && capturing(s)) return kNoScratch;
-    return scratch_prefill(s, bytes, ws);
 }
 
 ScratchSet *scratch_set_new() { return new ScratchSet; }
@@ -155,6 +152,18 @@ void scratch_set_free(ScratchSet *set) {
     delete set;
 }
 
+ScratchCall::ScratchCall(hipStream_t s) : stream_(s), set_(set_for(s)) {
+    if (set_) set_->mu.lock();
+}
+ScratchCall::~ScratchCall() {
+    if (set_) set_->mu.unlock();
+}
+int ScratchCall::workspace(size_t bytes, void **ws) {
+    if (!set_) return kHipFailed;
+    if (!t_scope && capturing(stream_)) return kNoScratch;
+    return grow(*set_, set_->xws, bytes, size_t{1} << 20, false, stream_, ws);
+}
+
 ScratchScope::ScratchScope(ScratchSet *set) : prev_(t_scope) { t_scope = set; }
 ScratchScope::~ScratchScope() { t_scope = prev_; }
 
@@ -173,7 +182,7 @@ void scratch_forget_stream(hipStream_t s) {
     // so does their set. Otherwise the buffers and the set go: the stream is being destroyed,
     // so no other thread may still launch on it (the caller's contract, as for the stream).
     {
-        std::lock_guard<std::mutex> lock(set->mu);
+        std::lock_guard<std::recursive_mutex> lock(set->mu);
         if (set->split.captured || set->xws.captured || !set->retired.empty()) return;  // leaked on purpose
         if (set->split.p) (void)hipFree(set->split.p);
         if (set->xws.p) (void)hipFree(set->xws.p);
@@ -198,7 +207,7 @@ ScratchStats scratch_stats(hipStream_t s) {
         if (it == g_streams.end()) return st;
         set = it->second;
     }
-    std::lock_guard<std::mutex> lock(set->mu);
+    std::lock_guard<std::recursive_mutex> lock(set->mu);
     st.split_bytes = set->split.cap;
     st.prefill_bytes = set->xws.cap;
     st.split_captured = set->split.captured ? 1 : 0;

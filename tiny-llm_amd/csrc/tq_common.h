@@ -167,12 +167,27 @@ int device_cu_count();
 struct ScratchSet;
 int scratch_split_slots(hipStream_t s, size_t nslots, unsigned long long **slots);
 int scratch_prefill(hipStream_t s, size_t bytes, void **ws);
-int scratch_batch(hipStream_t s, size_t bytes, void **ws);  // kNoScratch under the caller's own capture
 ScratchSet *scratch_set_new();
 ScratchSet *scratch_set_fixed(void *xws, size_t xws_bytes);
 void scratch_set_free(ScratchSet *set);  // the caller has synchronised every launch that used it
 void scratch_forget_stream(hipStream_t s);  // the stream is being destroyed (synchronised)
 long scratch_live_sets();                    // ScratchSet objects alive (bookkeeping checks)
+// From before a call's first request for scratch until its last launch is enqueued: calls of other
+// host threads on the same stream wait meanwhile, so the buffers are the call's own until then.
+class ScratchCall {
+  public:
+    explicit ScratchCall(hipStream_t s);
+    ~ScratchCall();
+    ScratchCall(const ScratchCall &) = delete;
+    ScratchCall &operator=(const ScratchCall &) = delete;
+    // The prefill workspace for a call that takes the caller's own workspace too: kNoScratch under a capture
+    // that no scope owns, because two graphs captured on one stream would share the buffer.
+    int workspace(size_t bytes, void **ws);
+
+  private:
+    hipStream_t stream_;
+    ScratchSet *set_;
+};
 class ScratchScope {
   public:
     explicit ScratchScope(ScratchSet *set);
