@@ -243,7 +243,8 @@ int tqhip_qk_norm_rope_dev(const tqhip_head_proj *proj, void *stream);
 
 /* k and v into the cache rows of their tokens' positions, k finished as above; q -> q_out in the
  * same launch where both are given. The rotation takes proj->positions, or the cache positions
- * where that is NULL. k_out is not used. Two tokens of a call must not fall on one row. */
+ * where that is NULL. k_out is not used. Two tokens of a call must not fall on one row, and strides under
+ * which two rows of the cache share elements are refused (attention may read over such a cache). */
 int tqhip_kv_append_dev(const tqhip_head_proj *proj, const tqhip_kv_cache *cache, const tqhip_seqs *seqs,
                         void *stream);
 

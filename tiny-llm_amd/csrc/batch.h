@@ -4,7 +4,10 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <array>
 #include <cstdint>
+#include <utility>
 
 #include "../../include/tqhip.h"
 
@@ -129,7 +132,7 @@ __device__ inline int64_t row_in_page(const Pages &g, int page, int p) {
 }
 __device__ inline int64_t row_offset(const Pages &g, int b, int p) { return row_in_page(g, page_number(g, b, p), p); }
 
-// The cache's strides with the contiguous layout for zeros; false: not a layout in which every row is apart.
+// The cache's strides with the contiguous layout for zeros; false: less than a head's row apart.
 inline bool cache_strides(const tqhip_kv_cache &c, int64_t *page, int64_t *token, int64_t *head) {
     if (c.page_stride == 0 && c.token_stride == 0 && c.head_stride == 0) {
         *head = c.head_dim;
@@ -141,6 +144,21 @@ inline bool cache_strides(const tqhip_kv_cache &c, int64_t *page, int64_t *token
     *token = c.token_stride;
     *head = c.head_stride;
     return *page > 0 && *token >= c.head_dim && *head >= c.head_dim;
+}
+
+// Whether no two heads' rows share an element, so that writing them is no race: with the axes ordered by stride, a step along one clears
+// all that lies along those before it. (Reading rows that share elements is fine.)
+inline bool rows_apart(const tqhip_kv_cache &c) {
+    std::array<std::pair<int64_t, int>, 3> axis{{{0, c.n_pages}, {0, c.page_size}, {0, c.n_kv_heads}}};
+    (void)cache_strides(c, &axis[0].first, &axis[1].first, &axis[2].first);
+    std::sort(axis.begin(), axis.end());
+    __int128 extent = c.head_dim;
+    for (const auto &[stride, n] : axis) {
+        if (n == 1) continue;
+        if (stride < extent) return false;
+        extent += static_cast<__int128>(stride) * (n - 1);
+    }
+    return true;
 }
 
 // Checks of the cache and the batch that kv_append and paged_attention share.

@@ -268,7 +268,7 @@ int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip
     const int st = check_cache(*cache, *seqs);
     if (st != kOk) return st;
     if (!p.k || !p.v || cache->n_kv_heads != p.n_kv_heads || cache->head_dim != p.head_dim ||
-        seqs->n_tokens != p.n_tokens)
+        seqs->n_tokens != p.n_tokens || !rows_apart(*cache))
         return kBadShape;
     // f16 / bf16 activations go into a cache of their own type, f32 into any
     if (p.dtype != TQHIP_F32 && cache->dtype != p.dtype) return kBadShape;
