@@ -277,6 +277,10 @@ int tqhip_paged_attention_dev(const tqhip_attn *attn, const tqhip_kv_cache *cach
                               void *stream);
 /* Bytes of workspace that call needs (0: none), from the host's numbers alone. */
 size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs);
+/* How that call is cut, from the host's numbers alone: into tiles of *tile_rows rows (16 or 128, a kernel each; a row is a
+ * token's query head), and its keys into *parts parts. */
+int tqhip_paged_attention_plan(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs, int *tile_rows,
+                               int *parts);
 
 /* The low-rank adapters of many requests, beside the projection that they share:
  * y_t = base_t + scale[a] * B_a (A_a x_t), a = adapter[b] of the sequence b that token t is in.

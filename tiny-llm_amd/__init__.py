@@ -163,6 +163,7 @@ _SIGS = {
     "tqhip_kv_append_dev": (_i, [ctypes.POINTER(HeadProj), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _vp]),
     "tqhip_paged_attention_dev": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), _vp]),
     "tqhip_paged_attention_workspace": (_sz, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs)]),
+    "tqhip_paged_attention_plan": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), ctypes.POINTER(_i), ctypes.POINTER(_i)]),
     "tqhip_lora_add_dev": (_i, [ctypes.POINTER(Lora), _vp]),
     "tqhip_lora_workspace": (_sz, [ctypes.POINTER(Lora)]),
     # registry
@@ -538,6 +539,13 @@ def paged_attention_dev(attn: Attn, cache: KvCache, seqs: Seqs, stream=None) -> 
 
 def paged_attention_workspace(attn: Attn, cache: KvCache, seqs: Seqs) -> int:
     return int(lib().tqhip_paged_attention_workspace(attn, cache, seqs))
+
+
+def paged_attention_plan(attn: Attn, cache: KvCache, seqs: Seqs) -> "tuple[int, int]":
+    """(rows of a tile, parts of the keys) that the call is cut into."""
+    rows, parts = _i(), _i()
+    _check(lib().tqhip_paged_attention_plan(attn, cache, seqs, rows, parts), "tqhip_paged_attention_plan")
+    return rows.value, parts.value
 
 
 def lora_add_dev(lora: Lora, stream=None) -> None:

@@ -1141,4 +1141,15 @@ size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_ca
     return tqhip::plan_bytes(tqhip::plan(*attn, *cache, *seqs), *attn, *cache, *seqs);
 }
 
+int tqhip_paged_attention_plan(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs, int *tile_rows,
+                               int *parts) {
+    if (!attn || !cache || !seqs || !tile_rows || !parts) return tqhip::kBadShape;
+    const int st = tqhip::check_attn(*attn, *cache, *seqs);
+    if (st != tqhip::kOk) return st;
+    const tqhip::Plan n = tqhip::plan(*attn, *cache, *seqs);
+    *tile_rows = n.few ? tqhip::kFewRows : tqhip::kTileRows;
+    *parts = n.parts;
+    return tqhip::kOk;
+}
+
 }  // extern "C"
