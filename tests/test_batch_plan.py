@@ -30,3 +30,15 @@ def test_refusals(tqa):
         plan(tqa, 1, 1, 4, 2, D=96)
     with pytest.raises(RuntimeError):
         plan(tqa, 1, 1, 4, 2, window=-1)
+
+
+@pytest.mark.parametrize("tokens,seqs", [(1, 1), (256, 256), (2048, 256), (4096, 4096)])
+def test_workspace_of_many_rows_beside_a_long_sequence(tqa, tokens, seqs):
+    """Parts get longer where rows are many: a workspace of some 128 MB, not one of gigabytes."""
+    attn = tqa.Attn(dtype=0, n_heads=32, q=AT, out=AT, scale=0.1, causal=1)
+    cache = tqa.KvCache(k=AT, v=AT, dtype=1, n_pages=4, page_size=16, n_kv_heads=8, head_dim=128)
+    batch = tqa.Seqs(n_seqs=seqs, n_tokens=tokens, q_start=AT, kv_len=AT, block_table=AT, table_stride=8192, max_kv=131072)
+    rows, parts = tqa.paged_attention_plan(attn, cache, batch)
+    need = tqa.paged_attention_workspace(attn, cache, batch)
+    assert rows == 16 and need <= 128 << 20
+    assert need == (0 if parts == 1 else parts * tokens * 32 * (4 * 128 + 8))

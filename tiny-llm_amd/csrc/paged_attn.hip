@@ -990,7 +990,10 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
 // ---- host ----------------------------------------------------------------------------------------
 
 // How the work is cut, from the host's numbers alone.
+constexpr int64_t kMostPartBytes = int64_t{128} << 20;  // of attn_few's parts, where there are several
 constexpr int kMaxParts = 512;  // (a short window in a long cache asks for many, most of them empty)
+
+int64_t part_row_bytes(const tqhip_kv_cache &c) { return c.head_dim * sizeof(float) + sizeof(float2); }
 
 struct Plan {
     bool few;
@@ -1019,6 +1022,11 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
         // 128; of 14 heads over 3000: 14 of 128, 31 of 1024; 64 sequences of up to 16000: 423 of 1024, 455 of 512, 428 of 4096.
         const int64_t full = std::max<int64_t>(s.n_seqs, (rows + kFewRows - 1) / kFewRows) * c.n_kv_heads;  // tiles that there are
         n.span = static_cast<int>(std::clamp<int64_t>(up(seen * full / (2 * cus), kFewStep), kFewStep, 1024));
+        // Every row has room for every part up to the longest sequence's, and a workgroup too, most of them empty where one sequence of
+        // many is long: parts grow with the rows. 256 tokens of 32 heads of 128, one over 131072 keys, the rest over 2000: 740 us
+        // and 126 MB (64 MB at most: 711; 256: 887; parts of 1024: 1278 and 520 MB); 8 tokens each: 1369 (1845; 1172; 2587 and 4160 MB).
+        const int64_t most_parts = std::max<int64_t>(1, kMostPartBytes / (rows * c.n_kv_heads * part_row_bytes(c)));
+        if (kv > most_parts * n.span) n.span = static_cast<int>(up((kv + most_parts - 1) / most_parts, kFewStep));
     } else {
         // Two workgroups are resident per CU. With fewer tiles than 1.5 rounds of them, parts give three rounds, which evens out
         // ragged lengths too; of 512 keys at least, for a part's output is written and read again. Chunks of 257 over up
@@ -1035,8 +1043,7 @@ Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
 
 size_t plan_bytes(const Plan &n, const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
     if (n.parts == 1) return 0;
-    const size_t rows = static_cast<size_t>(s.n_tokens) * p.n_heads * n.parts;
-    return rows * (c.head_dim * sizeof(float) + sizeof(float2));
+    return static_cast<size_t>(s.n_tokens) * p.n_heads * n.parts * part_row_bytes(c);
 }
 
 template <typename T, typename C, int D>
