@@ -198,10 +198,15 @@ constexpr float kHeadroom = QT == 1 ? 7.0f : 1.0f;
 template <typename E>
 constexpr float kWeightShift = std::is_same_v<E, f16> ? 8.0f : 0.0f;
 
-// A bias is a rounded number: the key that it stands at has a weight of 2^kWeightShift times 2^(half a step of the bias) at most, which
-// leaves fp16's range, and then fp32's, when scores are of many millions. A row whose bias is past 2^22 (half a step is 1/4 there) gets a
-// sum of NaN, so formula_row takes it. (By size, not by whether it overflowed: so the parts of a row are treated alike.)
-__device__ inline float checked_sum(float bias, float l) { return fabsf(bias) > 4194304.0f ? NAN : l; }
+// A bias is a rounded number: the key that it stands at has a weight of 2^kWeightShift times 2^(up to half a step of the bias) either way,
+// and with scores of many millions that leaves fp16's range, and then fp32's. A row whose bias is past the last power of two at which it
+// does not (half a step of 1/2 on top of 2^15, of 4 on top of 2^9, of 8 in bf16, which would bear more) gets a sum of NaN, so
+// formula_row takes it: by size, not by whether it overflowed, so the parts of a row are treated alike.
+template <typename E, int QT>
+__device__ inline float checked_sum(float bias, float l) {
+    constexpr float kMost = !std::is_same_v<E, f16> ? 0x1p28f : QT == 1 ? 0x1p24f : 0x1p27f;
+    return fabsf(bias) > kMost ? NAN : l;
+}
 
 // ---- the sequence and the rows of a tile -----------------------------------------------------------
 
@@ -329,7 +334,7 @@ __device__ inline void formula_row(const AttnArgs &a, int b, int row, int token0
         const int64_t at = (static_cast<int64_t>(token) * a.n_heads + head) * a.parts + blockIdx.y;
         // (as everywhere, weights are 2^(score + bias): what the bias loses by its rounding goes into the sums, as far as fp32 holds it)
         const float bias = l > 0.0 ? static_cast<float>(fmin(fmax(-m, -FLT_MAX), FLT_MAX)) : 0.0f;
-        const double g = l > 0.0 ? exp2(fmin(fmax(m + bias, -100.0), 100.0)) : 1.0;
+        const double g = l > 0.0 ? exp2(fmin(fmax(m + bias, -64.0), 64.0)) : 1.0;
         if (lane == 0) a.part_ml[at] = make_float2(bias, static_cast<float>(l * g));
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = static_cast<float>(acc[i] * g);
@@ -584,7 +589,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     wait_loads();  // (the loads past the last step: into LDS that is used for other things below)
     l += lane_xor<16>(l, lane);
     l += lane_xor<32>(l, lane);
-    l = checked_sum(bias, l);
+    l = checked_sum<E, QT>(bias, l);
     // the four waves' sums, brought to the least exponent bias among those that have any
     if (g == 0) {
         sh.meet[0][wave][col] = bias;
@@ -891,7 +896,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
         }
         step(n, k0, partial, exist, &sh.v[kDirect ? buf : 0][0][0], &sh.k[kDirect ? buf ^ 1 : 0][0][0], &sh.v[kDirect ? buf ^ 1 : 0][0][0]);
     }
-    l = checked_sum(bias, l + lane_xor<32>(l, lane));
+    l = checked_sum<E, QT>(bias, l + lane_xor<32>(l, lane));
     float z = l * 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) z = not_finite<16>(acc[d], z);
