@@ -155,23 +155,44 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NR>) void lora_shrink(LoraArgs p)
     const float scale = p.scale[ad];
     const int live = min(BM, t.n - t.r0);
     float *u = p.u + (static_cast<int64_t>(blockIdx.y) * p.n_tokens + t.first + t.r0) * p.rank;
+    bool odd = false;
     for (int i = threadIdx.x; i < live * p.rank; i += 64 * NW) {
         const int row = i / p.rank, c = i - row * p.rank;
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += sum[w][row][c];
-        if (v * 0.0f != 0.0f) {  // infinite or NaN: by the formula, over what the workgroup's waves had
-            const int64_t k0 = 32 * (static_cast<int64_t>(steps) * blockIdx.y * NW / workers);
-            const int64_t k1 = min(32 * (static_cast<int64_t>(steps) * (blockIdx.y + 1) * NW / workers), static_cast<int64_t>(p.K));
-            const float *xr = p.x + static_cast<int64_t>(t.first + t.r0 + row) * p.K;
-            const W *ar = a + static_cast<int64_t>(c) * p.K;
-            double w = 0.0;
-#pragma unroll 1
-            for (int64_t k = k0; k < k1 && w == w; ++k) w += static_cast<double>(xr[k]) * static_cast<float>(ar[k]);
-            v = static_cast<float>(w);
-        }
+        odd = odd || v * 0.0f != 0.0f;
         u[i] = scale * v;
     }
+    if (!odd) return;
+    // the thread's infinite and NaN sums by the formula, over what the workgroup's waves had
+    const int64_t k0 = 32 * (static_cast<int64_t>(steps) * blockIdx.y * NW / workers);
+    const int64_t k1 = min(32 * (static_cast<int64_t>(steps) * (blockIdx.y + 1) * NW / workers), static_cast<int64_t>(p.K));
+#pragma unroll 1
+    for (int i = threadIdx.x; i < live * p.rank; i += 64 * NW) {
+        const int row = i / p.rank, c = i - row * p.rank;
+        if (u[i] * 0.0f == 0.0f) continue;
+        const float *xr = p.x + static_cast<int64_t>(t.first + t.r0 + row) * p.K;
+        const W *ar = a + static_cast<int64_t>(c) * p.K;
+        double v = 0.0;
+#pragma unroll 1
+        for (int64_t k = k0; k < k1 && v == v; ++k) v += static_cast<double>(xr[k]) * static_cast<float>(ar[k]);
+        u[i] = scale * static_cast<float>(v);
+    }
+}
+
+// One output by the formula.
+template <typename W>
+__device__ inline float formula_output(const float *base, const float *u, const W *b, int rank, int splits, int64_t split_stride) {
+    double v = base ? *base : 0.0f;
+#pragma unroll 1
+    for (int r = 0; r < rank && v == v; ++r) {
+        float u_r = 0.0f;
+#pragma unroll 1
+        for (int z = 0; z < splits; ++z) u_r += u[z * split_stride + r];
+        v += static_cast<double>(u_r) * static_cast<float>(b[r]);
+    }
+    return static_cast<float>(v);
 }
 
 // y = base + u B^T for a tile of 16 TT tokens and 128 S outputs, 32 of them per wave and step: the lane holds outputs
@@ -275,41 +296,21 @@ __global__ __launch_bounds__(256) void lora_expand(LoraArgs p) {
             }
         }
     }
-    // (a lane's outputs of a token are formed again together, and none of them is stored before: base may be y)
+    // Which of the lane's groups of 8 outputs are not all finite (or so large that products of pairs are not): they are not stored here,
+    // for base may be y.
     unsigned again = 0;
-#pragma unroll
-    for (int j = 0; j < TT; ++j) {
-        float z = 0.0f;
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) z = fmaf(acc[i][h][j][e], 0.0f, z);
-        if (z != 0.0f && 16 * j + col < live) again |= 1u << j;
-    }
-    for (unsigned left = again; left; left &= left - 1) {
-        const int64_t token = token0 + 16 * __builtin_ctz(left) + col;
-#pragma unroll 1
-        for (int n = 0; n < 8 * S; ++n) {
-            const int m = m_first + 128 * (n >> 3) + 32 * wave + 16 * (n >> 2 & 1) + 4 * g + (n & 3);
-            if (m >= p.M) continue;
-            double v = p.base ? p.base[token * p.M + m] : 0.0f;
-#pragma unroll 1
-            for (int r = 0; r < p.rank && v == v; ++r) {
-                float u_r = 0.0f;
-#pragma unroll 1
-                for (int z = 0; z < p.splits; ++z) u_r += p.u[(static_cast<int64_t>(z) * p.n_tokens + token) * p.rank + r];
-                v += static_cast<double>(u_r) * static_cast<float>(b[static_cast<int64_t>(m) * p.rank + r]);
-            }
-            p.y[token * p.M + m] = static_cast<float>(v);
-        }
-    }
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
-            if (16 * j + col >= live || again >> j & 1) continue;
+            float z = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) z = fmaf(acc[i][h][j][e], acc[i][h][j][e + 1], z);
+            z *= 0.0f;
+            again |= static_cast<unsigned>(z != 0.0f) << (i * TT + j);
+            if (16 * j + col >= live || z != 0.0f) continue;
             float *dst = p.y + (token0 + 16 * j + col) * p.M;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -322,6 +323,21 @@ __global__ __launch_bounds__(256) void lora_expand(LoraArgs p) {
                 }
             }
         }
+    if (__builtin_expect(again == 0, 1)) return;
+#pragma unroll 1
+    for (; again; again &= again - 1) {
+        const int i = __builtin_ctz(again) / TT, j = __builtin_ctz(again) % TT;
+        const int64_t token = token0 + 16 * j + col;
+        if (16 * j + col >= live) continue;
+#pragma unroll 1
+        for (int n = 0; n < 8; ++n) {
+            const int m = m_first + 128 * i + 32 * wave + 16 * (n >> 2) + 4 * g + (n & 3);
+            if (m >= p.M) continue;
+            const int64_t at = token * p.M + m;
+            p.y[at] = formula_output(p.base ? p.base + at : nullptr, p.u + token * p.rank, b + static_cast<int64_t>(m) * p.rank, p.rank, p.splits,
+                                     static_cast<int64_t>(p.n_tokens) * p.rank);
+        }
+    }
 }
 
 // ---- host ----------------------------------------------------------------------------------------

@@ -525,8 +525,8 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
         }
         vec<E, 8> p[QT];
         split<E, QT>(w, p);
-        unsigned wild = 0;
         if (partial) {  // infinite and NaN values as in attn_tiles
+            unsigned wild = 0;
             if constexpr (kDirect) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
@@ -549,6 +549,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
                     wild |= static_cast<unsigned>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff) << (16 * kt);
                 }
             }
+            if (wild & exist & below(hi - k0) & ~below(lo - k0)) l = NAN;  // (formula_row takes the row)
         }
 #pragma unroll
         for (int kj = 0; kj < KT; ++kj) {
@@ -577,7 +578,6 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
             }
             if constexpr (!kDirect) wave_lds_order();
         }
-        if (wild & exist & below(hi - k0) & ~below(lo - k0)) l = NAN;  // (formula_row takes the row)
         k0 += kFewStep;
     };
     E *v0 = &sh.v[wave][0][0][0], *v1 = &sh.v[wave][kDirect ? 1 : 0][0][0];
@@ -641,7 +641,9 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
             }
         }
     }
-    for (int i = 0; odd && i < 4; ++i)
+    if (__builtin_expect(odd == 0, 1)) return;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i)
         if (odd >> (16 * i) & 0xffff) {
             const int ro = t.r0 + 4 * wave + i, p = t.pos0 + ro / a.group;
             formula_row<T, C, D>(a, t.b, ro, t.first, kvh, max(kb, key_lo(a, p)), min(ke, key_hi(a, p, t.len)));
@@ -927,6 +929,8 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
                 }
         }
     }
+    if (__builtin_expect(odd == 0, 1)) return;
+#pragma unroll 1
     for (; odd; odd &= odd - 1) {
         const int ro = wr0 + __builtin_ctzll(odd), p = t.pos0 + ro / a.group;
         formula_row<T, C, D>(a, t.b, ro, t.first, kvh, max(kb, key_lo(a, p)), min(ke, key_hi(a, p, t.len)));
