@@ -208,3 +208,27 @@ def test_lora_of_infinities(gpu, dtype, new, K, M, r):
     gpu.synchronize()
     same = (dy0.download(np.int32, T * M) == bits) | np.isnan(got.ravel())
     assert same.all()
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("cache", [F16, BF16, F32])
+@pytest.mark.parametrize("large", [1e3, 1e5, 1e7])
+def test_queries_with_one_large_dimension(gpu, new, kv, Hq, Hk, cache, large):
+    """A dimension in which queries are large and keys small: its terms are no larger than the others', so the others' bits count. The
+    bound is that of every row, (2 (D + 4) S + 2 N + 32) u of sum p |v|, S the size of the scores' terms. Over an fp16 cache a query element
+    is two fp16 terms of a row scaled to below 2^15: the second one is off by 2^-25 at most where it is subnormal, 2^-39 of the row's
+    largest element (which is 2^14 at least), so a score by 2^-39 max|q| sum |k| scale more, e, and a result by 2 e of sum p |v|."""
+    D = 64
+    b = Batch(gpu, new, kv, 16, Hk, D, cache, seed=8)
+    k = b.k.values
+    k[..., 5] /= large
+    bits, b.k.values = ref.raw(k, cache)
+    b.k.buf.upload(bits)
+    x = 1.5 * b.rng.standard_normal((b.tokens, Hq, D))
+    x[..., 5] *= large
+    q = Dev(gpu, x, F32)
+    got = attend(gpu, b, F32, Hq, 0.125, q)
+    want, spread, score, _ = ref.attention(b, q.values, 0.125, 1, 0)
+    e = 2.0 ** -39 * np.abs(q.values).max(-1, keepdims=True) * np.nansum(np.abs(b.k.values), -1).max() * 0.125 * (cache == F16)
+    assert np.all(np.abs(got - want) <= (2 * (D + 4) * score + 2 * max(kv) + 32) * U * spread + 2 * e * spread)
+    assert np.linalg.norm(got - want) <= 2.0 ** -17 * np.linalg.norm(want) + np.linalg.norm(2 * e * spread)

@@ -234,7 +234,9 @@ constexpr float kLeastScale = 1e-37f;
 
 // A row's query as the operand of the score products: N chunks of 8 elements, STEP apart, in each of the lanes that hold the
 // row (wide(x): the largest x over them). Returns the factor that takes a product to a power of two's exponent. fp32 rows
-// against fp16 keys are scaled into fp16's range by a power of two, which that factor takes back.
+// against fp16 keys are scaled by a power of two, which that factor takes back, so that their largest element is below 2^15: at the upper
+// end of fp16's range, because an element's second term is off by up to 2^-25 where it is subnormal, which is to be little for small
+// elements beside a large one too: 2^-39 of the largest. (With the largest below 1, elements 1000 times smaller kept 15 bits.)
 template <typename T, typename E, int QT, int N, int STEP, typename Wide>
 __device__ inline float load_query(const AttnArgs &a, const T *qp, vec<E, 8> (*q)[N], Wide wide) {
     float c = a.scale;
@@ -256,7 +258,7 @@ __device__ inline float load_query(const AttnArgs &a, const T *qp, vec<E, 8> (*q
                 for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
             }
             mx = wide(mx);
-            if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex);
+            if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &ex), ex -= 15;
             c = fmaxf(ldexpf(c, ex), kLeastScale);
         }
 #pragma unroll
