@@ -232,3 +232,34 @@ def test_queries_with_one_large_dimension(gpu, new, kv, Hq, Hk, cache, large):
     e = 2.0 ** -39 * np.abs(q.values).max(-1, keepdims=True) * np.nansum(np.abs(b.k.values), -1).max() * 0.125 * (cache == F16)
     assert np.all(np.abs(got - want) <= (2 * (D + 4) * score + 2 * max(kv) + 32) * U * spread + 2 * e * spread)
     assert np.linalg.norm(got - want) <= 2.0 ** -17 * np.linalg.norm(want) + np.linalg.norm(2 * e * spread)
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("cache", [F16, BF16, F32])
+@pytest.mark.parametrize("gap", [12.0, 14.0, 20.0])
+def test_a_first_key_with_nearly_all_the_weight(gpu, new, kv, Hq, Hk, cache, gap):
+    """The first key outweighs each of the others by e^12 to e^20 or so and its value is zero: the result is made of the small weights.
+    Beside the bound of every row: over an fp16 cache a weight is two fp16 terms, the largest weight at 2^14 or above, so a small one is off by 2^-25,
+    2^-39 of the largest, and a result by e = 2^-39 sum |v|."""
+    D = 64
+    b = Batch(gpu, new, kv, 16, Hk, D, cache, seed=9)
+    k, v = b.k.values, b.v.values
+    k[..., 0] = np.where(np.isnan(k[..., 0]), np.nan, 0.0)
+    for s in range(len(kv)):
+        place = b.place(s, 0)
+        k[place] = 0.0
+        k[place][:, 0], v[place] = 1.0, 0.0
+    for dev, x in ((b.k, k), (b.v, v)):
+        bits, dev.values = ref.raw(x, cache)
+        dev.buf.upload(bits)
+    x = 0.5 * b.rng.standard_normal((b.tokens, Hq, D))
+    x[..., 0] = 8 * gap
+    q = Dev(gpu, x, F32)
+    got = attend(gpu, b, F32, Hq, 0.125, q)
+    want, spread, score, _ = ref.attention(b, q.values, 0.125, 1, 0)
+    assert 0 < np.linalg.norm(spread[-1]) < 1e-3 * max(kv)
+    e = 2.0 ** -39 * np.nansum(np.abs(v)) * (cache == F16)
+    assert np.all(np.abs(got - want) <= (2 * (D + 4) * score + 2 * max(kv) + 32) * U * spread + e)
+    # errors of the weights are random, so their sum is that of their squares: sqrt(N) of a half step at most, in each dimension
+    typical = 2.0 ** -39 * np.sqrt(max(kv)) * 2 * np.sqrt(want.size) * (cache == F16)
+    assert np.linalg.norm(got - want) <= 2.0 ** -17 * np.linalg.norm(want) + typical

@@ -194,18 +194,19 @@ __device__ inline void wait_loads() {
 template <int QT>
 constexpr float kHeadroom = QT == 1 ? 7.0f : 1.0f;
 
-// Weights are 2^(s c + bias): with fp16 terms they are held 2^8 times larger, above fp16's subnormals.
-template <typename E>
-constexpr float kWeightShift = std::is_same_v<E, f16> ? 8.0f : 0.0f;
+// Weights are 2^(s c + bias), held as large as fp16's range lets them be, 2^15 with the headroom: below 2^-14 they are subnormal, off by up
+// to 2^-25, and weights small beside the largest count where its value is small. (Two terms at 2^8 lost half of the bits of weights
+// 2^-20 of the largest.) bf16 has the range.
+template <typename E, int QT>
+constexpr float kWeightShift = std::is_same_v<E, f16> ? 15.0f - kHeadroom<QT> : 0.0f;
 
 // A bias is a rounded number: the key that it stands at has a weight of 2^kWeightShift times 2^(up to half a step of the bias) either way,
 // and with scores of many millions that leaves fp16's range, and then fp32's. A row whose bias is past the last power of two at which it
-// does not (half a step of 1/2 on top of 2^15, of 4 on top of 2^9, of 8 in bf16, which would bear more) gets a sum of NaN, so
-// formula_row takes it: by size, not by whether it overflowed, so the parts of a row are treated alike.
-template <typename E, int QT>
+// does not (half a step of 1/2 on top of 2^15, of 8 in bf16, which would bear more) gets a sum of NaN, so formula_row takes it: by
+// size, not by whether it overflowed, so the parts of a row are treated alike.
+template <typename E>
 __device__ inline float checked_sum(float bias, float l) {
-    constexpr float kMost = !std::is_same_v<E, f16> ? 0x1p28f : QT == 1 ? 0x1p24f : 0x1p27f;
-    return fabsf(bias) > kMost ? NAN : l;
+    return fabsf(bias) > (std::is_same_v<E, f16> ? 0x1p24f : 0x1p28f) ? NAN : l;
 }
 
 // ---- the sequence and the rows of a tile -----------------------------------------------------------
@@ -511,7 +512,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
         mx = fmaxf(mx, lane_xor<16>(mx, lane));
         mx = fmaxf(mx, lane_xor<32>(mx, lane));
         if (__ballot((mx - m) * c > kHeadroom<QT>)) {
-            const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
+            const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E, QT>);
             const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
             m = mx;
             bias = nb;
@@ -591,7 +592,7 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
     wait_loads();  // (the loads past the last step: into LDS that is used for other things below)
     l += lane_xor<16>(l, lane);
     l += lane_xor<32>(l, lane);
-    l = checked_sum<E, QT>(bias, l);
+    l = checked_sum<E>(bias, l);
     // the four waves' sums, brought to the least exponent bias among those that have any
     if (g == 0) {
         sh.meet[0][wave][col] = bias;
@@ -809,7 +810,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
             mx = fmaxf(mx, lane_xor<32>(mx, lane));
             if (__ballot((mx - m) * c > kHeadroom<QT>)) {
-                const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E>);
+                const float nb = mx == -INFINITY ? 0.0f : fmaf(-mx, c, kWeightShift<E, QT>);
                 const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
                 m = mx;
                 bias = nb;
@@ -900,7 +901,7 @@ __global__ __launch_bounds__(256, (TileShape<T, C, D>::kWavesPerSimd)) void attn
         }
         step(n, k0, partial, exist, &sh.v[kDirect ? buf : 0][0][0], &sh.k[kDirect ? buf ^ 1 : 0][0][0], &sh.v[kDirect ? buf ^ 1 : 0][0][0]);
     }
-    l = checked_sum<E, QT>(bias, l + lane_xor<32>(l, lane));
+    l = checked_sum<E>(bias, l + lane_xor<32>(l, lane));
     float z = l * 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) z = not_finite<16>(acc[d], z);
