@@ -182,7 +182,11 @@ int tqhip_matvec_i4_generic_dev(const uint8_t *w, const float *x, float *y, int 
  *
  * Types: activations f32 (what the projections above read and write), or f16 / bf16; the
  * cache f32 / f16 / bf16. Arithmetic, norms and softmax statistics are in fp32, angles in
- * fp64; results are rounded once, to nearest even. */
+ * fp64; results are rounded once, to nearest even, but for attention with f16 / bf16 activations:
+ * there each softmax weight is rounded to that type too before it meets its value (in f16, whose
+ * range ends, by up to 2^-33 of the row's largest weight). With f32 activations attention and adapters
+ * keep 22 to 24 bits of every operand (over an f16 cache: or 2^-39 of the row's largest query element,
+ * or weight, where that is more). */
 #define TQHIP_F32 0
 #define TQHIP_F16 1
 #define TQHIP_BF16 2
@@ -230,7 +234,7 @@ typedef struct tqhip_kv_cache {
  * written nor attended to. */
 typedef struct tqhip_seqs {
     int n_seqs, n_tokens;
-    const int *q_start;              /* device, [n_seqs + 1], not decreasing */
+    const int *q_start;              /* device, [n_seqs + 1], not decreasing, 0 to n_tokens */
     const int *kv_len;               /* device, [n_seqs] */
     const int *block_table;          /* device, [n_seqs][table_stride] */
     int table_stride;

@@ -9,9 +9,11 @@
 // An infinity is its first term, and no number beside the zero or the other sign of the other operand's next one: results that
 // are not finite are formed again by the formula, in 64 bits, by the threads that have them. The loops carry nothing for it.
 //
-// Both launches are bound by HBM (x once; base and y once; A and B stay in L2) or, with few tokens, by latency. 3555 tokens of 8
-// requests, rank 64 in bf16 beside 9728x2560: 26 and 73 us for 38 and 287 MB. 64 requests of a token, rank 16 in fp16 beside
-// 4096x2560: 5.7 and 7 us.
+// Both launches are bound by HBM (x once; base and y once) or, with few tokens, by latency. 3555 tokens of 8
+// requests, rank 64 in bf16 beside 9728x2560: 26 and 73 us; the second reads base and u, 139 MB, and writes as much, and as its tiles of one
+// block of outputs go to all XCDs, each of those reads all of B into its L2, another 60 MB. 64 requests of a token, rank 16 in fp16 beside
+// 4096x2560: 5.8 and 7 us. Requests of one token are a tile each, also where they share an adapter: 256 of them, rank 64 beside
+// 9728x2560, take 28 and 57 us for one adapter or four.
 #include <algorithm>
 #include <optional>
 #include <type_traits>

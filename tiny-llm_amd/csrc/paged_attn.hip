@@ -17,10 +17,11 @@
 // key/value heads is its head: with 8 of them an XCD reads one head's keys and keeps them in its L2.
 // (Every XCD taking all heads: 878 us instead of 789 for the prompts below.)
 //   64 tokens of 32 heads on 8 of 128, up to 16000 fp16 keys each (2.06 GB):        395 us, 5.2 TB/s
-//   two prompts of up to 8192, the same heads, all in bf16 (706 GFLOP):             789 us, 0.90 PFLOP/s
-//   four chunks of up to 257 fp32 tokens over up to 8000 fp16 keys, the same heads:  204 us (72 GFLOP of two terms each), 17 of them the join
-//   three prompts of up to 5001 fp32 tokens, a window of 1000 bf16 keys, 14 heads on 2 of 64: 130 us (33.5 GFLOP of three terms each)
-//   one fp32 token of 14 heads on 2 of 64 over 3000 fp32 keys:                        9.4 us and 4.0 for the join
+//   two prompts of up to 8192, the same heads, all in bf16 (706 GFLOP):             735 to 807 us, 0.87 to 0.96 PFLOP/s
+//   four chunks of up to 257 fp32 tokens over up to 8000 fp16 keys, the same heads:  191 to 206 us (72 GFLOP of two terms each), 17 of them the join
+//   three prompts of up to 5001 fp32 tokens, a window of 1000 bf16 keys, 14 heads on 2 of 64: 130 to 138 us (33.5 GFLOP of three terms each)
+//   one fp32 token of 14 heads on 2 of 64 over 3000 fp32 keys:                        9.5 us and 4.0 for the join
+// (from card to card; one of them took 880, 217 and 144 us for the three that the products bound)
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -55,6 +56,8 @@ struct AttnArgs {
 // or a weight, KT of a cache element. 16-bit activations meet a cache of their own type as they are.
 // fp32 activations keep their precision: against an fp16 cache two fp16 terms (22 bits), against
 // a bf16 one three bf16 terms (24 bits), and an fp32 cache is three bf16 terms itself.
+// (One term rounds the weights too, once more than the result: bf16 prompts are 2.1e-3 from 64 bits, where the result's
+// rounding alone is 1.6e-3. A second term would be half as many products again, for bits that the result does not keep.)
 template <typename T, typename C>
 struct Terms {
     using E = std::conditional_t<std::is_same_v<C, f16>, f16, bf16>;
@@ -657,8 +660,8 @@ __global__ __launch_bounds__(256, (D == 256 || (D == 128 && sizeof(C) == 4) ? 1 
 
 // A wave takes 32 of the rows, all four the same keys: 64 at a time (32 where registers are short), K and V in LDS, the next tile's
 // on the way there while this one's are used. Two workgroups a CU, so a wave that waits for LDS or for its workgroup leaves
-// the SIMD to one of the other's. Of the 789 us of the bf16 prompts at the top the matrix cores are busy 39 %, the vector
-// units 45 %, LDS 22 %; without the exponentials they would take 760, without the next tile's loads 670, without the second
+// the SIMD to one of the other's. Of the time of the bf16 prompts at the top the matrix cores are busy 42 %, the vector
+// units 42 %, LDS 24 %; of 789 us, without the exponentials they would take 760, without the next tile's loads 670, without the second
 // product's instructions 694, and the loads and barriers alone 451: it is no single unit but the waits between them.
 template <typename T, typename C, int D>
 struct TileShape {
