@@ -309,6 +309,63 @@ typedef struct tqhip_lora {
 int tqhip_lora_add_dev(const tqhip_lora *lora, void *stream);
 size_t tqhip_lora_workspace(const tqhip_lora *lora);
 
+/* The pages of a batch from the lengths of its requests, without the host: sequence b is to have past[b] + n_new[b] cached
+ * positions, and so ceil of that / page_size pages. Pages that it has too many (a request that ended has length 0, one whose
+ * drafts were refused is shorter than it was) are put on the list of free pages and their table entries become -1, sequence by sequence,
+ * in their order in the table; then the pages that sequences lack are taken off the end of the list, sequence by sequence. The first
+ * sequence whose pages are not all there gets none, nor does any after it that lacks some, nor one that needs more than table_stride:
+ * missing[b] says how many (0: all there), and such a sequence's new positions past its pages do not exist.
+ * Written for the calls above: q_start, kv_len (past + n_new; may be past itself), and for every token its position and its slot
+ * (page * page_size + row; -1 where it does not exist), both -1 for tokens past the last sequence's. The sum of n_new is at most n_tokens.
+ * A new server starts with n_held of 0, tables of -1 and all pages on the list. Numbers that make no sense (negative lengths,
+ * n_held past the table, a list longer than the cache) are taken as the nearest that does. Up to 4096 sequences. */
+typedef struct tqhip_page_map {
+    int n_seqs, n_tokens;
+    int n_pages, page_size, table_stride;
+    const int *past;                 /* device, [n_seqs]: cached positions that stay */
+    const int *n_new;                /* device, [n_seqs]: tokens of the coming call */
+    int *block_table;                /* device, [n_seqs][table_stride], updated */
+    int *n_held;                     /* device, [n_seqs], updated: pages that a sequence has, its first entries of the table */
+    int *free_pages;                 /* device, [n_pages], updated */
+    int *n_free;                     /* device, [1], updated */
+    int *q_start;                    /* device, [n_seqs + 1] */
+    int *kv_len, *missing;           /* device, [n_seqs] */
+    int *positions, *slots;          /* device, [n_tokens], or NULL */
+} tqhip_page_map;
+int tqhip_page_map_dev(const tqhip_page_map *map, void *stream);
+
+/* Verification of drafted tokens, and the draw of the token after them. Sequence b has the call's tokens q_start[b] .. q_start[b + 1] - 1: the
+ * last one that it was given, then its drafts (none: a plain draw). Row t of logits is the target's for what follows token t (as matmul_i4
+ * writes them), row t of draft the draft model's from which tokens[t + 1] was drawn; draft NULL: each draft is its
+ * distribution's only token. With p = softmax(logits / T), q = softmax(draft / T) of row t, T = temperature[b], the draft x = tokens[t + 1] is
+ * accepted iff accept[t] q(x) < p(x). The first draft refused is replaced by a draw from max(p - q, 0) (from p, where that is nothing),
+ * and the row of the last token, or of one before a token outside [0, vocab) (a sequence with fewer drafts than it has room for), draws from p: the token is the first whose
+ * prefix sum exceeds pick[b] times the sum. A T that is not above 0 takes each row's first largest logit. Sums are in 64 bits.
+ * out_tokens: from q_start[b] on the accepted drafts and the token drawn, n_out[b] in all, then -1. logprob: log p of each (T of 0: as of 1), then 0.
+ * past: kv_len[b] less the refused drafts, the cached positions that stay. Logits of minus infinity have probability 0; a row with NaN or plus infinity, or
+ * with nothing else, has no probabilities: as a target it ends its sequence with a token of -1, which n_out counts, as a draft it refuses,
+ * and the draw is from p. Tokens of no sequence keep their outputs. vocab up to 2^22.
+ * workspace: as for the attention, tqhip_verify_tokens_workspace() bytes. */
+typedef struct tqhip_verify {
+    int dtype;                       /* of logits and draft: TQHIP_F32 / F16 / BF16 */
+    int n_seqs, n_tokens, vocab;
+    const void *logits, *draft;      /* [n_tokens][vocab]; draft may be NULL */
+    int64_t logits_stride, draft_stride;  /* elements from row to row; 0: vocab */
+    const int *q_start;              /* device, [n_seqs + 1], not decreasing, 0 to n_tokens */
+    const int *tokens;               /* device, [n_tokens] */
+    const float *temperature;        /* device, [n_seqs], or NULL: 1 */
+    const float *accept;             /* device, [n_tokens]: random numbers in [0, 1) */
+    const float *pick;               /* device, [n_seqs]: random numbers in [0, 1) */
+    const int *kv_len;               /* device, [n_seqs], where past is given */
+    int *past;                       /* device, [n_seqs], or NULL; may be kv_len */
+    int *out_tokens, *n_out;         /* device, [n_tokens] and [n_seqs] */
+    float *logprob;                  /* device, [n_tokens], or NULL */
+    void *workspace;
+    size_t workspace_bytes;
+} tqhip_verify;
+int tqhip_verify_tokens_dev(const tqhip_verify *verify, void *stream);
+size_t tqhip_verify_tokens_workspace(const tqhip_verify *verify);
+
 /* ---- 3. registry (kernels/dispatch.h:155-159, 191-195; set_matmul_i4_impl_by_name is new) */
 
 int tqhip_set_matvec_i4_impl_by_name(const char *name);   /* 1 = selected, 0 = unknown name */
@@ -383,6 +440,8 @@ typedef struct tqhip_op {
 #define TQHIP_OP_KV_APPEND 10    /* w = const tqhip_head_proj *, w2 = const tqhip_kv_cache *, w3 = const tqhip_seqs * */
 #define TQHIP_OP_PAGED_ATTENTION 11  /* w = const tqhip_attn *, w2 = const tqhip_kv_cache *, w3 = const tqhip_seqs * */
 #define TQHIP_OP_LORA_ADD 12     /* w = const tqhip_lora * */
+#define TQHIP_OP_PAGE_MAP 13     /* w = const tqhip_page_map * */
+#define TQHIP_OP_VERIFY_TOKENS 14  /* w = const tqhip_verify * */
 int tqhip_run_ops(const tqhip_op *ops, int n_ops, int repeats, void *stream);
 /* As tqhip_run_ops, with a HIP event pair around every call; op_ms[i] gets the
  * mean event-to-event time of call i over the repeats (kernel duration as the

@@ -37,7 +37,7 @@ tqwen_synth = _load_sibling("tqwen_synth")
 OK, EBADSHAPE, EBADGROUP, ETOOLARGE, ELAUNCH, EFILE, EHIP, ENOSCRATCH = 0, -1, -2, -3, -4, -5, -6, -7
 NOALLOC_SCRATCH_BYTES = 16 << 20  # TQHIP_NOALLOC_SCRATCH_BYTES
 OP_I4_MATVEC, OP_VQ2_MATVEC, OP_I4_MATMUL, OP_I4_PAIR, OP_I4_QKV, OP_BIIP_ROTATE, OP_I4_SET, OP_VQ2_SET = 1, 2, 3, 4, 5, 6, 7, 8
-OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD = 9, 10, 11, 12
+OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD, OP_PAGE_MAP, OP_VERIFY_TOKENS = 9, 10, 11, 12, 13, 14
 F32, F16, BF16 = 0, 1, 2  # TQHIP_F32 / F16 / BF16
 
 _u8p = ctypes.POINTER(ctypes.c_uint8)
@@ -113,8 +113,23 @@ class Lora(ctypes.Structure):
                [("workspace_bytes", _sz)]
 
 
+class PageMap(ctypes.Structure):
+    """tqhip_page_map: the lengths of a batch's requests, their pages and the list of free ones."""
+    _fields_ = [(n, _i) for n in ("n_seqs", "n_tokens", "n_pages", "page_size", "table_stride")] + \
+               [(n, _vp) for n in ("past", "n_new", "block_table", "n_held", "free_pages", "n_free", "q_start", "kv_len", "missing", "positions",
+                                   "slots")]
+
+
+class Verify(ctypes.Structure):
+    """tqhip_verify: drafted tokens, the rows that judge them and the random numbers."""
+    _fields_ = [(n, _i) for n in ("dtype", "n_seqs", "n_tokens", "vocab")] + [("logits", _vp), ("draft", _vp)] + \
+               [("logits_stride", _i64), ("draft_stride", _i64)] + \
+               [(n, _vp) for n in ("q_start", "tokens", "temperature", "accept", "pick", "kv_len", "past", "out_tokens", "n_out", "logprob",
+                                   "workspace")] + [("workspace_bytes", _sz)]
+
+
 def batch_op(kind: int, *structs) -> Op:
-    """An Op of one of the batch calls (OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD) over its
+    """An Op of one of the batch calls (OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD, OP_PAGE_MAP, OP_VERIFY_TOKENS) over its
     structs, in the order in which the call takes them; keep the structs alive while the op is used."""
     at = [ctypes.addressof(s) for s in structs] + [None, None]
     return Op(kind, at[0], None, None, 0, 0, 0, 0, at[1], at[2])
@@ -166,6 +181,9 @@ _SIGS = {
     "tqhip_paged_attention_plan": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), ctypes.POINTER(_i), ctypes.POINTER(_i)]),
     "tqhip_lora_add_dev": (_i, [ctypes.POINTER(Lora), _vp]),
     "tqhip_lora_workspace": (_sz, [ctypes.POINTER(Lora)]),
+    "tqhip_page_map_dev": (_i, [ctypes.POINTER(PageMap), _vp]),
+    "tqhip_verify_tokens_dev": (_i, [ctypes.POINTER(Verify), _vp]),
+    "tqhip_verify_tokens_workspace": (_sz, [ctypes.POINTER(Verify)]),
     # registry
     "tqhip_set_ops_impl_by_name": (_i, [ctypes.c_char_p]),
     "tqhip_ops_impl_name": (ctypes.c_char_p, []),
@@ -555,6 +573,20 @@ def lora_add_dev(lora: Lora, stream=None) -> None:
 
 def lora_workspace(lora: Lora) -> int:
     return int(lib().tqhip_lora_workspace(lora))
+
+
+def page_map_dev(page_map: PageMap, stream=None) -> None:
+    """Block tables, free pages, q_start, kv_len, positions and slots of a batch from the lengths of its requests."""
+    _check(lib().tqhip_page_map_dev(page_map, _stream(stream)), "tqhip_page_map_dev")
+
+
+def verify_tokens_dev(verify: Verify, stream=None) -> None:
+    """Drafted tokens accepted or refused, and the token after them drawn, from given random numbers."""
+    _check(lib().tqhip_verify_tokens_dev(verify, _stream(stream)), "tqhip_verify_tokens_dev")
+
+
+def verify_tokens_workspace(verify: Verify) -> int:
+    return int(lib().tqhip_verify_tokens_workspace(verify))
 
 
 class Stream:

@@ -1,4 +1,4 @@
-// batch.h -- what the kernels of a batch of requests share (heads.hip, paged_attn.hip, lora.hip):
+// batch.h -- what the kernels of a batch of requests share (heads.hip, paged_attn.hip, lora.hip, page_map.hip, verify.hip):
 // element types, the search of a token's sequence, positions to pages.
 #pragma once
 
@@ -43,6 +43,18 @@ __device__ inline void store_rounded(T *p, const float *in) {
 __device__ inline void wave_lds_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+}
+
+// The last i in [0, n) with at[i] <= x (at[0] <= x).
+template <typename I>
+__device__ inline int last_at_most(const I *at, int n, I x) {
+    int lo = 0;
+    while (n > 1) {
+        const int half = n / 2;
+        if (at[lo + half] <= x) lo += half;
+        n -= half;
+    }
+    return lo;
 }
 
 // The sequence b of token t and the token's position in it; false where it is in none. The 64 lanes of a wave search

@@ -536,6 +536,8 @@ static int launch_op(const tqhip_op &op, hipStream_t s) {
                                              static_cast<const tqhip_kv_cache *>(op.w2),
                                              static_cast<const tqhip_seqs *>(op.w3), s);
         case TQHIP_OP_LORA_ADD: return tqhip_lora_add_dev(static_cast<const tqhip_lora *>(op.w), s);
+        case TQHIP_OP_PAGE_MAP: return tqhip_page_map_dev(static_cast<const tqhip_page_map *>(op.w), s);
+        case TQHIP_OP_VERIFY_TOKENS: return tqhip_verify_tokens_dev(static_cast<const tqhip_verify *>(op.w), s);
         default: return kBadShape;
     }
 }
