@@ -190,6 +190,8 @@ int tqhip_matvec_i4_generic_dev(const uint8_t *w, const float *x, float *y, int 
 #define TQHIP_F32 0
 #define TQHIP_F16 1
 #define TQHIP_BF16 2
+#define TQHIP_I8 3      /* codes of a cache of 8 bits: integers from -127 to 127 */
+#define TQHIP_E4M3 4    /* the same, as floating-point numbers of 4 bits of exponent and 3 of fraction, up to 448 */
 
 /* The query, key and value heads of a batch of tokens as the projections leave them. Head h
  * of token t is at pointer + t * stride + h * head_dim elements; a stride of 0 stands for
@@ -308,6 +310,32 @@ typedef struct tqhip_lora {
 } tqhip_lora;
 int tqhip_lora_add_dev(const tqhip_lora *lora, void *stream);
 size_t tqhip_lora_workspace(const tqhip_lora *lora);
+
+/* A paged cache of 8-bit codes (pages and strides as of tqhip_kv_cache, an element a byte). Rows of a page come in blocks of `block`, and a
+ * block has a scale for each key/value head, for keys and for values: an element is its code times its block's scale. The scales of block i of page p,
+ * head h, are the two floats at scales + 2 * ((p * n_kv_heads + h) * (page_size / block) + i): of the keys, of the values. */
+typedef struct tqhip_kv_cache8 {
+    void *k, *v;
+    float *scales;                   /* [n_pages][n_kv_heads][page_size / block][2], 8-byte aligned */
+    int dtype;                       /* TQHIP_I8 or TQHIP_E4M3 */
+    int n_pages, page_size, block;   /* block divides page_size */
+    int n_kv_heads, head_dim;
+    int64_t page_stride, token_stride, head_stride;
+} tqhip_kv_cache8;
+
+/* tqhip_kv_append_dev into such a cache. Of a block's new rows, scale = max(largest |x| / top, 2^-60), top 127 (i8) or 448 (e4m3), and an
+ * element's code is x / scale rounded to nearest even. A block whose first rows are there already (as the lengths say) keeps its scale where that is larger;
+ * where it is not, its codes are brought to the new one, code * old / new, rounded again. Rows past the new ones are left as they are. An infinity
+ * or NaN makes its block's scale, and so all of the block, NaN, until the block is written from its first row on. head_dim 64, 128 or 256; the cache
+ * 16-byte aligned, its strides multiples of 16. Two sequences of a call must not have new rows in one block. */
+int tqhip_kv_append8_dev(const tqhip_head_proj *proj, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, void *stream);
+
+/* tqhip_paged_attention_dev over such a cache, with activations of any of the three types; the codes enter as they are and the scales in fp32.
+ * With f16 / bf16 activations softmax weights, times their value's scale, are rounded to fp16; with f32 they keep 22 bits, or 2^-39 of the row's largest
+ * such product where that is more. What is said there of infinities and NaN holds for elements: codes times scales. */
+int tqhip_paged_attention8_dev(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, void *stream);
+size_t tqhip_paged_attention8_workspace(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs);
+int tqhip_paged_attention8_plan(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, int *tile_rows, int *parts);
 
 /* The pages of a batch from the lengths of its requests, without the host: sequence b is to have past[b] + n_new[b] cached
  * positions, and so ceil of that / page_size pages. Pages that it has too many (a request that ended has length 0, one whose
@@ -442,6 +470,8 @@ typedef struct tqhip_op {
 #define TQHIP_OP_LORA_ADD 12     /* w = const tqhip_lora * */
 #define TQHIP_OP_PAGE_MAP 13     /* w = const tqhip_page_map * */
 #define TQHIP_OP_VERIFY_TOKENS 14  /* w = const tqhip_verify * */
+#define TQHIP_OP_KV_APPEND8 15     /* w = const tqhip_head_proj *, w2 = const tqhip_kv_cache8 *, w3 = const tqhip_seqs * */
+#define TQHIP_OP_PAGED_ATTENTION8 16  /* w = const tqhip_attn *, w2 = const tqhip_kv_cache8 *, w3 = const tqhip_seqs * */
 int tqhip_run_ops(const tqhip_op *ops, int n_ops, int repeats, void *stream);
 /* As tqhip_run_ops, with a HIP event pair around every call; op_ms[i] gets the
  * mean event-to-event time of call i over the repeats (kernel duration as the

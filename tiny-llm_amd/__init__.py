@@ -37,8 +37,8 @@ tqwen_synth = _load_sibling("tqwen_synth")
 OK, EBADSHAPE, EBADGROUP, ETOOLARGE, ELAUNCH, EFILE, EHIP, ENOSCRATCH = 0, -1, -2, -3, -4, -5, -6, -7
 NOALLOC_SCRATCH_BYTES = 16 << 20  # TQHIP_NOALLOC_SCRATCH_BYTES
 OP_I4_MATVEC, OP_VQ2_MATVEC, OP_I4_MATMUL, OP_I4_PAIR, OP_I4_QKV, OP_BIIP_ROTATE, OP_I4_SET, OP_VQ2_SET = 1, 2, 3, 4, 5, 6, 7, 8
-OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD, OP_PAGE_MAP, OP_VERIFY_TOKENS = 9, 10, 11, 12, 13, 14
-F32, F16, BF16 = 0, 1, 2  # TQHIP_F32 / F16 / BF16
+OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD, OP_PAGE_MAP, OP_VERIFY_TOKENS, OP_KV_APPEND8, OP_PAGED_ATTENTION8 = range(9, 17)
+F32, F16, BF16, I8, E4M3 = 0, 1, 2, 3, 4  # TQHIP_F32 / F16 / BF16 / I8 / E4M3
 
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _f32p = ctypes.POINTER(ctypes.c_float)
@@ -113,6 +113,13 @@ class Lora(ctypes.Structure):
                [("workspace_bytes", _sz)]
 
 
+class KvCache8(ctypes.Structure):
+    """tqhip_kv_cache8: a paged cache of 8-bit codes with a scale for each block of tokens and head."""
+    _fields_ = [("k", _vp), ("v", _vp), ("scales", _vp)] + \
+               [(n, _i) for n in ("dtype", "n_pages", "page_size", "block", "n_kv_heads", "head_dim")] + \
+               [(n, _i64) for n in ("page_stride", "token_stride", "head_stride")]
+
+
 class PageMap(ctypes.Structure):
     """tqhip_page_map: the lengths of a batch's requests, their pages and the list of free ones."""
     _fields_ = [(n, _i) for n in ("n_seqs", "n_tokens", "n_pages", "page_size", "table_stride")] + \
@@ -129,8 +136,8 @@ class Verify(ctypes.Structure):
 
 
 def batch_op(kind: int, *structs) -> Op:
-    """An Op of one of the batch calls (OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD, OP_PAGE_MAP, OP_VERIFY_TOKENS) over its
-    structs, in the order in which the call takes them; keep the structs alive while the op is used."""
+    """An Op of one of the batch calls (OP_QK_NORM_ROPE, OP_KV_APPEND, OP_PAGED_ATTENTION, OP_LORA_ADD, OP_PAGE_MAP,
+    OP_VERIFY_TOKENS, OP_KV_APPEND8, OP_PAGED_ATTENTION8) over its structs, in the order in which the call takes them; keep the structs alive while the op is used."""
     at = [ctypes.addressof(s) for s in structs] + [None, None]
     return Op(kind, at[0], None, None, 0, 0, 0, 0, at[1], at[2])
 
@@ -181,6 +188,10 @@ _SIGS = {
     "tqhip_paged_attention_plan": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache), ctypes.POINTER(Seqs), ctypes.POINTER(_i), ctypes.POINTER(_i)]),
     "tqhip_lora_add_dev": (_i, [ctypes.POINTER(Lora), _vp]),
     "tqhip_lora_workspace": (_sz, [ctypes.POINTER(Lora)]),
+    "tqhip_kv_append8_dev": (_i, [ctypes.POINTER(HeadProj), ctypes.POINTER(KvCache8), ctypes.POINTER(Seqs), _vp]),
+    "tqhip_paged_attention8_dev": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache8), ctypes.POINTER(Seqs), _vp]),
+    "tqhip_paged_attention8_workspace": (_sz, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache8), ctypes.POINTER(Seqs)]),
+    "tqhip_paged_attention8_plan": (_i, [ctypes.POINTER(Attn), ctypes.POINTER(KvCache8), ctypes.POINTER(Seqs), ctypes.POINTER(_i), ctypes.POINTER(_i)]),
     "tqhip_page_map_dev": (_i, [ctypes.POINTER(PageMap), _vp]),
     "tqhip_verify_tokens_dev": (_i, [ctypes.POINTER(Verify), _vp]),
     "tqhip_verify_tokens_workspace": (_sz, [ctypes.POINTER(Verify)]),
@@ -573,6 +584,27 @@ def lora_add_dev(lora: Lora, stream=None) -> None:
 
 def lora_workspace(lora: Lora) -> int:
     return int(lib().tqhip_lora_workspace(lora))
+
+
+def kv_append8_dev(proj: HeadProj, cache: KvCache8, seqs: Seqs, stream=None) -> None:
+    """k (normed and rotated) and v into the sequences' pages of 8-bit codes; q -> q_out beside them where both are given."""
+    _check(lib().tqhip_kv_append8_dev(proj, cache, seqs, _stream(stream)), "tqhip_kv_append8_dev")
+
+
+def paged_attention8_dev(attn: Attn, cache: KvCache8, seqs: Seqs, stream=None) -> None:
+    """Attention of the batch's tokens over their sequences' pages of 8-bit codes."""
+    _check(lib().tqhip_paged_attention8_dev(attn, cache, seqs, _stream(stream)), "tqhip_paged_attention8_dev")
+
+
+def paged_attention8_workspace(attn: Attn, cache: KvCache8, seqs: Seqs) -> int:
+    return int(lib().tqhip_paged_attention8_workspace(attn, cache, seqs))
+
+
+def paged_attention8_plan(attn: Attn, cache: KvCache8, seqs: Seqs) -> "tuple[int, int]":
+    """(rows of a tile, parts of the keys) that the call is cut into."""
+    rows, parts = _i(), _i()
+    _check(lib().tqhip_paged_attention8_plan(attn, cache, seqs, rows, parts), "tqhip_paged_attention8_plan")
+    return rows.value, parts.value
 
 
 def page_map_dev(page_map: PageMap, stream=None) -> None:

@@ -1,4 +1,4 @@
-// batch.h -- what the kernels of a batch of requests share (heads.hip, paged_attn.hip, lora.hip, page_map.hip, verify.hip):
+// batch.h -- what the kernels of a batch of requests share (heads.hip, append8.hip, paged_attn.hip, paged_attn8.hip, lora.hip, page_map.hip, verify.hip):
 // element types, the search of a token's sequence, positions to pages.
 #pragma once
 
@@ -12,6 +12,12 @@
 #include "../../include/tqhip.h"
 
 namespace tqhip {
+
+// heads.hip, for append8.hip: checks of what is neither pointer nor stride, and the queries that ride along with an append.
+int check_heads(const tqhip_head_proj &p);
+int finish_queries(const tqhip_head_proj &p, const tqhip_kv_cache &rows, const tqhip_seqs &seqs, hipStream_t s);
+constexpr int kMostHeads = 8192;  // (rounds of all heads times their parts fit 32 bits)
+
 namespace {
 
 using bf16 = __bf16;
@@ -184,6 +190,20 @@ inline int check_cache(const tqhip_kv_cache &c, const tqhip_seqs &s) {
     // offsets are 64-bit; what has to fit 32 bits, a tile's length to spare, are the positions
     if (static_cast<int64_t>(s.table_stride) * c.page_size > INT32_MAX / 2) return TQHIP_ETOOLARGE;
     return TQHIP_OK;
+}
+
+// A cache of 8-bit codes as a cache of rows: its pages and strides (in bytes, which are its elements).
+inline tqhip_kv_cache rows_of(const tqhip_kv_cache8 &c) {
+    return {c.k, c.v, TQHIP_F16, c.n_pages, c.page_size, c.n_kv_heads, c.head_dim, c.page_stride, c.token_stride, c.head_stride};
+}
+inline int check_cache8(const tqhip_kv_cache8 &c, const tqhip_seqs &s) {
+    const int st = check_cache(rows_of(c), s);
+    if (st != TQHIP_OK) return st;
+    if ((c.dtype != TQHIP_I8 && c.dtype != TQHIP_E4M3) || !c.scales || reinterpret_cast<uintptr_t>(c.scales) % 8 || c.block < 1 ||
+        c.page_size % c.block)
+        return TQHIP_EBADSHAPE;
+    // places of scales are 32-bit
+    return static_cast<__int128>(c.n_pages) * c.n_kv_heads * (c.page_size / c.block) > INT32_MAX ? TQHIP_ETOOLARGE : TQHIP_OK;
 }
 
 inline Pages make_pages(const tqhip_kv_cache &c, const tqhip_seqs &s) {

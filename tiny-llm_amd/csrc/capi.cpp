@@ -538,6 +538,14 @@ static int launch_op(const tqhip_op &op, hipStream_t s) {
         case TQHIP_OP_LORA_ADD: return tqhip_lora_add_dev(static_cast<const tqhip_lora *>(op.w), s);
         case TQHIP_OP_PAGE_MAP: return tqhip_page_map_dev(static_cast<const tqhip_page_map *>(op.w), s);
         case TQHIP_OP_VERIFY_TOKENS: return tqhip_verify_tokens_dev(static_cast<const tqhip_verify *>(op.w), s);
+        case TQHIP_OP_KV_APPEND8:
+            return tqhip_kv_append8_dev(static_cast<const tqhip_head_proj *>(op.w),
+                                        static_cast<const tqhip_kv_cache8 *>(op.w2),
+                                        static_cast<const tqhip_seqs *>(op.w3), s);
+        case TQHIP_OP_PAGED_ATTENTION8:
+            return tqhip_paged_attention8_dev(static_cast<const tqhip_attn *>(op.w),
+                                              static_cast<const tqhip_kv_cache8 *>(op.w2),
+                                              static_cast<const tqhip_seqs *>(op.w3), s);
         default: return kBadShape;
     }
 }

@@ -229,16 +229,13 @@ bool aligned(const void *p, int64_t stride, int bytes) {
 }
 
 int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip_seqs *seqs, hipStream_t s) {
-    if (!type_known(p.dtype) || p.n_tokens < 1 || p.head_dim < 2 || p.head_dim > 512 || p.head_dim % 2 ||
-        p.rotary_dim < 0 || p.rotary_dim > p.head_dim || p.rotary_dim % 2 || p.n_heads < 0 || p.n_kv_heads < 0)
-        return kBadShape;
+    const int ok = check_heads(p);
+    if (ok != kOk) return ok;
     const bool q = p.q && p.q_out, k = cache || (p.k && p.k_out);
     if ((!p.q) != (!p.q_out) || (!cache && (!p.k) != (!p.k_out))) return kBadShape;
     if ((!q && !k) || (q && p.n_heads < 1) || (k && p.n_kv_heads < 1)) return kBadShape;
     if (!cache && !p.positions && p.rotary_dim) return kBadShape;
-    if (p.rotary_dim && !p.inv_freq && !(p.theta > 0.0 && std::isfinite(p.theta))) return kBadShape;
-    if (!(p.eps >= 0.0f)) return kBadShape;
-    if (std::max(p.n_heads, p.n_kv_heads) > 8192) return kTooLarge;  // (rounds of all heads times their parts fit 32 bits)
+    if (std::max(p.n_heads, p.n_kv_heads) > kMostHeads) return kTooLarge;
     HeadArgs a{{p.q, p.k, p.v}, {}, {p.q_bias, p.k_bias, p.v_bias}, {p.q_norm, p.k_norm}, {p.q_out, p.k_out}, {},
                {nullptr, nullptr}, {q ? p.n_heads : 0, k ? p.n_kv_heads : 0, cache ? p.n_kv_heads : 0}, p.n_tokens,
                p.head_dim, p.rotary_dim, p.eps, p.rotary_dim && !p.inv_freq ? std::log2(p.theta) : 0.0, p.inv_freq,
@@ -291,6 +288,36 @@ int run_heads(const tqhip_head_proj &p, const tqhip_kv_cache *cache, const tqhip
 }
 
 }  // namespace
+
+int check_heads(const tqhip_head_proj &p) {
+    if (!type_known(p.dtype) || p.n_tokens < 1 || p.head_dim < 2 || p.head_dim > 512 || p.head_dim % 2 ||
+        p.rotary_dim < 0 || p.rotary_dim > p.head_dim || p.rotary_dim % 2 || p.n_heads < 0 || p.n_kv_heads < 0)
+        return kBadShape;
+    if (p.rotary_dim && !p.inv_freq && !(p.theta > 0.0 && std::isfinite(p.theta))) return kBadShape;
+    return p.eps >= 0.0f ? kOk : kBadShape;
+}
+
+// The queries of a call whose keys and values are another kernel's: a call without them, whose positions are those in the cache.
+int finish_queries(const tqhip_head_proj &p, const tqhip_kv_cache &rows, const tqhip_seqs &seqs, hipStream_t s) {
+    HeadArgs a{{p.q, nullptr, nullptr}, {p.q_stride, 0, 0}, {p.q_bias, nullptr, nullptr}, {p.q_norm, nullptr}, {p.q_out, nullptr}, {p.q_out_stride, 0},
+               {nullptr, nullptr}, {p.n_heads, 0, 0}, p.n_tokens, p.head_dim, p.rotary_dim, p.eps,
+               p.rotary_dim && !p.inv_freq ? std::log2(p.theta) : 0.0, p.inv_freq, p.positions, 1, seqs.q_start, seqs.kv_len, seqs.n_seqs,
+               make_pages(rows, seqs)};
+    const int64_t row = static_cast<int64_t>(p.n_heads) * p.head_dim;
+    if (!a.in_stride[0]) a.in_stride[0] = row;
+    if (!a.out_stride[0]) a.out_stride[0] = row;
+    if (p.n_tokens > 1 && (a.in_stride[0] < row || a.out_stride[0] < row)) return kBadShape;
+    const int bytes = type_bytes(p.dtype), v = 16 / bytes, lanes = p.head_dim / (2 * v);
+    const bool wide = p.head_dim % (2 * v) == 0 && p.rotary_dim % (2 * v) == 0 && lanes >= 4 && lanes <= 32 && (lanes & (lanes - 1)) == 0 &&
+                      aligned(p.q, a.in_stride[0], bytes) && aligned(p.q_out, a.out_stride[0], bytes) && aligned(p.q_bias, 0, 4) &&
+                      aligned(p.q_norm, 0, 4);
+    switch (p.dtype) {
+        case TQHIP_F32: return launch_heads<float, float, true>(a, wide, s);
+        case TQHIP_F16: return launch_heads<f16, f16, true>(a, wide, s);
+        default: return launch_heads<bf16, bf16, true>(a, wide, s);
+    }
+}
+
 }  // namespace tqhip
 
 extern "C" {
