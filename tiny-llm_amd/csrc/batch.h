@@ -86,6 +86,25 @@ __device__ inline bool find_token(const int *start, const int *len, int n, int t
     return t < e;
 }
 
+// The sequence b of token t and where its tokens end; false where it is in none. The wave searches as in find_token.
+__device__ inline bool find_seq(const int *start, int n, int t, int &b, int &end) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    while (n > 64) {
+        const int step = (n + 63) / 64, i = lane * step;
+        const int c = __popcll(__ballot(i < n && start[lo + i] <= t));
+        if (c == 0) return false;
+        lo += (c - 1) * step;
+        n = min(step, n - (c - 1) * step);
+    }
+    const int at = lo + min(lane, n - 1), first = start[at], next = start[at + 1];
+    const int c = __popcll(__ballot(lane < n && first <= t));
+    if (c == 0) return false;
+    b = lo + c - 1;
+    end = __builtin_amdgcn_readlane(next, c - 1);
+    return t < end;
+}
+
 // The rows of a ragged batch in tiles of BM: a sequence with n tokens has n * per rows (per: rows of a token). Tiles are numbered
 // over the batch without a scan of the lengths: sequence b's start at floor(start[b] per / BM) + b, which leaves room for
 // ceil(n per / BM) of them, so there are floor(n_tokens per / BM) + n_seqs numbers and some name no tile.
