@@ -57,7 +57,7 @@ def check(gpu, b, act, Hq, causal=1, window=0, scale=None, q_std=1.5, stream=Non
 
 TYPES = [(a, c) for c in (I8, E4M3) for a in (F32, F16, BF16)]
 SHAPES = [(14, 2, 64), (8, 2, 128), (2, 1, 256)]
-# new tokens, cached positions, query heads, key/value heads: 16 rows a tile and 128, in one part and in several
+# new tokens, cached positions, query heads, key/value heads: tiles of 16, 32 and (twice) 128 rows, in one part and in several
 FORMS = [([3, 9], [9, 100], 2, 1), ([40, 1], [1400, 2100], 4, 2), ([90, 170], [90, 200], 8, 8), ([150, 130], [1700, 900], 8, 8)]
 
 
@@ -82,7 +82,7 @@ def test_forms(gpu, act, dtype, new, kv, Hq, Hk):
     b = Batch8(gpu, new, kv, 32, Hk, 128, dtype, 8, seed=2, spread=3)
     rows, parts = gpu.paged_attention8_plan(gpu.Attn(dtype=act, n_heads=Hq, q=256, out=256, scale=1.0, causal=1), b.c, b.s)
     i = FORMS.index((new, kv, Hq, Hk))
-    assert (rows, parts > 1) == ((16, 128)[i // 2], bool(i % 2))
+    assert (rows, parts > 1) == ((16, 32, 128, 128)[i], bool(i % 2))
     check(gpu, b, act, Hq)
 
 

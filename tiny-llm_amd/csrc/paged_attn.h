@@ -476,10 +476,10 @@ inline int64_t part_row_bytes(const tqhip_kv_cache &c) { return c.head_dim * siz
 
 struct Plan {
     bool few;
-    int tiles, parts, span;
+    int rows, tiles, parts, span;  // rows of a tile: 16 or (over codes of 8 bits) 32, or 128
 };
 
-inline Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
+inline Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s, bool codes) {
     const int group = p.n_heads / c.n_kv_heads;
     const int64_t rows = static_cast<int64_t>(s.n_tokens) * group;
     Plan n{};
@@ -488,19 +488,24 @@ inline Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs 
     // as there are few of them in all, because there they come in shorter parts (one sequence of 64 rows on 8 K/V heads 22 us and 32,
     // 128 rows 34 and 34; 448 rows on 2 heads of 64 30 and 41, 1792 rows 79 and 47; 1024 on one of 256 52 and 81).
     n.few = rows <= int64_t{2} * kFewRows * s.n_seqs || (rows + kFewRows - 1) / kFewRows * c.n_kv_heads <= 56;
-    n.tiles = static_cast<int>(rows / (n.few ? kFewRows : kTileRows)) + s.n_seqs;
+    // Over codes of 8 bits, 32 rows a tile where sequences have more than 16, so that their keys are read once: five tokens each of 32 sequences of up to 9000
+    // keys, 20 rows a head: FEW32. (Heads of 256 with fp32 terms for two of them do not fit the registers.)
+    const bool pairs = codes && !(c.head_dim == 256 && p.dtype == TQHIP_F32);
+    n.rows = !n.few ? kTileRows : pairs && rows > int64_t{kFewRows} * s.n_seqs ? 2 * kFewRows : kFewRows;
+    n.tiles = static_cast<int>(rows / n.rows) + s.n_seqs;
     const int64_t most = static_cast<int64_t>(s.table_stride) * c.page_size;
     const int64_t kv = s.max_kv > 0 ? std::min<int64_t>(s.max_kv, most) : most;
     // keys that one tile reads
-    const int64_t seen = p.causal && p.window > 0 ? std::min<int64_t>(kv, int64_t{p.window} + (n.few ? kFewRows : kTileRows)) : kv;
+    const int64_t seen = p.causal && p.window > 0 ? std::min<int64_t>(kv, int64_t{p.window} + n.rows) : kv;
     const int64_t blocks = static_cast<int64_t>(n.tiles) * c.n_kv_heads, cus = device_cu_count();
     const auto up = [](int64_t x, int64_t to) { return (x + to - 1) / to * to; };
     if (n.few) {
         // A workgroup's start and end cost as much as some 500 keys, so parts are as long as two workgroups per CU make them, up to
         // 1024 keys, which evens out ragged lengths. One token of 32 heads over 30000 keys: 35 us in parts of 512, 61 of
-        // 128; of 14 heads over 3000: 14 of 128, 31 of 1024; 64 sequences of up to 16000: 423 of 1024, 455 of 512, 428 of 4096.
-        const int64_t full = std::max<int64_t>(s.n_seqs, (rows + kFewRows - 1) / kFewRows) * c.n_kv_heads;  // tiles that there are
-        n.span = static_cast<int>(std::clamp<int64_t>(up(seen * full / (2 * cus), kFewStep), kFewStep, 1024));
+        // 128; of 14 heads over 3000: 14 of 128, 31 of 1024; 64 sequences of up to 16000: 423 of 1024, 455 of 512, 428 of 4096; over codes of
+        // 8 bits, half the bytes a key, 269 of 1024, 245 of 2048, 242 of 4096.
+        const int64_t full = std::max<int64_t>(s.n_seqs, (rows + n.rows - 1) / n.rows) * c.n_kv_heads;  // tiles that there are
+        n.span = static_cast<int>(std::clamp<int64_t>(up(seen * full / (2 * cus), kFewStep), kFewStep, codes ? 2048 : 1024));
         // Every row has room for every part up to the longest sequence's, and a workgroup too, most of them empty where one sequence of
         // many is long: parts grow with the rows. 256 tokens of 32 heads of 128, one over 131072 keys, the rest over 2000: 740 us
         // and 126 MB (64 MB at most: 711; 256: 887; parts of 1024: 1278 and 520 MB); 8 tokens each: 1369 (1845; 1172; 2587 and 4160 MB).

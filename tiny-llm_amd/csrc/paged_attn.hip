@@ -637,7 +637,7 @@ int check(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &s) {
 int run(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs &b, hipStream_t s) {
     const int st = check(p, c, b);
     if (st != kOk) return st;
-    return run_attn(p, c, b, plan(p, c, b), s, [&](const AttnArgs &a, const Plan &n) {
+    return run_attn(p, c, b, plan(p, c, b, false), s, [&](const AttnArgs &a, const Plan &n) {
         if (p.dtype == TQHIP_F16)
             launch_attn<f16, f16>(a, n, c.head_dim, s);
         else if (p.dtype == TQHIP_BF16)
@@ -668,7 +668,7 @@ int tqhip_paged_attention_dev(const tqhip_attn *attn, const tqhip_kv_cache *cach
 
 size_t tqhip_paged_attention_workspace(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs) {
     if (!attn || !cache || !seqs || tqhip::check(*attn, *cache, *seqs) != tqhip::kOk) return 0;
-    return tqhip::plan_bytes(tqhip::plan(*attn, *cache, *seqs), *attn, *cache, *seqs);
+    return tqhip::plan_bytes(tqhip::plan(*attn, *cache, *seqs, false), *attn, *cache, *seqs);
 }
 
 int tqhip_paged_attention_plan(const tqhip_attn *attn, const tqhip_kv_cache *cache, const tqhip_seqs *seqs, int *tile_rows,
@@ -676,8 +676,8 @@ int tqhip_paged_attention_plan(const tqhip_attn *attn, const tqhip_kv_cache *cac
     if (!attn || !cache || !seqs || !tile_rows || !parts) return tqhip::kBadShape;
     const int st = tqhip::check(*attn, *cache, *seqs);
     if (st != tqhip::kOk) return st;
-    const tqhip::Plan n = tqhip::plan(*attn, *cache, *seqs);
-    *tile_rows = n.few ? tqhip::kFewRows : tqhip::kTileRows;
+    const tqhip::Plan n = tqhip::plan(*attn, *cache, *seqs, false);
+    *tile_rows = n.rows;
     *parts = n.parts;
     return tqhip::kOk;
 }

@@ -85,26 +85,32 @@ constexpr int kScaleA = 0, kScaleLog = 1, kScaleB = 2;
 
 // As over the other caches: 32 keys a wave and step, K straight into operand registers (16 codes a lane and load, which are the chunks of
 // two products), V into LDS as it is and out of it by transposing reads of bytes.
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, int R>
 __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a) {
     constexpr int QT = Terms<T, C>::QT;
+    constexpr int kRows = R * kFewRows;
     constexpr int ND = D / 16, NS = D / 32, NL = D / 64, CH = D / 16, NV = kFewKeys * CH / 64;
     __shared__ struct {
         union {
             __attribute__((aligned(16))) unsigned char v[4][2][kFewKeys][D];
-            float o[4][kFewRows][D];
+            float o[4][kRows][D];
         };
         __attribute__((aligned(16))) float by[4][3][kFewKeys];
-        float meet[2][4][kFewRows];
+        float meet[2][4][kRows];
     } sh;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
     const int kv_heads = a.n_heads / a.group;
-    const int kvh = blockIdx.x % kv_heads;
+    // The heads of a tile follow one another on one XCD, eight tiles at a time on the eight: where a token's heads lie side by side, they
+    // read the same pages of memory at about the same time. Which tile goes to which XCD moves on with the eight and with the part, so that neither long
+    // sequences nor numbers that name no tile stay with one of them. (64 single tokens and 32 times five of them, the figures below: 228 and 88 us; each
+    // head an XCD of its own 250 and 101; without the moving on 231 and 129.)
+    const int tiles = gridDim.x / kv_heads, eights = tiles / 8, x = blockIdx.x, eight = x / (8 * kv_heads), over = x - eights * 8 * kv_heads;
+    const int kvh = over < 0 ? x / 8 % kv_heads : over % kv_heads;
     TileRows t;
-    if (!find_tile<kFewRows>(a, blockIdx.x / kv_heads, t)) return;
+    if (!find_tile<kRows>(a, over < 0 ? 8 * eight + (x + eight + static_cast<int>(blockIdx.y)) % 8 : 8 * eights + over / kv_heads, t)) return;
     const int rows = t.n * a.group;
-    const int last = min(t.r0 + kFewRows, rows) - 1;
+    const int last = min(t.r0 + kRows, rows) - 1;
     const int p_first = t.pos0 + t.r0 / a.group, p_last = t.pos0 + last / a.group;
     int ke = key_hi(a, p_last, t.len), kb = max(min(key_lo(a, p_first), ke), 0);  // (a window past the table is empty)
     if (a.parts > 1) {
@@ -113,10 +119,15 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
         if (kb >= ke) return;
     }
     const int full_lo = key_lo(a, p_last), full_hi = key_hi(a, p_first, t.len);
-    const int r = min(t.r0 + col, rows - 1);
-    const int token = t.first + r / a.group, head = kvh * a.group + r % a.group;
-    const int pos = t.pos0 + r / a.group;
-    const int lo = key_lo(a, pos), hi = key_hi(a, pos, t.len);
+    // the lane's rows: t.r0 + 16 r + col
+    const auto row_of = [&](int r) { return min(t.r0 + kFewRows * r + col, rows - 1); };
+    int lo[R], hi[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int pos = t.pos0 + row_of(r) / a.group;
+        lo[r] = key_lo(a, pos);
+        hi[r] = key_hi(a, pos, t.len);
+    }
 
     const unsigned char *kc = static_cast<const unsigned char *>(a.k) + kvh * a.pages.head_stride + 16 * g;
     const unsigned char *vc = static_cast<const unsigned char *>(a.v) + kvh * a.pages.head_stride;
@@ -171,18 +182,28 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
     load_values(off, &sh.v[wave][0][0][0]);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) by_next[kt] = a.scales[at[kt]];
-    vec<f16, 8> q[QT][NS];
-    const float c = load_query<T, f16, QT, NS>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 16 * g, q,
-                                               [](int i) { return 64 * (i / 2) + 8 * (i % 2); },
-                                               [&](float x) {
-                                                   x = fmaxf(x, lane_xor<16>(x, lane));
-                                                   return fmaxf(x, lane_xor<32>(x, lane));
-                                               });
-    const float unit = scale_unit(fmaxf(off[0] >= 0 ? by_next[0].y : 0.0f, off[1] >= 0 ? by_next[1].y : 0.0f)), per_unit = 1.0f / unit;
-    f32x4 acc[ND];
+    vec<f16, 8> q[R][QT][NS];
+    float c[R];
 #pragma unroll
-    for (int i = 0; i < ND; ++i) acc[i] = f32x4{};
-    float m = -INFINITY, bias = 0.0f, l = 0.0f;
+    for (int r = 0; r < R; ++r) {
+        const int row = row_of(r), token = t.first + row / a.group, head = kvh * a.group + row % a.group;
+        c[r] = load_query<T, f16, QT, NS>(a, static_cast<const T *>(a.q) + token * a.q_stride + head * D + 16 * g, q[r],
+                                          [](int i) { return 64 * (i / 2) + 8 * (i % 2); },
+                                          [&](float x) {
+                                              x = fmaxf(x, lane_xor<16>(x, lane));
+                                              return fmaxf(x, lane_xor<32>(x, lane));
+                                          });
+    }
+    const float unit = scale_unit(fmaxf(off[0] >= 0 ? by_next[0].y : 0.0f, off[1] >= 0 ? by_next[1].y : 0.0f)), per_unit = 1.0f / unit;
+    f32x4 acc[R][ND];
+    float m[R], bias[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc[r][i] = f32x4{};
+        m[r] = -INFINITY;
+        bias[r] = l[r] = 0.0f;
+    }
 
     // (The restrict pointers tell the compiler that the next step's transfers do not touch the values that are read meanwhile.)
     const auto step = [&](const vec<unsigned, 4> (*k_now)[NL], vec<unsigned, 4> (*k_next)[NL], const unsigned char *__restrict__ v_now,
@@ -206,62 +227,70 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
             sh.by[wave][kScaleB][16 * g + col] = relative_scale(x.y, per_unit, log);
             sh.by[wave][kScaleLog][16 * g + col] = log;
         }
-        // S^T: the lane holds its row's scores of keys 16 kt + 4 g + i
-        f32x4 s[2];
+        // S^T: the lane holds its rows' scores of keys 16 kt + 4 g + i
+        f32x4 s[R][2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            s[kt] = f32x4{};
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r][kt] = f32x4{};
 #pragma unroll
             for (int j = 0; j < NL; ++j)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const vec<f16, 8> kf = as_halves<C>(k_now[kt][j][2 * half], k_now[kt][j][2 * half + 1]);
 #pragma unroll
-                    for (int qi = 0; qi < QT; ++qi) s[kt] = mfma16(kf, q[qi][2 * j + half], s[kt]);
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int qi = 0; qi < QT; ++qi) s[r][kt] = mfma16(kf, q[r][qi][2 * j + half], s[r][kt]);
                 }
         }
         wave_lds_order();
-        f32x4 lg[2], b[2];
+        const auto by_of = [&](int what, int kt) { return *reinterpret_cast<const f32x4 *>(&sh.by[wave][what][16 * kt + 4 * g]); };
+        const f32x4 sa[2] = {by_of(kScaleA, 0), by_of(kScaleA, 1)}, lg[2] = {by_of(kScaleLog, 0), by_of(kScaleLog, 1)},
+                    b[2] = {by_of(kScaleB, 0), by_of(kScaleB, 1)};
+        vec<f16, 8> p[R][QT];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            s[kt] *= *reinterpret_cast<const f32x4 *>(&sh.by[wave][kScaleA][16 * kt + 4 * g]);
-            lg[kt] = *reinterpret_cast<const f32x4 *>(&sh.by[wave][kScaleLog][16 * kt + 4 * g]);
-            b[kt] = *reinterpret_cast<const f32x4 *>(&sh.by[wave][kScaleB][16 * kt + 4 * g]);
+        for (int r = 0; r < R; ++r) {
+            unsigned may = ~0u;
+            if (partial) {
+                const int k1 = k0 + 4 * g;
+                may = (exist >> (4 * g)) & below(hi[r] - k1) & ~below(lo[r] - k1);
+            }
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) s[r][kt] *= sa[kt];
+            if (partial) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!(may & (1u << (16 * (e / 4) + e % 4)))) s[r][e / 4][e % 4] = -INFINITY;
+            }
+            float mx = m[r];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fmaf(s[r][e / 4][e % 4], c[r], lg[e / 4][e % 4]));
+            mx = fmaxf(mx, lane_xor<16>(mx, lane));
+            mx = fmaxf(mx, lane_xor<32>(mx, lane));
+            if (__ballot(mx - m[r] > kHeadroom<QT>)) {
+                const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, QT> - mx;
+                const float f = m[r] == -INFINITY ? 0.0f : exp2f(nb - bias[r]);
+                m[r] = mx;
+                bias[r] = nb;
+                l[r] *= f;
+#pragma unroll
+                for (int i = 0; i < ND; ++i) acc[r][i] *= f;
+            }
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(fmaf(s[r][e / 4][e % 4], c[r], bias[r]));
+                l[r] += w[e];
+                w[e] = as_fp32(w[e] * b[e / 4][e % 4]);
+            }
+            if (partial) {  // (the scale of a masked value may be no number)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!(may & (1u << (16 * (e / 4) + e % 4)))) w[e] = 0.0f;
+            }
+            split<f16, QT>(w, p[r]);
         }
-        if (partial) {
-            const int k1 = k0 + 4 * g;
-            const unsigned may = (exist >> (4 * g)) & below(hi - k1) & ~below(lo - k1);
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!(may & (1u << (16 * kt + i)))) s[kt][i] = -INFINITY, b[kt][i] = 0.0f;
-        }
-        float mx = m;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaf(s[kt][i], c, lg[kt][i]));
-        mx = fmaxf(mx, lane_xor<16>(mx, lane));
-        mx = fmaxf(mx, lane_xor<32>(mx, lane));
-        if (__ballot(mx - m > kHeadroom<QT>)) {
-            const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, QT> - mx;
-            const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
-            m = mx;
-            bias = nb;
-            l *= f;
-#pragma unroll
-            for (int i = 0; i < ND; ++i) acc[i] *= f;
-        }
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            w[e] = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], c, bias));
-            l += w[e];
-            w[e] = as_fp32(w[e] * b[e / 4][e % 4]);
-        }
-        vec<f16, 8> p[QT];
-        split<f16, QT>(w, p);
         if constexpr (std::is_same_v<C, e4m3>) {
             if (partial) {  // NaN codes as the infinite and NaN values of attn_tiles
                 unsigned wild = 0;
@@ -276,7 +305,9 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
                         if (bad & ((1ull << CH) - 1)) wild |= 1u << row;
                 }
                 wave_lds_order();
-                if (wild & exist & below(hi - k0) & ~below(lo - k0)) l = NAN;  // (formula_row takes the row)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (wild & exist & below(hi[r] - k0) & ~below(lo[r] - k0)) l[r] = NAN;  // (formula_row takes the row)
             }
         }
 #pragma unroll
@@ -285,7 +316,9 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
             const vec<unsigned, 2> u = lds_code_columns(v_now + row * D + (d ^ swap(row)) * 16 + 8 * (lane & 1));
             const vec<f16, 8> vf = as_halves<C>(u[0], u[1]);
 #pragma unroll
-            for (int qi = 0; qi < QT; ++qi) acc[d] = mfma16(vf, p[qi], acc[d]);
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int qi = 0; qi < QT; ++qi) acc[r][d] = mfma16(vf, p[r][qi], acc[r][d]);
         }
         k0 += kFewStep;
     };
@@ -296,67 +329,78 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
         step(kr[1], kr[0], v1, v0);
     }
     wait_loads();  // (the loads past the last step: into LDS that is used for other things below)
-    l += lane_xor<16>(l, lane);
-    l += lane_xor<32>(l, lane);
-    l = checked_sum<f16>(bias, l);
     // the four waves' sums, brought to the least exponent bias among those that have any
-    if (g == 0) {
-        sh.meet[0][wave][col] = bias;
-        sh.meet[1][wave][col] = l;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l[r] += lane_xor<16>(l[r], lane);
+        l[r] += lane_xor<32>(l[r], lane);
+        l[r] = checked_sum<f16>(bias[r], l[r]);
+        if (g == 0) {
+            sh.meet[0][wave][kFewRows * r + col] = bias[r];
+            sh.meet[1][wave][kFewRows * r + col] = l[r];
+        }
     }
     __syncthreads();  // (and every wave is done with V)
-    float least = INFINITY, total = 0.0f;
+    float least[R], total[R];
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-        if (sh.meet[1][w][col] != 0.0f) least = fminf(least, sh.meet[0][w][col]);
+    for (int r = 0; r < R; ++r) {
+        const int row = kFewRows * r + col;
+        least[r] = INFINITY, total[r] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-        if (sh.meet[1][w][col] != 0.0f) total += sh.meet[1][w][col] * exp2f(least - sh.meet[0][w][col]);
-    const float f = l != 0.0f ? exp2f(least - bias) * unit : 0.0f;
-    if (l != 0.0f) {
+        for (int w = 0; w < 4; ++w)
+            if (sh.meet[1][w][row] != 0.0f) least[r] = fminf(least[r], sh.meet[0][w][row]);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] *= f;
+        for (int w = 0; w < 4; ++w)
+            if (sh.meet[1][w][row] != 0.0f) total[r] += sh.meet[1][w][row] * exp2f(least[r] - sh.meet[0][w][row]);
+        if (l[r] != 0.0f) {
+            const float f = exp2f(least[r] - bias[r]) * unit;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[r][d] *= f;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&sh.o[wave][row][16 * d + 4 * g]) = acc[r][d];
     }
-#pragma unroll
-    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4 *>(&sh.o[wave][col][16 * d + 4 * g]) = acc[d];
     __syncthreads();
-    // thread: row tid / 16, every 16th group of four dimensions
-    const int row = tid >> 4;
-    const int r2 = t.r0 + row, token2 = t.first + r2 / a.group, head2 = kvh * a.group + r2 % a.group;
-    const float total2 = __shfl(total, row), least2 = __shfl(least, row);
-    f32x4 o[D / 64];
-    float z = total2 * 0.0f;
+    // thread: rows tid / 16 of each 16, every 16th group of four dimensions
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-        const int d = 4 * (tid & 15) + 64 * i;
-        o[i] = *reinterpret_cast<f32x4 *>(&sh.o[0][row][d]);
-#pragma unroll
-        for (int w = 1; w < 4; ++w) o[i] += *reinterpret_cast<f32x4 *>(&sh.o[w][row][d]);
-        z = not_finite<4>(o[i], z);
-    }
-    const unsigned long long odd = __ballot(r2 < rows && z != 0.0f);  // 16 lanes a row
-    if (r2 < rows && !(odd >> (lane & 48) & 0xffff)) {
-        const int64_t to = (static_cast<int64_t>(token2) * a.n_heads + head2) * a.parts + blockIdx.y;
-        if (a.parts > 1 && (tid & 15) == 0) a.part_ml[to] = make_float2(least2, total2);
-        const float inv = total2 == 0.0f ? 0.0f : 1.0f / total2;
+    for (int r = 0; r < R; ++r) {
+        const int row = kFewRows * r + (tid >> 4);
+        const int r2 = t.r0 + row, token2 = t.first + r2 / a.group, head2 = kvh * a.group + r2 % a.group;
+        const float total2 = __shfl(total[r], tid >> 4), least2 = __shfl(least[r], tid >> 4);
+        f32x4 o[D / 64];
+        float z = total2 * 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
             const int d = 4 * (tid & 15) + 64 * i;
-            if (a.parts > 1) {
-                *reinterpret_cast<f32x4 *>(a.part_o + to * D + d) = o[i];
-            } else {
-                float x[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
-                store_rounded<T, 4>(static_cast<T *>(a.out) + token2 * a.out_stride + head2 * D + d, x);
+            o[i] = *reinterpret_cast<f32x4 *>(&sh.o[0][row][d]);
+#pragma unroll
+            for (int w = 1; w < 4; ++w) o[i] += *reinterpret_cast<f32x4 *>(&sh.o[w][row][d]);
+            z = not_finite<4>(o[i], z);
+        }
+        const unsigned long long odd = __ballot(r2 < rows && z != 0.0f);  // 16 lanes a row
+        if (r2 < rows && !(odd >> (lane & 48) & 0xffff)) {
+            const int64_t to = (static_cast<int64_t>(token2) * a.n_heads + head2) * a.parts + blockIdx.y;
+            if (a.parts > 1 && (tid & 15) == 0) a.part_ml[to] = make_float2(least2, total2);
+            const float inv = total2 == 0.0f ? 0.0f : 1.0f / total2;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const int d = 4 * (tid & 15) + 64 * i;
+                if (a.parts > 1) {
+                    *reinterpret_cast<f32x4 *>(a.part_o + to * D + d) = o[i];
+                } else {
+                    float x[4] = {o[i][0] * inv, o[i][1] * inv, o[i][2] * inv, o[i][3] * inv};
+                    store_rounded<T, 4>(static_cast<T *>(a.out) + token2 * a.out_stride + head2 * D + d, x);
+                }
             }
         }
-    }
-    if (__builtin_expect(odd == 0, 1)) return;
+        if (__builtin_expect(odd == 0, 1)) continue;
 #pragma unroll 1
-    for (int i = 0; i < 4; ++i)
-        if (odd >> (16 * i) & 0xffff) {
-            const int ro = t.r0 + 4 * wave + i, p = t.pos0 + ro / a.group;
-            formula_row<T, C, D>(a, t.b, ro, t.first, kvh, max(kb, key_lo(a, p)), min(ke, key_hi(a, p, t.len)));
-        }
+        for (int i = 0; i < 4; ++i)
+            if (odd >> (16 * i) & 0xffff) {
+                const int ro = t.r0 + kFewRows * r + 4 * wave + i, p = t.pos0 + ro / a.group;
+                formula_row<T, C, D>(a, t.b, ro, t.first, kvh, max(kb, key_lo(a, p)), min(ke, key_hi(a, p, t.len)));
+            }
+    }
 }
 
 // ---- many rows: tiles of 128 rows ---------------------------------------------------------------
@@ -529,16 +573,23 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
             // which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
             unsigned may = ~0u;
             if (partial) may = (static_cast<unsigned>(exist >> (32 * kt)) >> (4 * h)) & below(hi - k1 - 4 * h) & ~below(lo - k1 - 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 sa = by_of(kScaleA, kt, j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * j + i] *= sa[i];
+            }
+            if (partial) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = -INFINITY;
+            }
             float mx = m;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const f32x4 sa = by_of(kScaleA, kt, j), lg = by_of(kScaleLog, kt, j);
+                const f32x4 lg = by_of(kScaleLog, kt, j);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[4 * j + i] *= sa[i];
-                    if (partial && !(may & (1u << (i + 8 * j)))) s[4 * j + i] = -INFINITY;
-                    mx = fmaxf(mx, fmaf(s[4 * j + i], c, lg[i]));
-                }
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaf(s[4 * j + i], c, lg[i]));
             }
             mx = fmaxf(mx, lane_xor<32>(mx, lane));
             if (__ballot(mx - m > kHeadroom<QT>)) {
@@ -558,8 +609,13 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
                 for (int i = 0; i < 4; ++i) {
                     const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, bias));
                     l += x;
-                    s[4 * j + i] = partial && !(may & (1u << (i + 8 * j))) ? 0.0f : as_fp32(x * b[i]);
+                    s[4 * j + i] = as_fp32(x * b[i]);
                 }
+            }
+            if (partial) {  // (the scale of a masked value may be no number)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = 0.0f;
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -646,8 +702,11 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
 template <typename T, typename C, int D>
 void launch_dim(const AttnArgs &a, const Plan &n, hipStream_t s) {
     const dim3 grid(n.tiles * (a.n_heads / a.group), n.parts);
-    if (n.few)
-        attn8_few<T, C, D><<<grid, 256, 0, s>>>(a);
+    constexpr int kPair = D == 256 && std::is_same_v<T, float> ? 1 : 2;  // (as plan has it)
+    if (n.rows == kFewRows)
+        attn8_few<T, C, D, 1><<<grid, 256, 0, s>>>(a);
+    else if (n.rows == 2 * kFewRows)
+        attn8_few<T, C, D, kPair><<<grid, 256, 0, s>>>(a);
     else
         attn8_tiles<T, C, D><<<grid, 256, 0, s>>>(a);
     launch_join<T, D>(a, n, s);
@@ -681,7 +740,7 @@ int run(const tqhip_attn &p, const tqhip_kv_cache8 &c, const tqhip_seqs &b, hipS
     const int st = check(p, c, b);
     if (st != kOk) return st;
     const tqhip_kv_cache rows = rows_of(c);
-    return run_attn(p, rows, b, plan(p, rows, b), s, [&](AttnArgs a, const Plan &n) {
+    return run_attn(p, rows, b, plan(p, rows, b, true), s, [&](AttnArgs a, const Plan &n) {
         a.scales = reinterpret_cast<const float2 *>(c.scales);
         a.block = FastDiv(static_cast<uint32_t>(c.block));
         a.blocks = c.page_size / c.block;
@@ -709,15 +768,15 @@ int tqhip_paged_attention8_dev(const tqhip_attn *attn, const tqhip_kv_cache8 *ca
 size_t tqhip_paged_attention8_workspace(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs) {
     if (!attn || !cache || !seqs || tqhip::check(*attn, *cache, *seqs) != tqhip::kOk) return 0;
     const tqhip_kv_cache rows = tqhip::rows_of(*cache);
-    return tqhip::plan_bytes(tqhip::plan(*attn, rows, *seqs), *attn, rows, *seqs);
+    return tqhip::plan_bytes(tqhip::plan(*attn, rows, *seqs, true), *attn, rows, *seqs);
 }
 
 int tqhip_paged_attention8_plan(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, int *tile_rows, int *parts) {
     if (!attn || !cache || !seqs || !tile_rows || !parts) return tqhip::kBadShape;
     const int st = tqhip::check(*attn, *cache, *seqs);
     if (st != tqhip::kOk) return st;
-    const tqhip::Plan n = tqhip::plan(*attn, tqhip::rows_of(*cache), *seqs);
-    *tile_rows = n.few ? tqhip::kFewRows : tqhip::kTileRows;
+    const tqhip::Plan n = tqhip::plan(*attn, tqhip::rows_of(*cache), *seqs, true);
+    *tile_rows = n.rows;
     *parts = n.parts;
     return tqhip::kOk;
 }
