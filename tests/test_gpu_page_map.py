@@ -134,6 +134,16 @@ def test_tokens_by_one_launch_or_two(gpu, n_tokens):
         assert dev.read("slots")[n_tokens - 1] == -1 and dev.read("slots")[n_tokens - 2] >= 0
 
 
+@pytest.mark.parametrize("n_seqs", [1, 7, 40])
+def test_long_runs_of_pages(gpu, n_seqs):
+    """Long prompts come, end, and others come into their pages: hundreds of pages of a sequence, given and taken."""
+    rng = np.random.default_rng(n_seqs)
+    lengths = rng.integers(1000, 6000, n_seqs)
+    some = np.where(np.arange(n_seqs) % 3 == 0, lengths, 0)
+    zero = np.zeros(n_seqs, np.int64)
+    steps(gpu, n_seqs, 900, 1000 * n_seqs, 7, [(zero, lengths), (some, lengths - some), (zero, zero), (zero, some), (zero, lengths[::-1]), (zero, zero + 6000)], 6000 * n_seqs)
+
+
 def test_pages_given_back_serve_the_same_call(gpu):
     host, _ = steps(gpu, 3, 8, 8, 4, [([0, 0, 0], [20, 12, 0]), ([0, 12, 0], [0, 0, 20])], 40)
     assert host.n_free == 0 and host.held.tolist() == [0, 3, 5]

@@ -8,12 +8,11 @@
 // A wave takes one block's keys, or its values, of one head: that is where the largest is needed, and no other wave touches
 // the block's codes or scale. Its rows lie side by side as in heads.hip (a head in D / (2 V) lanes), all of them in registers while they
 // fit (32, 16 or 8 fp32 rows of 64, 128 or 256); a larger block is a workgroup's, and one past four times that is read twice.
-// The queries that ride along are a launch of heads.hip's.
+// The queries that ride along are the same launch's, finished as heads.h does it (a launch of their own where something is off the vector path).
 #include <algorithm>
 #include <cmath>
 
-#include "batch.h"
-#include "tq_common.h"
+#include "heads.h"
 
 namespace tqhip {
 namespace {
@@ -92,7 +91,7 @@ __device__ inline unsigned recode(unsigned u, float ratio, int dtype) {
 // D: head dimension; V: elements per load (1: any rotary dimension and alignment); WAVES: of a block's head; KEEP: rounds of rows held in
 // registers, 0: none, they are read and finished twice.
 template <typename T, int D, int V, int WAVES, int KEEP>
-__global__ __launch_bounds__(kAppendThreads) void append8(Append8Args a) {
+__device__ inline void append_block(const Append8Args &a) {
     constexpr int LPR = D / (2 * V) < 64 ? D / (2 * V) : 64, NU = D / (2 * V) / LPR, RPW = 64 / LPR;
     constexpr int kRows = RPW * WAVES;  // of a round
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -291,29 +290,40 @@ __global__ __launch_bounds__(kAppendThreads) void append8(Append8Args a) {
     if (lane == 0 && mine == 0) *scale_at = scale;
 }
 
+// The first `blocks` workgroups take the keys and values, those after them the queries.
 template <typename T, int D, int V, int WAVES, int KEEP>
-int launch_append(const Append8Args &a, hipStream_t s) {
-    const int64_t units = static_cast<int64_t>(a.tiles) * 2 * a.heads, groups = WAVES == 1 ? (units + 3) / 4 : units;
+__global__ __launch_bounds__(kAppendThreads) void append8(Append8Args a, HeadArgs q, int blocks) {
+    if (static_cast<int>(blockIdx.x) < blocks)
+        append_block<T, D, V, WAVES, KEEP>(a);
+    else if constexpr (V > 1)
+        finish_heads<T, T, V, D / (2 * V), true>(q, blockIdx.x - blocks);
+}
+
+// with_q: the queries are this launch's.
+template <typename T, int D, int V, int WAVES, int KEEP>
+int launch_append(const Append8Args &a, HeadArgs q, bool with_q, hipStream_t s) {
+    const int64_t units = static_cast<int64_t>(a.tiles) * 2 * a.heads, blocks = WAVES == 1 ? (units + 3) / 4 : units;
+    const int64_t groups = blocks + (with_q ? plan_heads(q, D / (2 * V)) : 0);
     if (groups > INT32_MAX / kAppendThreads) return kTooLarge;
-    append8<T, D, V, WAVES, KEEP><<<static_cast<unsigned>(groups), kAppendThreads, 0, s>>>(a);
+    append8<T, D, V, WAVES, KEEP><<<static_cast<unsigned>(groups), kAppendThreads, 0, s>>>(a, q, static_cast<int>(blocks));
     return hipGetLastError() == hipSuccess ? kOk : kLaunchFailed;
 }
 
 template <typename T, int D>
-int launch_append_dim(const Append8Args &a, bool wide, hipStream_t s) {
+int launch_append_dim(const Append8Args &a, const HeadArgs &q, bool with_q, bool wide, hipStream_t s) {
     constexpr int V = 16 / sizeof(T), kRound = 64 / (D / (2 * V));
-    if (!wide) return launch_append<T, D, 1, 4, 0>(a, s);
+    if (!wide) return launch_append<T, D, 1, 4, 0>(a, q, false, s);
     const int block = static_cast<int>(a.block.d);
-    if (block <= 4 * kRound) return launch_append<T, D, V, 1, 4>(a, s);
-    if (block <= 16 * kRound) return launch_append<T, D, V, 4, 4>(a, s);
-    return launch_append<T, D, V, 4, 0>(a, s);
+    if (block <= 4 * kRound) return launch_append<T, D, V, 1, 4>(a, q, with_q, s);
+    if (block <= 16 * kRound) return launch_append<T, D, V, 4, 4>(a, q, with_q, s);
+    return launch_append<T, D, V, 4, 0>(a, q, with_q, s);
 }
 
 template <typename T>
-int launch_append_type(const Append8Args &a, int D, bool wide, hipStream_t s) {
-    if (D == 64) return launch_append_dim<T, 64>(a, wide, s);
-    if (D == 128) return launch_append_dim<T, 128>(a, wide, s);
-    return launch_append_dim<T, 256>(a, wide, s);
+int launch_append_type(const Append8Args &a, const HeadArgs &q, bool with_q, int D, bool wide, hipStream_t s) {
+    if (D == 64) return launch_append_dim<T, 64>(a, q, with_q, wide, s);
+    if (D == 128) return launch_append_dim<T, 128>(a, q, with_q, wide, s);
+    return launch_append_dim<T, 256>(a, q, with_q, wide, s);
 }
 
 int run_append8(const tqhip_head_proj &p, const tqhip_kv_cache8 &c, const tqhip_seqs &b, hipStream_t s) {
@@ -333,7 +343,7 @@ int run_append8(const tqhip_head_proj &p, const tqhip_kv_cache8 &c, const tqhip_
                   p.eps, p.rotary_dim && !p.inv_freq ? std::log2(p.theta) : 0.0, p.inv_freq, p.positions, b.q_start, b.kv_len, b.n_seqs,
                   make_pages(rows, b), FastDiv(static_cast<uint32_t>(c.block)), c.page_size / c.block};
     const int64_t tiles = b.n_tokens / c.block + int64_t{2} * b.n_seqs;
-    if (tiles > INT32_MAX / 2) return kTooLarge;
+    if (2 * tiles * p.n_kv_heads > INT32_MAX / kAppendThreads) return kTooLarge;  // (of any form: nothing is launched before that is known)
     a.tiles = static_cast<int>(tiles);
     if (p.n_tokens > 1 && (a.in_stride[0] < row || a.in_stride[1] < row)) return kBadShape;
     // codes are written, and written again, 16 bytes at a time
@@ -343,11 +353,15 @@ int run_append8(const tqhip_head_proj &p, const tqhip_kv_cache8 &c, const tqhip_
     bool wide = p.rotary_dim % (2 * v) == 0;
     for (int i = 0; i < 2; ++i) wide = wide && !apart(a.in[i], a.in_stride[i] * bytes);
     for (const float *f : {p.k_bias, p.v_bias, p.k_norm}) wide = wide && !apart(f, 0);
-    if (p.q && (st = finish_queries(p, rows, b, s)) != kOk) return st;
+    const HeadArgs q = query_args(p, rows, b);
+    const int64_t q_row = static_cast<int64_t>(p.n_heads) * D;
+    if (p.q && p.n_tokens > 1 && (q.in_stride[0] < q_row || q.out_stride[0] < q_row)) return kBadShape;
+    const bool with_q = p.q && wide && wide_queries(p, q);
+    if (p.q && !with_q && (st = finish_queries(p, rows, b, s)) != kOk) return st;
     switch (p.dtype) {
-        case TQHIP_F32: return launch_append_type<float>(a, D, wide, s);
-        case TQHIP_F16: return launch_append_type<f16>(a, D, wide, s);
-        default: return launch_append_type<bf16>(a, D, wide, s);
+        case TQHIP_F32: return launch_append_type<float>(a, q, with_q, D, wide, s);
+        case TQHIP_F16: return launch_append_type<f16>(a, q, with_q, D, wide, s);
+        default: return launch_append_type<bf16>(a, q, with_q, D, wide, s);
     }
 }
 
