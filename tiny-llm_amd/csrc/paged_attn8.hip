@@ -426,6 +426,7 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
         int64_t offs[2][256];           // offsets of the rows of 256 keys, several tiles, and of the next 256
         int scale[2][256];              // places of their scales
         unsigned long long here[2][4];  // which of those keys exist
+        unsigned one[2][8];             // groups of 32 of those keys that share their scales: all ones
         unsigned long long wild[3];     // keys of a partly masked tile that have NaN codes
         float unit;
     } sh;
@@ -529,6 +530,9 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
         sh.offs[n & 1][tid] = max(o, int64_t{0});
         sh.scale[n & 1][tid] = o < 0 ? kvh * a.blocks : (page * kv_heads + kvh) * a.blocks + a.block.quot(row);
         if (lane == 0) sh.here[n & 1][wave] = m;
+        const int place = sh.scale[n & 1][tid], first = __shfl(place, lane & 32);
+        const unsigned long long same = __ballot(place == first);
+        if ((lane & 31) == 0) sh.one[n & 1][tid / 32] = static_cast<unsigned>(same >> (lane & 32));
     };
 
     f32x16 acc[ND];
@@ -570,28 +574,39 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt) {
             const int k1 = k0 + 32 * kt;
-            // which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
+            // Keys of one scale that all count: their scores' factor is c a, and b goes into the weights' exponent, and out of their sum.
+            const float a0 = sh.by[buf][kScaleA][32 * kt], b0 = sh.by[buf][kScaleB][32 * kt], lg0 = sh.by[buf][kScaleLog][32 * kt];
+            const bool one = __builtin_amdgcn_readfirstlane(!partial && sh.one[n / kTiles & 1][n % kTiles * NK + kt] == ~0u && a0 >= 0.0f && b0 > 0.0f);
+            // else: which of the lane's keys its row may attend to: bit (i % 4) + 8 (i / 4) for register i
             unsigned may = ~0u;
             if (partial) may = (static_cast<unsigned>(exist >> (32 * kt)) >> (4 * h)) & below(hi - k1 - 4 * h) & ~below(lo - k1 - 4 * h);
+            float mx;
+            if (one) {
+                mx = s[0];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 sa = by_of(kScaleA, kt, j);
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+                mx = fmaf(mx, c * a0, lg0);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[4 * j + i] *= sa[i];
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 sa = by_of(kScaleA, kt, j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[4 * j + i] *= sa[i];
+                }
+                if (partial) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = -INFINITY;
+                }
+                mx = m;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 lg = by_of(kScaleLog, kt, j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaf(s[4 * j + i], c, lg[i]));
+                }
             }
-            if (partial) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = -INFINITY;
-            }
-            float mx = m;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 lg = by_of(kScaleLog, kt, j);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaf(s[4 * j + i], c, lg[i]));
-            }
-            mx = fmaxf(mx, lane_xor<32>(mx, lane));
+            mx = fmaxf(m, fmaxf(mx, lane_xor<32>(mx, lane)));
             if (__ballot(mx - m > kHeadroom<QT>)) {
                 const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, QT> - mx;
                 const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
@@ -602,20 +617,31 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
                 for (int i = 0; i < ND; ++i) acc[i] *= f;
             }
             if (kt + 1 < NK) ahead = scores(kt + 1);
+            if (one) {
+                const float ca = c * a0, from = bias + lg0;
+                float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 b = by_of(kScaleB, kt, j);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, bias));
-                    l += x;
-                    s[4 * j + i] = as_fp32(x * b[i]);
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], ca, from));
+                    sum += s[i];
                 }
-            }
-            if (partial) {  // (the scale of a masked value may be no number)
+                l = fmaf(sum, __builtin_amdgcn_rcpf(b0), l);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = 0.0f;
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 b = by_of(kScaleB, kt, j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], c, bias));
+                        l += x;
+                        s[4 * j + i] = as_fp32(x * b[i]);
+                    }
+                }
+                if (partial) {  // (the scale of a masked value may be no number)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!(may & (1u << ((i & 3) + 8 * (i >> 2))))) s[i] = 0.0f;
+                }
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
