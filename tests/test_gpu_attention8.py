@@ -86,6 +86,12 @@ def test_forms(gpu, act, dtype, new, kv, Hq, Hk):
     check(gpu, b, act, Hq)
 
 
+@pytest.mark.parametrize("act,dtype", TYPES)
+@pytest.mark.parametrize("new,kv,Hq,Hk,D", [([9, 20], [100, 1500], 4, 2, 256), ([300, 170], [700, 200], 4, 2, 256), ([200, 230], [3000, 300], 4, 2, 256), ([300, 170], [700, 200], 6, 2, 64)])
+def test_chunks_of_wide_and_narrow_heads(gpu, act, dtype, new, kv, Hq, Hk, D):
+    check(gpu, Batch8(gpu, new, kv, 64, Hk, D, dtype, 32, seed=3, spread=2), act, Hq)
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1], [33, 1, 3], [150, 200, 90]])
 @pytest.mark.parametrize("page,block", [(1, 1), (7, 7), (40, 5), (64, 1), (1000, 125), (96, 3)])
 def test_page_and_block_sizes(gpu, page, block, new):

@@ -17,7 +17,7 @@ namespace tqhip {
 namespace {
 
 constexpr int kMapThreads = 1024;
-constexpr int kAtOnce = 8, kLongRun = 16;
+constexpr int kAtOnce = 16, kLongRun = 16;
 constexpr int kMapSeqs = 4096;  // (their prefix sums are in LDS)
 
 struct MapArgs {
