@@ -7,7 +7,7 @@
 // Taking may take what has just been given, so the two are phases of one workgroup with a barrier between them.
 //
 // Nothing here is work: it is latency, a few dependent loads and the scans. 256 requests, a token each: 10 us (as much with a workgroup of 256); 48
-// prompts' 830000 tokens and 53000 pages: 17 us, and 6 to 7 for the tokens, which are a launch of their own past 4096.
+// prompts' 830000 tokens and 53000 pages: 16 us, and 6 to 7 for the tokens, which are a launch of their own past 4096.
 #include <algorithm>
 
 #include "batch.h"

@@ -487,9 +487,13 @@ inline Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs 
     // 128: 16 rows 140 us, against 182 with tiles of 128; 32 rows 195 and 189; 64 rows 294 and 223), and, whatever the rows, as long
     // as there are few of them in all, because there they come in shorter parts (one sequence of 64 rows on 8 K/V heads 22 us and 32,
     // 128 rows 34 and 34; 448 rows on 2 heads of 64 30 and 41, 1792 rows 79 and 47; 1024 on one of 256 52 and 81).
-    n.few = rows <= int64_t{2} * kFewRows * s.n_seqs || (rows + kFewRows - 1) / kFewRows * c.n_kv_heads <= 56;
-    // Over codes of 8 bits, 32 rows a tile where sequences have more than 16, so that their keys are read once: five tokens each of 32 sequences of up to 9000
-    // keys, 20 rows a head: FEW32. (Heads of 256 with fp32 terms for two of them do not fit the registers.)
+    // Codes of 8 bits win there for twice the rows, of a sequence (32 sequences of up to 9000 keys, 32 heads of 128 over 8: 45 rows of
+    // bf16 154 us, against 180 with tiles of 128; 35 of fp32 170 and 237; but 87 of fp32 342 and 268) and in all (one of 512 rows on 8
+    // heads of 128 24.9 and 31.3; 2400 on one of 256 54 and 76).
+    const int more = codes ? 2 : 1;
+    n.few = rows <= int64_t{2 * more} * kFewRows * s.n_seqs || (rows + kFewRows - 1) / kFewRows * c.n_kv_heads <= 56 * more;
+    // Over codes, 32 rows a tile where sequences have more than 16, so that their keys are read once: five tokens each of 32 sequences of
+    // up to 9000 keys, 20 rows a head: 101 us, against 118 with tiles of 16. (Heads of 256 with fp32 terms do not fit the registers twice.)
     const bool pairs = codes && !(c.head_dim == 256 && p.dtype == TQHIP_F32);
     n.rows = !n.few ? kTileRows : pairs && rows > int64_t{kFewRows} * s.n_seqs ? 2 * kFewRows : kFewRows;
     n.tiles = static_cast<int>(rows / n.rows) + s.n_seqs;
