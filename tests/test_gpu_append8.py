@@ -69,7 +69,8 @@ def same_codes(b, want):
 
 # Pages and blocks (rows of a block in a wave's registers, in a workgroup's, read twice; odd ones), heads, layouts.
 FORMS = [(16, 16, 2, 64, "token"), (48, 24, 2, 64, "head"), (64, 64, 1, 128, "token"), (128, 128, 1, 256, "token"), (200, 200, 1, 64, "head"), (300, 300, 1, 128, "token"),
-         (7, 7, 3, 128, "token"), (6, 1, 2, 64, "token"), (30, 10, 8, 128, "head"), (20, 5, 1, 256, "token")]
+         (7, 7, 3, 128, "token"), (6, 1, 2, 64, "token"), (30, 10, 8, 128, "head"), (20, 5, 1, 256, "token"),
+         (12, 1, 5, 128, "head"), (12, 2, 3, 64, "token"), (9, 3, 9, 64, "head"), (8, 4, 4, 128, "token"), (5, 1, 8, 256, "token")]  # (several heads a wave)
 
 
 @pytest.mark.parametrize("dtype", [I8, E4M3])
@@ -93,7 +94,7 @@ def test_codes_and_scales_to_the_bit(gpu, page, block, Hk, D, layout, act, dtype
 
 
 @pytest.mark.parametrize("dtype", [I8, E4M3])
-@pytest.mark.parametrize("page,block,D", [(16, 16, 64), (32, 8, 128), (150, 150, 64), (24, 12, 256)])
+@pytest.mark.parametrize("page,block,D", [(16, 16, 64), (32, 8, 128), (150, 150, 64), (24, 12, 256), (12, 3, 64), (16, 4, 128)])
 def test_token_by_token(gpu, page, block, D, dtype):
     """Tokens of growing, shrinking and zero size, one or a few at a time: a block's scale only grows until it is begun anew, after lengths
     have gone back (refused drafts) too."""
@@ -130,7 +131,8 @@ def test_token_by_token(gpu, page, block, D, dtype):
 @pytest.mark.parametrize("dtype", [I8, E4M3])
 @pytest.mark.parametrize("act", [F32, F16, BF16])
 @pytest.mark.parametrize("Hq,Hk,D,page,block,rotary,packed", [(14, 2, 64, 48, 24, 64, True), (8, 2, 128, 16, 16, 128, False), (2, 1, 256, 64, 64, 64, False),
-                                                              (3, 1, 64, 40, 40, 6, False), (2, 2, 128, 512, 512, 128, False), (2, 1, 256, 6, 3, 0, True)])
+                                                              (3, 1, 64, 40, 40, 6, False), (2, 2, 128, 512, 512, 128, False), (2, 1, 256, 6, 3, 0, True), (6, 3, 64, 8, 2, 64, True),
+                                                              (5, 5, 128, 8, 1, 64, False)])
 def test_finished_heads(gpu, Hq, Hk, D, page, block, rotary, packed, act, dtype):
     new, kv = [5, 1, 0, 40, 3, 1], [5, 100, 33, 90, 2, 2 * page + 1]
     b = Batch8(gpu, new, kv, page, Hk, D, dtype, block, seed=3, tail=2, lead=1)
@@ -168,7 +170,7 @@ def test_finished_heads(gpu, Hq, Hk, D, page, block, rotary, packed, act, dtype)
 
 
 @pytest.mark.parametrize("dtype", [I8, E4M3])
-@pytest.mark.parametrize("block", [8, 64])
+@pytest.mark.parametrize("block", [1, 4, 8, 64])
 def test_infinities_and_nan(gpu, block, dtype):
     """Such an element makes its block and head NaN, K or V alone, until the block is begun anew; other blocks and heads do not notice."""
     page = 64

@@ -7,7 +7,8 @@
 //
 // A wave takes one block's keys, or its values, of one head: that is where the largest is needed, and no other wave touches
 // the block's codes or scale. Its rows lie side by side as in heads.hip (a head in D / (2 V) lanes), all of them in registers while they
-// fit (32, 16 or 8 fp32 rows of 64, 128 or 256); a larger block is a workgroup's, and one past four times that is read twice.
+// fit (32, 16 or 8 fp32 rows of 64, 128 or 256); a larger block is a workgroup's, and one past four times that is read twice. Of blocks of
+// few rows it takes several heads side by side.
 // Bytes moved are the bound of a long batch, latency (sequence, page, rows, the block's scale) that of a short one. 12520 tokens of 14 + 2 + 2
 // heads of 64, 106 MB: 23 to 26 us, 4.1 to 4.6 TB/s, a copy's rate; 61 single tokens: 7 to 8.5 us, 14 of the caller's.
 // The queries that ride along are the same launch's, finished as heads.h does it (a launch of their own where something is off the vector path).
@@ -29,6 +30,7 @@ struct Append8Args {
     unsigned char *cache[2];
     float *scales;
     int n_tokens, heads, rot, dtype, tiles;
+    int side;  // heads that a wave takes side by side (a power of two), where KEEP is 1
     float eps;
     double log2_theta;
     const float *inv_freq;
@@ -91,21 +93,22 @@ __device__ inline unsigned recode(unsigned u, float ratio, int dtype) {
 }
 
 // D: head dimension; V: elements per load (1: any rotary dimension and alignment); WAVES: of a block's head; KEEP: rounds of rows held in
-// registers, 0: none, they are read and finished twice.
+// registers, 0: none, they are read and finished twice; 1: the wave's rows are those of `side` heads.
 template <typename T, int D, int V, int WAVES, int KEEP>
 __device__ inline void append_block(const Append8Args &a) {
     constexpr int LPR = D / (2 * V) < 64 ? D / (2 * V) : 64, NU = D / (2 * V) / LPR, RPW = 64 / LPR;
-    constexpr int kRows = RPW * WAVES;  // of a round
+    const int side = KEEP == 1 ? a.side : 1, per = RPW / side, kRows = per * WAVES;  // rows of a head in the wave, and in a round
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int unit = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x, mine = WAVES == 1 ? 0 : wave;
-    const int heads2 = 2 * a.heads, tile = unit / heads2, kv = unit % heads2 / a.heads, h = unit % a.heads;
+    const int sub = lane / LPR, row_lane = sub % per;
+    const int times = (a.heads + side - 1) / side, tile = unit / (2 * times), kv = unit % (2 * times) / times;
+    const int head = unit % times * side + (KEEP == 1 ? sub / per : 0), h = min(head, a.heads - 1);
     NewRows r;
     if (tile >= a.tiles || !find_block(a, tile, r)) return;
     const int page = page_number(a.pages, r.b, r.pos0);
     const int64_t row0 = row_in_page(a.pages, page, r.pos0);
     if (row0 < 0) return;
     const int n = r.pos1 - r.pos0, half = a.rot / 2;
-    const int sub = lane / LPR;
 
     int at0[NU], at1[NU];
     bool turned[NU];
@@ -138,7 +141,7 @@ __device__ inline void append_block(const Append8Args &a) {
         vec<T, V> x0[NU], x1[NU];
     };
     // the row of a round that the lane has part in (past the last: the last again)
-    const auto row_of = [&](int round) { return min(round * kRows + mine * RPW + sub, n - 1); };
+    const auto row_of = [&](int round) { return min(round * kRows + mine * per + row_lane, n - 1); };
     const auto load = [&](int round, Raw &x) {
         const T *src = in + static_cast<int64_t>(r.token0 + row_of(round)) * a.in_stride[kv];
 #pragma unroll
@@ -199,8 +202,8 @@ __device__ inline void append_block(const Append8Args &a) {
     };
     unsigned char *cache = a.cache[kv] + h * a.pages.head_stride;
     const auto store = [&](int round, const Row &x, float scale, bool bad) {
-        const int i = round * kRows + mine * RPW + sub;
-        if (i >= n) return;
+        const int i = round * kRows + mine * per + row_lane;
+        if (i >= n || (KEEP == 1 && head != h)) return;
         unsigned char *dst = cache + row0 + i * a.pages.token_stride;
 #pragma unroll
         for (int j = 0; j < NU; ++j) {
@@ -252,7 +255,8 @@ __device__ inline void append_block(const Append8Args &a) {
         }
     }
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), d)));
+    for (int d = 1; d < 64; d *= 2)
+        if (KEEP != 1 || d < LPR * per) top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), d)));
     if constexpr (WAVES > 1) {
         __shared__ unsigned top_of[WAVES];
         if (lane == 0) top_of[wave] = top;
@@ -264,13 +268,14 @@ __device__ inline void append_block(const Append8Args &a) {
     if (older > 0 && !(old <= scale)) scale = old;  // (larger, or NaN)
     if (top >= 0x7f800000u) scale = NAN;
     const bool bad = !(scale < INFINITY);
-    if (older > 0 && scale != old && !bad) {
+    if (older > 0 && scale != old && !bad && (KEEP != 1 || head == h)) {
         // 16 codes a lane
         const float ratio = old / scale;
-        constexpr int LANES = D / 16, kOld = 64 / LANES * WAVES;
+        constexpr int LANES = D / 16;
+        const int lanes = KEEP == 1 ? LPR * per : 64, of = lane % lanes, rows = lanes / LANES;  // (of a head)
         unsigned char *from = cache + row0 - static_cast<int64_t>(older) * a.pages.token_stride;
-        for (int i = mine * (64 / LANES) + lane / LANES; i < older; i += kOld) {
-            vec<unsigned, 4> *p = reinterpret_cast<vec<unsigned, 4> *>(from + i * a.pages.token_stride + lane % LANES * 16);
+        for (int i = mine * rows + of / LANES; i < older; i += rows * WAVES) {
+            vec<unsigned, 4> *p = reinterpret_cast<vec<unsigned, 4> *>(from + i * a.pages.token_stride + of % LANES * 16);
             vec<unsigned, 4> u = *p;
 #pragma unroll
             for (int w = 0; w < 4; ++w) u[w] = recode(u[w], ratio, a.dtype);
@@ -289,7 +294,7 @@ __device__ inline void append_block(const Append8Args &a) {
             store(i, x[0], scale, bad);
         }
     }
-    if (lane == 0 && mine == 0) *scale_at = scale;
+    if (lane % LPR == 0 && row_lane == 0 && mine == 0 && (KEEP != 1 || head == h)) *scale_at = scale;
 }
 
 // The first `blocks` workgroups take the keys and values, those after them the queries.
@@ -304,7 +309,8 @@ __global__ __launch_bounds__(kAppendThreads) void append8(Append8Args a, HeadArg
 // with_q: the queries are this launch's.
 template <typename T, int D, int V, int WAVES, int KEEP>
 int launch_append(const Append8Args &a, HeadArgs q, bool with_q, hipStream_t s) {
-    const int64_t units = static_cast<int64_t>(a.tiles) * 2 * a.heads, blocks = WAVES == 1 ? (units + 3) / 4 : units;
+    const int side = KEEP == 1 ? a.side : 1;
+    const int64_t units = static_cast<int64_t>(a.tiles) * 2 * ((a.heads + side - 1) / side), blocks = WAVES == 1 ? (units + 3) / 4 : units;
     const int64_t groups = blocks + (with_q ? plan_heads(q, D / (2 * V)) : 0);
     if (groups > INT32_MAX / kAppendThreads) return kTooLarge;
     append8<T, D, V, WAVES, KEEP><<<static_cast<unsigned>(groups), kAppendThreads, 0, s>>>(a, q, static_cast<int>(blocks));
@@ -312,10 +318,14 @@ int launch_append(const Append8Args &a, HeadArgs q, bool with_q, hipStream_t s) 
 }
 
 template <typename T, int D>
-int launch_append_dim(const Append8Args &a, const HeadArgs &q, bool with_q, bool wide, hipStream_t s) {
+int launch_append_dim(Append8Args a, const HeadArgs &q, bool with_q, bool wide, hipStream_t s) {
     constexpr int V = 16 / sizeof(T), kRound = 64 / (D / (2 * V));
     if (!wide) return launch_append<T, D, 1, 4, 0>(a, q, false, s);
     const int block = static_cast<int>(a.block.d);
+    // Blocks that leave lanes without a row, several heads a wave (8500 tokens of 32 + 8 heads of 128 in blocks of one: bf16 56 us, against 340
+    // with a head a wave, fp32 92 and 207; of two 54 and 184, of four 59 and 107; of sixteen, which fill the lanes, 58).
+    while (2 * a.side * block <= kRound && a.side < a.heads) a.side *= 2;
+    if (a.side > 1) return launch_append<T, D, V, 1, 1>(a, q, with_q, s);
     if (block <= 4 * kRound) return launch_append<T, D, V, 1, 4>(a, q, with_q, s);
     if (block <= 16 * kRound) return launch_append<T, D, V, 4, 4>(a, q, with_q, s);
     return launch_append<T, D, V, 4, 0>(a, q, with_q, s);
@@ -341,7 +351,7 @@ int run_append8(const tqhip_head_proj &p, const tqhip_kv_cache8 &c, const tqhip_
     if (D != 64 && D != 128 && D != 256) return kBadShape;
     const int64_t row = static_cast<int64_t>(p.n_kv_heads) * D;
     Append8Args a{{p.k, p.v}, {p.k_stride ? p.k_stride : row, p.v_stride ? p.v_stride : row}, {p.k_bias, p.v_bias}, p.k_norm,
-                  {static_cast<unsigned char *>(c.k), static_cast<unsigned char *>(c.v)}, c.scales, p.n_tokens, p.n_kv_heads, p.rotary_dim, c.dtype, 0,
+                  {static_cast<unsigned char *>(c.k), static_cast<unsigned char *>(c.v)}, c.scales, p.n_tokens, p.n_kv_heads, p.rotary_dim, c.dtype, 0, 1,
                   p.eps, p.rotary_dim && !p.inv_freq ? std::log2(p.theta) : 0.0, p.inv_freq, p.positions, b.q_start, b.kv_len, b.n_seqs,
                   make_pages(rows, b), FastDiv(static_cast<uint32_t>(c.block)), c.page_size / c.block};
     const int64_t tiles = b.n_tokens / c.block + int64_t{2} * b.n_seqs;
