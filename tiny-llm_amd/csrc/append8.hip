@@ -322,7 +322,7 @@ int launch_append_dim(Append8Args a, const HeadArgs &q, bool with_q, bool wide, 
     constexpr int V = 16 / sizeof(T), kRound = 64 / (D / (2 * V));
     if (!wide) return launch_append<T, D, 1, 4, 0>(a, q, false, s);
     const int block = static_cast<int>(a.block.d);
-    // Blocks that leave lanes without a row, several heads a wave (8500 tokens of 32 + 8 heads of 128 in blocks of one: bf16 56 us, against 340
+    // Blocks that leave lanes without a row, several heads a wave (7600 tokens of 32 + 8 heads of 128 in blocks of one: bf16 56 us, against 340
     // with a head a wave, fp32 92 and 207; of two 54 and 184, of four 59 and 107; of sixteen, which fill the lanes, 58).
     while (2 * a.side * block <= kRound && a.side < a.heads) a.side *= 2;
     if (a.side > 1) return launch_append<T, D, V, 1, 1>(a, q, with_q, s);

@@ -9,12 +9,12 @@
 //
 // The cut into tiles of 16, 32 and 128 rows, the parts and their join are those of the other caches (paged_attn.h, paged_attn.hip).
 // Few rows are bound by HBM: a key and a value of D bytes and their scales, read once for the rows of a K/V head. Many rows are bound by
-// the vector units, which make fp16 of the codes and weights of the scores while the matrix units wait (busy 24 % and 55 % of the time).
+// the vector units, which make fp16 of the codes and weights of the scores while the matrix units wait (busy 31 % and 45 % of the time).
 //   64 single tokens over up to 16000 i8 keys, 32 heads of 128 over 8 (1.04 GB)     220 us, 4.7 TB/s (f16 keys 390)
 //   32 sequences of 5 tokens over up to 9000 e4m3 keys, the same heads (316 MB)       93 us, 3.4 TB/s
 //   one token over 3000 keys, 14 heads of 64 over 2                                  13 us, 8 and 3.5 of them kernels
-//   752 fp32 tokens over up to 8000 i8 keys, 32 on 8 heads of 128 (72 GFLOP, twice that with two terms)  213 us
-//   12577 bf16 tokens of prompts, e4m3, the same heads (707 GFLOP)                  925 us, 764 TFLOP/s
+//   752 fp32 tokens over up to 8000 i8 keys, 32 on 8 heads of 128 (72 GFLOP, twice that with two terms)  211 us
+//   12577 bf16 tokens of prompts, e4m3, the same heads (707 GFLOP)                  915 us, 773 TFLOP/s
 #include "paged_attn.h"
 
 namespace tqhip {
@@ -473,9 +473,10 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
                                                    [&](float x) { return fmaxf(x, lane_xor<32>(x, lane)); });
     const unsigned char *kc = static_cast<const unsigned char *>(a.k) + kvh * a.pages.head_stride;
     const unsigned char *vc = static_cast<const unsigned char *>(a.v) + kvh * a.pages.head_stride;
-    // of a row's chunks of 8 elements (16 bytes), so that the reads below meet every bank once
-    const auto key_swap = [](int row) { return (D == 64 ? row >> 1 : row) & (D == 64 ? 7 : 15); };
-    const auto value_swap = [](int row) { return (row & 3) << (D == 64 ? 1 : 2); };
+    // Places of a row's chunks of 8 elements (16 bytes), so that the reads below meet every bank once, and the writes, of every other
+    // chunk of a row or two by 8 lanes, every second chunk's banks and the ones between (1 % of the time for prompts).
+    const auto key_at = [](int row, int ch) { return (D == 64 ? ch ^ (row >> 1 & 7) ^ (row & 1) : ch ^ (ch >> 3 & 1) ^ (row & 15)) * 8; };
+    const auto value_at = [](int row, int ch) { return (D == 64 ? ch ^ (row & 3) << 1 ^ (row & 1) : ch ^ (ch >> 3 & 1) ^ (row & 3) << 2) * 8; };
     vec<unsigned, 4> kr[NCH], vr[NCH];
     float2 by;
     // A tile's codes and scales on their way into registers. For a key that does not exist row 0 of page 0 is loaded.
@@ -513,8 +514,8 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
             const int ch = tid + 256 * i, row = ch / CH, at = ch % CH * 2;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                *reinterpret_cast<vec<f16, 8> *>(&sh.k[buf][row][((at + e) ^ key_swap(row)) * 8]) = as_halves<C>(kr[i][2 * e], kr[i][2 * e + 1]);
-                *reinterpret_cast<vec<f16, 8> *>(&sh.v[buf][row][((at + e) ^ value_swap(row)) * 8]) = as_halves<C>(vr[i][2 * e], vr[i][2 * e + 1]);
+                *reinterpret_cast<vec<f16, 8> *>(&sh.k[buf][row][key_at(row, at + e)]) = as_halves<C>(kr[i][2 * e], kr[i][2 * e + 1]);
+                *reinterpret_cast<vec<f16, 8> *>(&sh.v[buf][row][value_at(row, at + e)]) = as_halves<C>(vr[i][2 * e], vr[i][2 * e + 1]);
             }
         }
         if (tid < BN) {
@@ -570,7 +571,7 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
             f32x16 s{};
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                const vec<f16, 8> kf = *reinterpret_cast<const vec<f16, 8> *>(&sh.k[buf][32 * kt + col][((2 * i + h) ^ key_swap(col)) * 8]);
+                const vec<f16, 8> kf = *reinterpret_cast<const vec<f16, 8> *>(&sh.k[buf][32 * kt + col][key_at(col, 2 * i + h)]);
 #pragma unroll
                 for (int qi = 0; qi < QT; ++qi) s = mfma32(kf, q[qi][i], s);
             }
@@ -660,8 +661,7 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const int i = lane & 15, row = 32 * kt + 16 * half + 4 * h + i / 4;
-                    const int ch = (4 * d + (lane & 16) / 8 + (i & 3) / 2) ^ value_swap(i / 4);
-                    const f16 *v0 = &sh.v[buf][row][ch * 8 + 4 * (i & 1)];
+                    const f16 *v0 = &sh.v[buf][row][value_at(i / 4, 4 * d + (lane & 16) / 8 + (i & 3) / 2) + 4 * (i & 1)];
                     const vec<f16, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * D);
                     const vec<f16, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
