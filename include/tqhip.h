@@ -335,6 +335,7 @@ int tqhip_kv_append8_dev(const tqhip_head_proj *proj, const tqhip_kv_cache8 *cac
  * such product where that is more. What is said there of infinities and NaN holds for elements: codes times scales. */
 int tqhip_paged_attention8_dev(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, void *stream);
 size_t tqhip_paged_attention8_workspace(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs);
+/* (tiles of 16, 32 or 128 rows) */
 int tqhip_paged_attention8_plan(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, int *tile_rows, int *parts);
 
 /* The pages of a batch from the lengths of its requests, without the host: sequence b is to have past[b] + n_new[b] cached
@@ -372,7 +373,8 @@ int tqhip_page_map_dev(const tqhip_page_map *map, void *stream);
  * out_tokens: from q_start[b] on the accepted drafts and the token drawn, n_out[b] in all, then -1. logprob: log p of each (T of 0: as of 1), then 0.
  * past: kv_len[b] less the refused drafts, the cached positions that stay. Logits of minus infinity have probability 0; a row with NaN or plus infinity, or
  * with nothing else, has no probabilities: as a target it ends its sequence with a token of -1, which n_out counts, as a draft it refuses,
- * and the draw is from p. Tokens of no sequence keep their outputs. vocab up to 2^22.
+ * and the draw is from p. Tokens of no sequence keep their outputs. out_tokens and logprob share nothing with
+ * tokens and accept (refused). vocab up to 2^22.
  * workspace: as for the attention, tqhip_verify_tokens_workspace() bytes. */
 typedef struct tqhip_verify {
     int dtype;                       /* of logits and draft: TQHIP_F32 / F16 / BF16 */

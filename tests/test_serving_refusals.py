@@ -29,13 +29,14 @@ def test_null_structs(tqa):
 
 def verify(tqa, **kw):
     d = dict(dtype=F32, n_seqs=2, n_tokens=3, vocab=100, logits=AT, draft=AT, q_start=AT, tokens=AT, temperature=AT, accept=AT, pick=AT, kv_len=AT,
-             past=AT, out_tokens=AT, n_out=AT, logprob=AT)
+             past=AT, out_tokens=2 * AT, n_out=AT, logprob=2 * AT)
     return tqa.lib().tqhip_verify_tokens_dev(tqa.Verify(**{**d, **kw}), None)
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(n_seqs=0), dict(n_tokens=0), dict(vocab=0), dict(logits_stride=99), dict(draft_stride=-100),
                                 dict(kv_len=None), dict(logits=AT + 2), dict(dtype=F16, draft=AT + 1), dict(workspace=AT + 16, workspace_bytes=1 << 30)] +
-                         [{n: None} for n in ("logits", "q_start", "tokens", "accept", "pick", "out_tokens", "n_out")])
+                         [{n: None} for n in ("logits", "q_start", "tokens", "accept", "pick", "out_tokens", "n_out")] +
+                         [dict(out_tokens=AT), dict(out_tokens=AT + 8), dict(logprob=AT - 8), dict(tokens=2 * AT), dict(accept=2 * AT, logprob=None)])
 def test_verify_refuses(tqa, kw):
     assert verify(tqa, **kw) == -1
 

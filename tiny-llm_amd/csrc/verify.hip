@@ -482,6 +482,13 @@ int check_verify(const tqhip_verify &p) {
     const int64_t chunks = chunks_of(p);
     // (a launch has less than 2^32 threads along x)
     if (chunks * std::max(p.n_tokens, p.n_seqs) > INT32_MAX / kRowThreads || p.n_seqs > INT32_MAX / kDrawThreads) return kTooLarge;
+    // a sequence's workgroups read its tokens and numbers while the first of them writes
+    const auto meet = [&](const void *in, const void *out) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(in), y = reinterpret_cast<uintptr_t>(out);
+        return out && (x < y ? y - x : x - y) < 4 * static_cast<uintptr_t>(p.n_tokens);
+    };
+    for (const void *in : {static_cast<const void *>(p.tokens), static_cast<const void *>(p.accept)})
+        if (meet(in, p.out_tokens) || meet(in, p.logprob)) return kBadShape;
     return kOk;
 }
 
