@@ -323,9 +323,12 @@ int launch_append_dim(Append8Args a, const HeadArgs &q, bool with_q, bool wide, 
     if (!wide) return launch_append<T, D, 1, 4, 0>(a, q, false, s);
     const int block = static_cast<int>(a.block.d);
     // Blocks that leave lanes without a row, several heads a wave (7600 tokens of 32 + 8 heads of 128 in blocks of one: bf16 56 us, against 340
-    // with a head a wave, fp32 92 and 207; of two 54 and 184, of four 59 and 107; of sixteen, which fill the lanes, 58).
+    // with a head a wave, fp32 92 and 207; of two 54 and 184, of four 59 and 107).
     while (2 * a.side * block <= kRound && a.side < a.heads) a.side *= 2;
-    if (a.side > 1) return launch_append<T, D, V, 1, 1>(a, q, with_q, s);
+    if (block <= kRound) return launch_append<T, D, V, 1, 1>(a, q, with_q, s);
+    // Fewer rounds of 16-bit rows take fewer registers (105 instead of 141; bf16 in blocks of sixteen 52 us and 58). fp32 rows do not.
+    if constexpr (sizeof(T) == 2)
+        if (block <= 2 * kRound) return launch_append<T, D, V, 1, 2>(a, q, with_q, s);
     if (block <= 4 * kRound) return launch_append<T, D, V, 1, 4>(a, q, with_q, s);
     if (block <= 16 * kRound) return launch_append<T, D, V, 4, 4>(a, q, with_q, s);
     return launch_append<T, D, V, 4, 0>(a, q, with_q, s);
