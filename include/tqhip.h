@@ -343,7 +343,9 @@ int tqhip_paged_attention8_plan(const tqhip_attn *attn, const tqhip_kv_cache8 *c
  * drafts were refused is shorter than it was) are put on the list of free pages and their table entries become -1, sequence by sequence,
  * in their order in the table; then the pages that sequences lack are taken off the end of the list, sequence by sequence. The first
  * sequence whose pages are not all there gets none, nor does any after it that lacks some, nor one that needs more than table_stride:
- * missing[b] says how many (0: all there), and such a sequence's new positions past its pages do not exist.
+ * missing[b] says how many (0: all there), and such a sequence's new positions past its pages do not exist: it is not ready for the call, its
+ * kv_len counts positions that are never written, and they must not become its past. tqhip_verify_tokens_dev sees to that where it is given `missing`; a
+ * caller that moves the lengths itself leaves the sequence at its old past, and gives it the same new tokens again when pages are free.
  * Written for the calls above: q_start, kv_len (past + n_new; may be past itself), and for every token its position and its slot
  * (page * page_size + row; -1 where it does not exist), both -1 for tokens past the last sequence's. The sum of n_new is at most n_tokens.
  * A new server starts with n_held of 0, tables of -1 and all pages on the list. Numbers that make no sense (negative lengths,
@@ -373,8 +375,9 @@ int tqhip_page_map_dev(const tqhip_page_map *map, void *stream);
  * out_tokens: from q_start[b] on the accepted drafts and the token drawn, n_out[b] in all, then -1. logprob: log p of each (T of 0: as of 1), then 0.
  * past: kv_len[b] less the refused drafts, the cached positions that stay. Logits of minus infinity have probability 0; a row with NaN or plus infinity, or
  * with nothing else, has no probabilities: as a target it ends its sequence with a token of -1, which n_out counts, as a draft it refuses,
- * and the draw is from p. Tokens of no sequence keep their outputs. out_tokens and logprob share nothing with
- * tokens and accept (refused). vocab up to 2^22.
+ * and the draw is from p. Tokens of no sequence keep their outputs. A sequence with missing[b] > 0 (as tqhip_page_map_dev says it) found no pages for all of
+ * its tokens, so its rows stand for nothing: its out_tokens are -1, logprob and n_out 0, and its past is what it was before the call, kv_len[b] less its
+ * tokens, which the next call is given again. out_tokens and logprob share nothing with tokens and accept, missing with no output (refused). vocab up to 2^22.
  * workspace: as for the attention, tqhip_verify_tokens_workspace() bytes. */
 typedef struct tqhip_verify {
     int dtype;                       /* of logits and draft: TQHIP_F32 / F16 / BF16 */
@@ -392,6 +395,7 @@ typedef struct tqhip_verify {
     float *logprob;                  /* device, [n_tokens], or NULL */
     void *workspace;
     size_t workspace_bytes;
+    const int *missing;              /* device, [n_seqs], or NULL: no sequence lacks pages */
 } tqhip_verify;
 int tqhip_verify_tokens_dev(const tqhip_verify *verify, void *stream);
 size_t tqhip_verify_tokens_workspace(const tqhip_verify *verify);

@@ -132,7 +132,7 @@ class Verify(ctypes.Structure):
     _fields_ = [(n, _i) for n in ("dtype", "n_seqs", "n_tokens", "vocab")] + [("logits", _vp), ("draft", _vp)] + \
                [("logits_stride", _i64), ("draft_stride", _i64)] + \
                [(n, _vp) for n in ("q_start", "tokens", "temperature", "accept", "pick", "kv_len", "past", "out_tokens", "n_out", "logprob",
-                                   "workspace")] + [("workspace_bytes", _sz)]
+                                   "workspace")] + [("workspace_bytes", _sz), ("missing", _vp)]
 
 
 def batch_op(kind: int, *structs) -> Op:
@@ -613,7 +613,7 @@ def page_map_dev(page_map: PageMap, stream=None) -> None:
 
 
 def verify_tokens_dev(verify: Verify, stream=None) -> None:
-    """Drafted tokens accepted or refused, and the token after them drawn, from given random numbers."""
+    """Drafted tokens accepted or refused, and the token after them drawn, from given random numbers; with `missing`, nothing for a request that lacks pages."""
     _check(lib().tqhip_verify_tokens_dev(verify, _stream(stream)), "tqhip_verify_tokens_dev")
 
 

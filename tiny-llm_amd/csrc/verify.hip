@@ -54,7 +54,7 @@ struct VerifyArgs {
     int64_t stride, draft_stride;
     const int *q_start, *tokens;
     const float *heat, *accept, *pick;
-    const int *kv_len;
+    const int *kv_len, *missing;
     int *past, *out, *n_out;
     float *logprob;
     int n_seqs, n_tokens, vocab, chunks;
@@ -251,11 +251,18 @@ __global__ __launch_bounds__(kRowThreads) void judge(VerifyArgs a) {
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = min(max(a.q_start[b], 0), a.n_tokens), n = min(max(a.q_start[b + 1], 0), a.n_tokens) - first;
-    if (n <= 0) {
-        if (chunk == 0 && tid == 0) {
-            a.n_out[b] = 0;
-            a.ends[b].kind = kNone;
-            if (a.past) a.past[b] = a.kv_len[b];
+    // (a sequence without all of its pages has rows over positions that do not exist: it says nothing, and keeps the length it had before the call)
+    if (n <= 0 || (a.missing && a.missing[b] > 0)) {
+        if (chunk == 0) {
+            for (int t = first + tid; t < first + n; t += kRowThreads) {
+                a.out[t] = -1;
+                if (a.logprob) a.logprob[t] = 0.0f;
+            }
+            if (tid == 0) {
+                a.n_out[b] = 0;
+                a.ends[b].kind = kNone;
+                if (a.past) a.past[b] = a.kv_len[b] - max(n, 0);
+            }
         }
         return;
     }
@@ -483,12 +490,15 @@ int check_verify(const tqhip_verify &p) {
     // (a launch has less than 2^32 threads along x)
     if (chunks * std::max(p.n_tokens, p.n_seqs) > INT32_MAX / kRowThreads || p.n_seqs > INT32_MAX / kDrawThreads) return kTooLarge;
     // a sequence's workgroups read its tokens and numbers while the first of them writes
-    const auto meet = [&](const void *in, const void *out) {
+    const auto meet = [](const void *in, int n_in, const void *out, int n_out) {
         const uintptr_t x = reinterpret_cast<uintptr_t>(in), y = reinterpret_cast<uintptr_t>(out);
-        return out && (x < y ? y - x : x - y) < 4 * static_cast<uintptr_t>(p.n_tokens);
+        return in && out && (x < y ? y - x < 4 * static_cast<uintptr_t>(n_in) : x - y < 4 * static_cast<uintptr_t>(n_out));
     };
     for (const void *in : {static_cast<const void *>(p.tokens), static_cast<const void *>(p.accept)})
-        if (meet(in, p.out_tokens) || meet(in, p.logprob)) return kBadShape;
+        if (meet(in, p.n_tokens, p.out_tokens, p.n_tokens) || meet(in, p.n_tokens, p.logprob, p.n_tokens)) return kBadShape;
+    for (const void *out : {static_cast<const void *>(p.out_tokens), static_cast<const void *>(p.logprob)})
+        if (meet(p.missing, p.n_seqs, out, p.n_tokens)) return kBadShape;
+    if (meet(p.missing, p.n_seqs, p.n_out, p.n_seqs) || meet(p.missing, p.n_seqs, p.past, p.n_seqs)) return kBadShape;
     return kOk;
 }
 
@@ -528,7 +538,7 @@ int run_verify(const tqhip_verify &p, hipStream_t s) {
     Part *parts = static_cast<Part *>(ws);
     End *ends = reinterpret_cast<End *>(parts + static_cast<size_t>(chunks) * p.n_tokens * (p.draft ? 2 : 1));
     const VerifyArgs a{p.logits, p.draft, p.logits_stride ? p.logits_stride : p.vocab, p.draft_stride ? p.draft_stride : p.vocab, p.q_start, p.tokens,
-                       p.temperature, p.accept, p.pick, p.kv_len, p.past, p.out_tokens, p.n_out, p.logprob, p.n_seqs, p.n_tokens, p.vocab, chunks,
+                       p.temperature, p.accept, p.pick, p.kv_len, p.missing, p.past, p.out_tokens, p.n_out, p.logprob, p.n_seqs, p.n_tokens, p.vocab, chunks,
                        parts, reinterpret_cast<double *>(ends + p.n_seqs), ends};
     if (p.dtype == TQHIP_F32)
         launch_verify<float>(a, few, s);
