@@ -267,7 +267,9 @@ int tqhip_kv_append_dev(const tqhip_head_proj *proj, const tqhip_kv_cache *cache
  *
  * workspace: NULL takes the stream's scratch (grown on demand like that of the other calls); a
  * caller that captures the call itself gives device memory of tqhip_paged_attention_workspace()
- * bytes, 256-byte aligned, which no other launch may use at the same time. */
+ * bytes, 256-byte aligned, which no other launch may use at the same time. (A call of fewer tokens may
+ * need more: its keys are cut into more parts. So ask for every call, and take the largest; the same
+ * goes for the adapters' workspace.) */
 typedef struct tqhip_attn {
     int dtype;                       /* of q and out */
     int n_heads;
@@ -378,7 +380,7 @@ int tqhip_page_map_dev(const tqhip_page_map *map, void *stream);
  * and the draw is from p. Tokens of no sequence keep their outputs. A sequence with missing[b] > 0 (as tqhip_page_map_dev says it) found no pages for all of
  * its tokens, so its rows stand for nothing: its out_tokens are -1, logprob and n_out 0, and its past is what it was before the call, kv_len[b] less its
  * tokens, which the next call is given again. out_tokens and logprob share nothing with tokens and accept, missing with no output (refused). vocab up to 2^22.
- * workspace: as for the attention, tqhip_verify_tokens_workspace() bytes. */
+ * workspace: as for the attention, tqhip_verify_tokens_workspace() bytes, which do for calls with fewer tokens, fewer sequences or no draft too. */
 typedef struct tqhip_verify {
     int dtype;                       /* of logits and draft: TQHIP_F32 / F16 / BF16 */
     int n_seqs, n_tokens, vocab;

@@ -1,4 +1,5 @@
-"""What the verification of drafts refuses of its `missing` argument, before anything is launched: no GPU is needed (and no call gets that far)."""
+"""What the verification of drafts refuses of its `missing` argument, before anything is launched, and the workspace that it asks for: no GPU is needed (and
+no call gets that far)."""
 import pytest
 
 F32 = 0
@@ -19,3 +20,19 @@ def test_missing_over_an_output_is_refused(tqa, at):
 @pytest.mark.parametrize("at", [None, 5 * AT, 2 * AT - 8, 2 * AT + 30 * 4, 3 * AT + 8, 4 * AT - 8, AT + 8])
 def test_missing_beside_the_outputs_is_not(tqa, at):
     assert verify(tqa, missing=at) == -7  # (the workspace is too small, which is looked at last)
+
+
+@pytest.mark.parametrize("vocab", [1, 999, 4096, 4097, 9001, 24576, 24577, 98304, 100001, 151936])
+@pytest.mark.parametrize("draft", [AT, None])
+def test_one_workspace_for_smaller_calls(tqa, vocab, draft):
+    """Short chunks give way to long ones as rows grow (from 98304 logits a CU on): a workspace for some tokens and sequences does for fewer, and
+    for those without a draft."""
+    def need(tokens, seqs, draft=draft):
+        return tqa.verify_tokens_workspace(tqa.Verify(dtype=F32, n_seqs=seqs, n_tokens=tokens, vocab=vocab, logits=AT, draft=draft, q_start=AT, tokens=AT,
+                                                      accept=AT, pick=AT, out_tokens=2 * AT, n_out=3 * AT))
+
+    tokens = sorted({1, 2, 3, 5, 11, 12, 13, 23, 24, 25, 26, 97, 98, 99, 196, 197, 198, 500, 4000})
+    for seqs in (1, 7, 600):
+        rooms = [need(n, seqs) for n in tokens]
+        assert rooms == sorted(rooms) and rooms[0] > 0
+        assert all(need(n, max(1, seqs // 2)) <= r and need(n, seqs, None) <= r for n, r in zip(tokens, rooms))

@@ -470,9 +470,9 @@ __global__ __launch_bounds__(kDrawThreads) void draw(VerifyArgs a) {
 // Long chunks spread a workgroup's search, sums and barriers over more logits; short ones spread few rows over more of the
 // card. Up to 12 long ones a CU, of 151936 fp32 logits with drafts' rows: one request 17 us short and 20 long, 8 28 and 31, 16 38 and 41, 32 63 and 63, 64 112
 // and 105 (64 without drafts 28 and 27).
-bool few_rows(const tqhip_verify &p) {
-    return static_cast<int64_t>(p.n_tokens) * (p.draft ? 2 : 1) * p.vocab <= int64_t{12} * device_cu_count() * kChunk<kManyPerThread>;
-}
+int64_t rows_of(const tqhip_verify &p) { return static_cast<int64_t>(p.n_tokens) * (p.draft ? 2 : 1); }
+int64_t most_few_rows(const tqhip_verify &p) { return int64_t{12} * device_cu_count() * kChunk<kManyPerThread> / p.vocab; }
+bool few_rows(const tqhip_verify &p) { return rows_of(p) <= most_few_rows(p); }
 int chunks_of(const tqhip_verify &p) {
     const int chunk = few_rows(p) ? kChunk<kFewPerThread> : kChunk<kManyPerThread>;
     return (p.vocab + chunk - 1) / chunk;
@@ -502,9 +502,12 @@ int check_verify(const tqhip_verify &p) {
     return kOk;
 }
 
-size_t verify_bytes(const tqhip_verify &p) {
-    const size_t chunks = chunks_of(p);
-    return chunks * p.n_tokens * sizeof(Part) * (p.draft ? 2 : 1) + p.n_seqs * (sizeof(End) + chunks * sizeof(double));
+size_t part_bytes(int64_t rows, int n_seqs, size_t chunks) { return chunks * rows * sizeof(Part) + n_seqs * (sizeof(End) + chunks * sizeof(double)); }
+size_t verify_bytes(const tqhip_verify &p) { return part_bytes(rows_of(p), p.n_seqs, chunks_of(p)); }
+// What this call and every smaller one takes: short chunks are more of them, so the largest call of few rows may take more than one that is larger yet.
+size_t verify_room(const tqhip_verify &p) {
+    const size_t few_chunks = (p.vocab + kChunk<kFewPerThread> - 1) / kChunk<kFewPerThread>;
+    return std::max(verify_bytes(p), part_bytes(std::min(rows_of(p), most_few_rows(p)), p.n_seqs, few_chunks));
 }
 
 template <typename T, int PER>
@@ -564,7 +567,7 @@ int tqhip_verify_tokens_dev(const tqhip_verify *verify, void *stream) {
 }
 
 size_t tqhip_verify_tokens_workspace(const tqhip_verify *verify) {
-    return verify && tqhip::check_verify(*verify) == tqhip::kOk ? tqhip::verify_bytes(*verify) : 0;
+    return verify && tqhip::check_verify(*verify) == tqhip::kOk ? tqhip::verify_room(*verify) : 0;
 }
 
 }  // extern "C"
