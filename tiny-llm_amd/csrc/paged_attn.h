@@ -341,9 +341,8 @@ __device__ inline void formula_row(const AttnArgs &a, int b, int row, int token0
             load_as_float<T, 8>(q + d, x);
             load_stored<C, 8>(kc + max(o, int64_t{0}) + d, y);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += static_cast<double>(x[e]) * y[e];
+            for (int e = 0; e < 8; ++e) s += static_cast<double>(x[e]) * (kCodes<C> ? static_cast<double>(y[e]) * by : static_cast<double>(y[e]));
         }
-        if constexpr (kCodes<C>) s *= by;
         return o < 0 ? static_cast<double>(-INFINITY) : s * c;
     };
     float2 by;

@@ -77,6 +77,10 @@ __device__ inline float relative_scale(float scale, float per_unit, float &log) 
     return scale == 0.0f || fabsf(x) <= 100.0f ? b : NAN;
 }
 
+// A key's scale as the factor of its score. A product of codes times an infinity would be an infinity of its own sign, where elements of either sign
+// make no number; and what load_query's least factor and fp32 leave room for are scales of up to 2^60. One past that makes its rows NaN, so the formula takes them.
+__device__ inline float key_scale(float scale) { return fabsf(scale) <= 0x1p60f ? scale : NAN; }
+
 // x as it is rounded to fp32, for split: a product whose fp16 form is taken twice, as the first term and to find the rest, must not be rounded
 // to fp16 from its exact value once and from its fp32 one the other time (the compiler has an instruction for the former; the terms
 // then miss each other by a step of fp16 where the two roundings fall to different sides, one weight in some 10^4).
@@ -230,7 +234,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
         if (g < 2) {
             const float2 x = g == 0 ? by[0] : by[1];
             float log;
-            sh.by[wave][kScaleA][16 * g + col] = x.x;
+            sh.by[wave][kScaleA][16 * g + col] = key_scale(x.x);
             sh.by[wave][kScaleB][16 * g + col] = relative_scale(x.y, per_unit, log);
             sh.by[wave][kScaleLog][16 * g + col] = log;
         }
@@ -520,7 +524,7 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
         }
         if (tid < BN) {
             float log;
-            sh.by[buf][kScaleA][tid] = by.x;
+            sh.by[buf][kScaleA][tid] = key_scale(by.x);
             sh.by[buf][kScaleB][tid] = relative_scale(by.y, per_unit, log);
             sh.by[buf][kScaleLog][tid] = log;
         }
