@@ -263,7 +263,8 @@ int tqhip_kv_append_dev(const tqhip_head_proj *proj, const tqhip_kv_cache *cache
  * never used, whatever they hold (NaN and infinities too). Infinities and NaN among those attended
  * to go through the formula: a score of minus infinity is a weight of 0, and a key of weight 0 does
  * not count whatever its value (where all are, the row gets zeros); a score of NaN or plus infinity makes
- * the row NaN; an infinite value reaches its own dimension. Such rows take longer.
+ * the row NaN; an infinite value reaches its own dimension. Such rows take longer. Finite scores are
+ * numbers of fp32: those past 3.4e38 are not told apart.
  *
  * workspace: NULL takes the stream's scratch (grown on demand like that of the other calls); a
  * caller that captures the call itself gives device memory of tqhip_paged_attention_workspace()

@@ -62,3 +62,30 @@ def test_large_scales_of_keys_with_small_queries(gpu, new, kv, Hq, Hk, dtype, ac
     b.scales[..., 0] *= np.float32(2.0 ** power)
     b.put()
     attention.check(gpu, b, act, Hq, scale=0.125, q_std=1.5 * 2.0 ** -power)
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("act", [F32, BF16])
+def test_scores_below_zero_of_large_queries(gpu, new, kv, Hq, Hk, act):
+    """Queries times the scale pass fp32, and keys bring the scores back to some -10^28, all of them below zero: the largest takes it all (unless fp32, in which
+    the parts of a row compare theirs, may not tell it from the next)."""
+    b = Batch8(gpu, new, kv, 16, Hk, 64, I8, 16, seed=73)
+    b.codes[0] = np.maximum(b.codes[0] & 0x7f, 0x10)  # positive, of 16 at least
+    b.scales[..., 0] = 2.0 ** -60
+    b.put()
+    q = Dev(gpu, -1e36 * (0.5 + np.abs(b.rng.standard_normal((b.tokens, Hq, 64)))), act)
+    scale = float(np.float32(1e7))
+    got = attend(gpu, b, q, act, Hq, scale)
+    want, spread, _, _ = ref.attention(b, q.values, scale, 1, 0)
+    bound = 2 * U * spread + HALF[act] * np.abs(want) + TINY[act]  # (one value, times its scale, rounded)
+    keys, decided = b.k.values, 0
+    for t, (s, pos) in b.token_positions().items():
+        if pos < 0:
+            continue
+        pg, r = np.array([b.place(s, p) for p in range(pos + 1)]).T
+        for h in range(Hq):
+            z = np.sort(keys[pg, r, h // (Hq // Hk)] @ q.values[t, h])
+            if pos == 0 or z[-1] - z[-2] > 2.0 ** -22 * abs(z[-1]):
+                decided += 1
+                assert np.all(np.abs(got[t, h] - want[t, h]) <= bound[t, h]), (t, h)
+    assert decided > 0.9 * b.tokens * Hq

@@ -80,6 +80,9 @@ __device__ inline float relative_scale(float scale, float per_unit, float &log) 
 // A key's scale as the factor of its score. A product of codes times an infinity would be an infinity of its own sign, where elements of either sign
 // make no number; and what load_query's least factor and fp32 leave room for are scales of up to 2^60. One past that makes its rows NaN, so the formula takes them.
 __device__ inline float key_scale(float scale) { return fabsf(scale) <= 0x1p60f ? scale : NAN; }
+// A row of queries so large that its products times its factor pass fp32, or the factor alone, whatever the keys' scales make of them, may have had nothing but minus
+// infinities: its sum of 0 says nothing then, and the formula takes it. (Products of queries and codes stay below 2^34, scales below 2^60.)
+__device__ inline bool may_overflow(float c) { return c > 0x1p30f; }
 
 // x as it is rounded to fp32, for split: a product whose fp16 form is taken twice, as the first term and to find the rest, must not be rounded
 // to fp16 from its exact value once and from its fp32 one the other time (the compiler has an instruction for the former; the terms
@@ -346,6 +349,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
         l[r] += lane_xor<16>(l[r], lane);
         l[r] += lane_xor<32>(l[r], lane);
         l[r] = checked_sum<f16>(bias[r], l[r]);
+        if (l[r] == 0.0f && may_overflow(c[r])) l[r] = NAN;
         if (g == 0) {
             sh.meet[0][wave][kFewRows * r + col] = bias[r];
             sh.meet[1][wave][kFewRows * r + col] = l[r];
@@ -693,6 +697,7 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
         if (k0 + 2 * BN < ke) load_tile(n + 2);
     }
     l = checked_sum<f16>(bias, l + lane_xor<32>(l, lane));
+    if (l == 0.0f && may_overflow(c)) l = NAN;
     float z = l * 0.0f;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
