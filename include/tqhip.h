@@ -334,7 +334,7 @@ typedef struct tqhip_kv_cache8 {
 int tqhip_kv_append8_dev(const tqhip_head_proj *proj, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, void *stream);
 
 /* tqhip_paged_attention_dev over such a cache, with activations of any of the three types; the codes enter as they are and the scales in fp32.
- * With f16 / bf16 activations softmax weights, times their value's scale, are rounded to fp16; with f32 they keep 22 bits, or 2^-39 of the row's largest
+ * With bf16 activations softmax weights, times their value's scale, are rounded to fp16; with f16 and f32 they keep 22 bits, or 2^-39 of the row's largest
  * such product where that is more. What is said there of infinities and NaN holds for elements: codes times scales. */
 int tqhip_paged_attention8_dev(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs, void *stream);
 size_t tqhip_paged_attention8_workspace(const tqhip_attn *attn, const tqhip_kv_cache8 *cache, const tqhip_seqs *seqs);

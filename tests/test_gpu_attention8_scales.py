@@ -89,3 +89,18 @@ def test_scores_below_zero_of_large_queries(gpu, new, kv, Hq, Hk, act):
                 decided += 1
                 assert np.all(np.abs(got[t, h] - want[t, h]) <= bound[t, h]), (t, h)
     assert decided > 0.9 * b.tokens * Hq
+
+
+@pytest.mark.parametrize("new,kv,Hq,Hk", FORMS)
+@pytest.mark.parametrize("dtype", [I8, E4M3])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_f16_rows_are_off_by_their_results_rounding(gpu, new, kv, Hq, Hk, dtype, D):
+    """Within fp32's tolerance of the formula before the result is rounded to f16, half a step: no rounding of the weights shows."""
+    b = Batch8(gpu, new, kv, 16, Hk, D, dtype, 8, seed=74)
+    q = Dev(gpu, 1.5 * b.rng.standard_normal((b.tokens, Hq, D)), F16)
+    got = attend(gpu, b, q, F16, Hq, D ** -0.5)
+    want, spread, score, _ = ref.attention(b, q.values, float(np.float32(D ** -0.5)), 1, 0)
+    before = bound_of(b, F32, want, spread, score)
+    assert np.all(np.abs(got - want) <= before + HALF[F16] * (np.abs(want) + before) + TINY[F16])
+    rounded = want.astype(np.float16).astype(np.float64)
+    assert np.linalg.norm(got - want) <= np.linalg.norm(rounded - want) + 2.0 ** -17 * np.linalg.norm(want)

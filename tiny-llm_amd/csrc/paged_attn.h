@@ -84,14 +84,20 @@ __device__ inline float2 row_scales(const AttnArgs &a, int page, int kvh, int p)
 // or a weight, KT of a cache element. 16-bit activations meet a cache of their own type as they are.
 // fp32 activations keep their precision: against an fp16 cache two fp16 terms (22 bits), against
 // a bf16 one three bf16 terms (24 bits), and an fp32 cache is three bf16 terms itself. Codes of 8 bits are fp16 numbers without
-// rounding, and activations of 16 bits meet them as one fp16 term: bf16's 8 bits fit, and a row's power of two keeps its range.
-// (One term rounds the weights too, once more than the result: bf16 prompts are 2.1e-3 from 64 bits, where the result's
+// rounding, and queries of 16 bits meet them as one fp16 term: bf16's 8 bits fit, and a row's power of two keeps its range. (One term
+// rounds the weights too, once more than the result: bf16 prompts over a bf16 cache are 2.1e-3 from 64 bits, where the result's
 // rounding alone is 1.6e-3. A second term would be half as many products again, for bits that the result does not keep.)
+// Over codes a bf16 row's weights are one fp16 term as well: 1.67e-3 from 64 bits in all, 1.66e-3 with the result's rounding alone. An f16
+// result does show it: 2.3e-4 to 2.7e-4, 2.0e-4 to 2.1e-4 without. So f16 rows get a second term of their weights, and are off by their result's
+// rounding. It costs 1 % of a step of single tokens (64 over up to 16000 keys 214 us, 212 with one term), 4 % of drafted ones (94.5, 91), 16 % of
+// chunks (201, 173), 23 % of prompts (two of up to 8192: 1281, 1041).
 template <typename T, typename C>
 struct Terms {
     using E = std::conditional_t<std::is_same_v<C, f16> || kCodes<C>, f16, bf16>;
     static constexpr int KT = std::is_same_v<C, float> ? 3 : 1;
     static constexpr int QT = !std::is_same_v<T, float> ? 1 : std::is_same_v<E, f16> ? 2 : 3;
+    // terms of a weight times its value's scale, over codes
+    static constexpr int WT = std::is_same_v<T, f16> ? 2 : QT;
     // products of term i and term j are kept while i + j < max(QT, KT): the next ones are below 2^-24
     static constexpr int kMost = QT > KT ? QT : KT;
 };

@@ -7,6 +7,8 @@
 // running maximum that sets the bias is that of c a_j q.x_j + log2 b_j, and b is taken relative to a power of two near the first
 // block's, which the sums get back at the end. Rows that this does not hold (infinities, NaN, scales 2^100 apart) are done by the formula.
 //
+// Weights times scales are two fp16 terms where the result shows more than one (see Terms).
+//
 // The cut into tiles of 16, 32 and 128 rows, the parts and their join are those of the other caches (paged_attn.h, paged_attn.hip).
 // Few rows are bound by HBM: a key and a value of D bytes and their scales, read once for the rows of a K/V head. Many rows are bound by
 // the vector units, which make fp16 of the codes and weights of the scores while the matrix units wait (busy 31 % and 45 % of the time).
@@ -101,7 +103,7 @@ constexpr int kScaleA = 0, kScaleLog = 1, kScaleB = 2;
 // two products), V into LDS as it is and out of it by transposing reads of bytes.
 template <typename T, typename C, int D, int R>
 __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a) {
-    constexpr int QT = Terms<T, C>::QT;
+    constexpr int QT = Terms<T, C>::QT, WT = Terms<T, C>::WT;
     constexpr int kRows = R * kFewRows;
     constexpr int ND = D / 16, NS = D / 32, NL = D / 64, CH = D / 16, NV = kFewKeys * CH / 64;
     __shared__ struct {
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
         const auto by_of = [&](int what, int kt) { return *reinterpret_cast<const f32x4 *>(&sh.by[wave][what][16 * kt + 4 * g]); };
         const f32x4 sa[2] = {by_of(kScaleA, 0), by_of(kScaleA, 1)}, lg[2] = {by_of(kScaleLog, 0), by_of(kScaleLog, 1)},
                     b[2] = {by_of(kScaleB, 0), by_of(kScaleB, 1)};
-        vec<f16, 8> p[R][QT];
+        vec<f16, 8> p[R][WT];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             unsigned may = ~0u;
@@ -282,8 +284,8 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
             for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fmaf(s[r][e / 4][e % 4], c[r], lg[e / 4][e % 4]));
             mx = fmaxf(mx, lane_xor<16>(mx, lane));
             mx = fmaxf(mx, lane_xor<32>(mx, lane));
-            if (__ballot(mx - m[r] > kHeadroom<QT>)) {
-                const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, QT> - mx;
+            if (__ballot(mx - m[r] > kHeadroom<WT>)) {
+                const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, WT> - mx;
                 const float f = m[r] == -INFINITY ? 0.0f : exp2f(nb - bias[r]);
                 m[r] = mx;
                 bias[r] = nb;
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
                 for (int e = 0; e < 8; ++e)
                     if (!(may & (1u << (16 * (e / 4) + e % 4)))) w[e] = 0.0f;
             }
-            split<f16, QT>(w, p[r]);
+            split<f16, WT>(w, p[r]);
         }
         if constexpr (std::is_same_v<C, e4m3>) {
             if (partial) {  // NaN codes as the infinite and NaN values of attn_tiles
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void attn8_few(AttnArgs a)
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int qi = 0; qi < QT; ++qi) acc[r][d] = mfma16(vf, p[r][qi], acc[r][d]);
+                for (int wi = 0; wi < WT; ++wi) acc[r][d] = mfma16(vf, p[r][wi], acc[r][d]);
         }
         k0 += kFewStep;
     };
@@ -431,7 +433,7 @@ struct TileShape8 {
 
 template <typename T, typename C, int D>
 __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void attn8_tiles(AttnArgs a) {
-    constexpr int QT = Terms<T, C>::QT, BN = TileShape8<T, C, D>::BN;
+    constexpr int QT = Terms<T, C>::QT, WT = Terms<T, C>::WT, BN = TileShape8<T, C, D>::BN;
     constexpr int CH = D / 16, NCH = BN * CH / 256;  // chunks of 16 codes a row, and a thread
     constexpr int NK = BN / 32, ND = D / 32, kTiles = 256 / BN;
     __shared__ struct {
@@ -623,8 +625,8 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
                 }
             }
             mx = fmaxf(m, fmaxf(mx, lane_xor<32>(mx, lane)));
-            if (__ballot(mx - m > kHeadroom<QT>)) {
-                const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, QT> - mx;
+            if (__ballot(mx - m > kHeadroom<WT>)) {
+                const float nb = mx == -INFINITY ? 0.0f : kWeightShift<f16, WT> - mx;
                 const float f = m == -INFINITY ? 0.0f : exp2f(nb - bias);
                 m = mx;
                 bias = nb;
@@ -662,10 +664,10 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 float x[8];
-                vec<f16, 8> p[QT];
+                vec<f16, 8> p[WT];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = s[8 * half + e];
-                split<f16, QT>(x, p);
+                split<f16, WT>(x, p);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const int i = lane & 15, row = 32 * kt + 16 * half + 4 * h + i / 4;
@@ -673,7 +675,7 @@ __global__ __launch_bounds__(256, (TileShape8<T, C, D>::kWavesPerSimd)) void att
                     const vec<f16, 4> a0 = lds_columns(v0), a1 = lds_columns(v0 + 8 * D);
                     const vec<f16, 8> vf = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                    for (int qi = 0; qi < QT; ++qi) acc[d] = mfma32(vf, p[qi], acc[d]);
+                    for (int wi = 0; wi < WT; ++wi) acc[d] = mfma32(vf, p[wi], acc[d]);
                 }
             }
             s = ahead;
