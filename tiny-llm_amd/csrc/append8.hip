@@ -10,7 +10,8 @@
 // fit (32, 16 or 8 fp32 rows of 64, 128 or 256); a larger block is a workgroup's, and one past four times that is read twice. Of blocks of
 // few rows it takes several heads side by side.
 // Bytes moved are the bound of a long batch, latency (sequence, page, rows, the block's scale) that of a short one. 12520 tokens of 14 + 2 + 2
-// heads of 64, 106 MB: 23 to 26 us, 4.1 to 4.6 TB/s, a copy's rate; 61 single tokens: 7 to 8.5 us, 14 of the caller's.
+// heads of 64, 106 MB: 23 to 26 us, 4.1 to 4.6 TB/s, a copy's rate; 61 single tokens: 11 us where two blocks in five get a larger scale, or all of them, and
+// the older rows' codes are read and written again; 7 to 8.5 where none does.
 // The queries that ride along are the same launch's, finished as heads.h does it (a launch of their own where something is off the vector path).
 #include <algorithm>
 #include <cmath>

@@ -493,8 +493,11 @@ inline Plan plan(const tqhip_attn &p, const tqhip_kv_cache &c, const tqhip_seqs 
     // as there are few of them in all, because there they come in shorter parts (one sequence of 64 rows on 8 K/V heads 22 us and 32,
     // 128 rows 34 and 34; 448 rows on 2 heads of 64 30 and 41, 1792 rows 79 and 47; 1024 on one of 256 52 and 81).
     // Codes of 8 bits win there for twice the rows, of a sequence (32 sequences of up to 9000 keys, 32 heads of 128 over 8: 45 rows of
-    // bf16 154 us, against 180 with tiles of 128; 35 of fp32 170 and 237; but 87 of fp32 342 and 268) and in all (one of 512 rows on 8
-    // heads of 128 24.9 and 31.3; 2400 on one of 256 54 and 76).
+    // bf16 154 us, against 180 with tiles of 128; 35 of fp32 170 and 237; but 87 of fp32 342 and 268), and for twice as many tiles in all.
+    // There the two cross at 256 to 384 rows on each of 8 heads of 128 (over 4000 keys; 224 rows bf16 32 us and 32, fp32 37 and 41; 256 rows 32 and 33, 39
+    // and 41; 384 rows 44 and 34, 53 and 43), past the rule on two of 64 (896 rows 23 and 28, 25 and 33; 1792 rows 29 and 33, 32 and 38; 3584 rows
+    // 46 and 44, 52 and 52), and on one of 256 before it in bf16 and past it in fp32 (1200 rows 59 and 53, 50 and 79; 1792 rows 68 and 56, 59 and 81;
+    // 2400 rows 75 and 58, 69 and 84).
     const int more = codes ? 2 : 1;
     n.few = rows <= int64_t{2 * more} * kFewRows * s.n_seqs || (rows + kFewRows - 1) / kFewRows * c.n_kv_heads <= 56 * more;
     // Over codes, 32 rows a tile where sequences have more than 16, so that their keys are read once: five tokens each of 32 sequences of

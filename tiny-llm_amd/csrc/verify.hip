@@ -12,7 +12,7 @@
 // Reading the rows once and an exponential for each logit are the work. Three launches:
 //   row_sums  maximum, sum of exponentials and argmax of every chunk of every row;
 //   judge     a sequence's chunks each join the sums of its rows, find the row that ends it, and sum their part of that row's r
-//             (the row is read a second time, from L2);
+//             (the row is read a second time, and comes from behind the L2s again: of many requests more has passed them since than they hold);
 //   draw      the chunk and then the token that the draw falls into.
 // 64 requests with up to 4 drafts and their model's rows, 151936 fp32 logits (316 MB): 73, 24 and 10 us
 // 100 requests with up to 7 drafts of no model, bf16 logits (215 MB, 107 million exponentials): 96, 13 and 9
